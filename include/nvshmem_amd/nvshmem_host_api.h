@@ -341,6 +341,71 @@ NVSHMEMI_REPT_FOR_ALL_REDUCE_TYPES_AND_OPS(NVSHMEMI_DECL_TYPED_REDUCE_HOST)
 #undef NVSHMEMI_DECL_TYPED_REDUCE_HOST
 
 /*
+ * Operators on rows of tokens (no counterpart in the reference): what stands in front of and behind the token shuffle of
+ * nvshmem_perftest.h in a model with experts.  As with the collectives, one call serves all PEs: every operand is a canonical
+ * symmetric address, PE p works on its own copy, and work is enqueued on `stream` and not waited for.  Outputs must not overlap
+ * other operands.  Each call returns 0 or an nvshmemx_status (nvshmemx_amd_last_error() has the text); nothing is enqueued by a
+ * call that is refused.  No call allocates, and all of them can be captured into a graph; calls that can run at the same time
+ * need workspaces of their own.  Workspaces are symmetric memory of the size that the functions named *_workspace give (bytes
+ * per PE, 0 before nvshmem_init), aligned to 64 bytes, with nothing to initialise.  Arithmetic is in fp32 and results are
+ * rounded once; every sum has a fixed order, so that equal inputs give equal bits.
+ *
+ * <T>_embedding: out[t] = scale * row ids[t] of a table of `vocab` rows that is cut over the PEs: with R = ceil(vocab / npes),
+ *   row v is row v % R of PE v / R's copy of `table` (R rows of dim elements on each).  An id outside [0, vocab) is padding and
+ *   gives a row of zeros.
+ * <T>_embedding_grad: the table's gradient, cut the same way: row v becomes scale * the sum of dout[t] over all tokens of all PEs
+ *   with ids[t] = v, added up in the order of (PE, t), and zeros where no token names it.  Rows that a PE holds
+ *   behind the vocabulary are left as they were.
+ *
+ * <T>_moe_route: for every token the `topk` (at most 16) largest of `experts` (at most 1024) logits, larger ones first, ties
+ *   to the lowest expert.  A logit of -inf or NaN masks an expert out: where fewer are left than topk, expert is -1 and gate 0.
+ *   gate = scale * softmax(logits)[expert], divided by the sum of the token's chosen ones if `normalise`.
+ *   counts[e] = copies that the PE sends to expert e.  With loss and balance (both or neither): over the tokens of all PEs,
+ *   with c_e copies to expert e, C = sum of c_e, N tokens that have an expert, and p = softmax(logits),
+ *   loss[0] = experts / (C N) * sum over e and t of c_e p[t, e], and balance[e] = experts c_e / (C N), its derivative by p[t, e];
+ *   every PE gets both.
+ * <T>_moe_route_grad: dlogits from dgate, the gates' upstream gradient, and - with dloss and balance, both or neither - from
+ *   dloss[0], the loss's (each PE takes its own copy).  `expert` is moe_route's; the counts are constants.  Masked logits get 0.
+ * moe_place: the shuffle's tables from moe_route's expert and counts: copy k of token t goes to PE dest_pe[t * topk + k], the one
+ *   that owns its expert (experts / npes consecutive ones each), at row dest_row; rows lie there in the order (expert,
+ *   source PE, t, k).  Copies without an expert and those for which a PE's recv_cap_rows have no room get -1 and -1, which
+ *   dispatch and combine skip.  expected[src]: rows that arrive here from PE src, what the dispatch waits for.
+ *   expert_row[i], i = 0..experts / npes: the first row of the i-th of this PE's experts, and the end of the last.
+ * <T>_moe_combine_sum: out[t] = sum over k of gate[t * topk + k] * row dest_row of PE dest_pe's recv (gate NULL: ones).  A copy
+ *   outside [0, npes) x [0, recv_cap_rows) adds nothing.  Without gates it is the gradient of the dispatch as well.
+ * <T>_moe_combine_grad: drecv@dest_pe[dest_row] = gate * dout[t] and dgate = <dout[t], that row of recv>, 0 for a copy that was
+ *   skipped.  Rows of drecv that no copy names are left as they were; drecv may be recv.  No two copies may name one row.
+ */
+#define NVSHMEMI_AMD_DECL_TOKENS(NAME, TYPE)                                                                              \
+    NVSHMEMI_HOST_ONLY int nvshmemx_amd_##NAME##_embedding_on_stream(                                                     \
+        TYPE *out, const TYPE *table, const int64_t *ids, size_t tokens, size_t vocab, size_t dim, float scale,           \
+        nvshmemx_stream_t stream);                                                                                        \
+    NVSHMEMI_HOST_ONLY int nvshmemx_amd_##NAME##_embedding_grad_on_stream(                                                \
+        TYPE *dtable, const TYPE *dout, const int64_t *ids, void *workspace, size_t tokens, size_t vocab, size_t dim,     \
+        float scale, nvshmemx_stream_t stream);                                                                           \
+    NVSHMEMI_HOST_ONLY int nvshmemx_amd_##NAME##_moe_route_on_stream(                                                     \
+        int32_t *expert, float *gate, int64_t *counts, float *loss, float *balance, void *workspace, const TYPE *logits,  \
+        size_t tokens, int experts, int topk, int normalise, float scale, nvshmemx_stream_t stream);                      \
+    NVSHMEMI_HOST_ONLY int nvshmemx_amd_##NAME##_moe_route_grad_on_stream(                                                \
+        TYPE *dlogits, const TYPE *logits, const int32_t *expert, const float *dgate, const float *balance,               \
+        const float *dloss, size_t tokens, int experts, int topk, int normalise, float scale, nvshmemx_stream_t stream);  \
+    NVSHMEMI_HOST_ONLY int nvshmemx_amd_##NAME##_moe_combine_sum_on_stream(                                               \
+        TYPE *out, const TYPE *recv, size_t recv_cap_rows, const float *gate, const int32_t *dest_pe,                     \
+        const int64_t *dest_row, size_t tokens, int topk, size_t dim, nvshmemx_stream_t stream);                          \
+    NVSHMEMI_HOST_ONLY int nvshmemx_amd_##NAME##_moe_combine_grad_on_stream(                                              \
+        TYPE *drecv, float *dgate, const TYPE *dout, const TYPE *recv, size_t recv_cap_rows, const float *gate,           \
+        const int32_t *dest_pe, const int64_t *dest_row, size_t tokens, int topk, size_t dim, nvshmemx_stream_t stream);
+NVSHMEMI_AMD_REPT_FOR_TOKEN_TYPES(NVSHMEMI_AMD_DECL_TOKENS)
+#undef NVSHMEMI_AMD_DECL_TOKENS
+NVSHMEMI_HOST_ONLY int nvshmemx_amd_moe_place_on_stream(int32_t *dest_pe, int64_t *dest_row, uint64_t *expected,
+                                                        int64_t *expert_row, void *workspace, const int32_t *expert,
+                                                        const int64_t *counts, size_t tokens, int topk, int experts,
+                                                        size_t recv_cap_rows, nvshmemx_stream_t stream);
+NVSHMEMI_HOST_ONLY size_t nvshmemx_amd_embedding_grad_workspace(size_t tokens, size_t vocab, size_t dim);
+NVSHMEMI_HOST_ONLY size_t nvshmemx_amd_moe_route_workspace(size_t tokens, int experts);
+NVSHMEMI_HOST_ONLY size_t nvshmemx_amd_moe_place_workspace(size_t tokens, int topk, int experts);
+
+/*
  * Cooperative launch of a kernel that uses the device API (reference
  * src/device/launch/collective_launch.cpp:209-212).  One launch carries every logical PE:
  * the grid's z extent is set to npes (the caller's grid z must be 1) and a block acts as PE

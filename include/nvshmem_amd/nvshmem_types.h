@@ -24,6 +24,12 @@ typedef struct { uint16_t bits; } nvshmem_bfloat16_t;
 typedef struct { uint16_t bits; } nvshmem_half_t;
 #endif
 
+/* Element types of the operators on rows of tokens. */
+#define NVSHMEMI_AMD_REPT_FOR_TOKEN_TYPES(X) \
+    X(float, float)                          \
+    X(half, nvshmem_half_t)                  \
+    X(bfloat16, nvshmem_bfloat16_t)
+
 /* 25 standard RMA types. */
 #define NVSHMEMI_REPT_FOR_STANDARD_RMA_TYPES(X) \
     X(bfloat16, nvshmem_bfloat16_t, bf16)       \

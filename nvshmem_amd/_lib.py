@@ -27,6 +27,7 @@ def _open(name):
     return lib
 
 
+TOKEN_TYPES = ("float", "half", "bfloat16")     # element types of the operators on rows of tokens
 vp, sz, u64, i32 = C.c_void_p, C.c_size_t, C.c_uint64, C.c_int
 
 
@@ -108,6 +109,22 @@ def load():
         "nvshmemi_amd_mspace_free_bytes": (u64, [vp]),
         "nvshmemi_amd_mspace_free_chunks": (u64, [vp]),
     }
+    f32 = C.c_float
+    for t in TOKEN_TYPES:
+        sig.update({
+            "nvshmemx_amd_%s_embedding_on_stream" % t: (i32, [vp, vp, vp, sz, sz, sz, f32, vp]),
+            "nvshmemx_amd_%s_embedding_grad_on_stream" % t: (i32, [vp, vp, vp, vp, sz, sz, sz, f32, vp]),
+            "nvshmemx_amd_%s_moe_route_on_stream" % t: (i32, [vp] * 7 + [sz, i32, i32, i32, f32, vp]),
+            "nvshmemx_amd_%s_moe_route_grad_on_stream" % t: (i32, [vp] * 6 + [sz, i32, i32, i32, f32, vp]),
+            "nvshmemx_amd_%s_moe_combine_sum_on_stream" % t: (i32, [vp, vp, sz, vp, vp, vp, sz, i32, sz, vp]),
+            "nvshmemx_amd_%s_moe_combine_grad_on_stream" % t: (i32, [vp, vp, vp, vp, sz, vp, vp, vp, sz, i32, sz, vp]),
+        })
+    sig.update({
+        "nvshmemx_amd_moe_place_on_stream": (i32, [vp] * 7 + [sz, i32, i32, sz, vp]),
+        "nvshmemx_amd_embedding_grad_workspace": (sz, [sz, sz, sz]),
+        "nvshmemx_amd_moe_route_workspace": (sz, [sz, i32]),
+        "nvshmemx_amd_moe_place_workspace": (sz, [sz, i32, i32]),
+    })
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
         fn.restype, fn.argtypes = res, args
@@ -249,6 +266,8 @@ def declared_symbols(header_paths=None):
             names.update({"nvshmem_%s_%s_reduce" % (t, op), "nvshmemx_%s_%s_reduce_on_stream" % (t, op),
                           "nvshmem_%s_%s_reducescatter" % (t, op),
                           "nvshmemx_%s_%s_reducescatter_on_stream" % (t, op)})
+    for op in ("embedding", "embedding_grad", "moe_route", "moe_route_grad", "moe_combine_sum", "moe_combine_grad"):
+        names.update("nvshmemx_amd_%s_%s_on_stream" % (t, op) for t in TOKEN_TYPES)
     perf = open(os.path.join(INCLUDE, "nvshmem_perftest.h")).read()
     perf_names = set(re.findall(r"\bint\s+(nvshmem_perftest_\w+)\s*\(", perf))
     return names, perf_names

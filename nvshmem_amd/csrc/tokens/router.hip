@@ -1,0 +1,766 @@
+// The router in front of the token shuffle: top-k experts of every token with their gates, counts per expert, the balance loss
+// over all PEs, the gradient of gates and loss, and the shuffle's tables.
+//
+//   a logit of -inf or NaN masks an expert out;  m = max l, z = sum exp(l - m), p = exp(l - m) / z   (0 where masked)
+//   S = the topk largest logits that are not masked, ties to the lowest expert; expert = -1 and gate = 0 where there are fewer
+//   gate = scale * p / (normalise ? sum of p over S : 1)
+//   counts@p[e] = copies that PE p sends to expert e;  c_e = sum of them over the PEs, C = sum of c_e, N = tokens with an expert
+//   loss = E / (C N) sum_e c_e sum_t p[t, e],   balance[e] = d loss / d p[t, e] = E c_e / (C N)
+//
+// Backward, for upstream dgate and dloss:  q_e = dloss balance_e + (normalise ? 0 : scale dgate_e on S)
+//   dl = p (q - sum q p) + (normalise ? w scale (dgate - sum_S w dgate) on S, w = p / sum_S p : 0)
+#include "token_common.hpp"
+
+namespace nvshmem_amd {
+namespace tokens {
+namespace {
+
+constexpr int kMostExperts = 1024, kMostTopk = 16;
+
+// ---- lanes: a token belongs to a group of G lanes (16, or the wavefront) ----
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
+}
+// The value of the lane that step STEP of a reduction over a group pairs with.  Steps 2 and 3 mirror 8 and 16 lanes: after the
+// steps before, all lanes of a quad (a half of the row) hold the same.
+template <int STEP>
+__device__ __forceinline__ uint32_t partner(uint32_t x) {
+    if (STEP == 0) return dpp<0xB1>(x);   // quad_perm [1,0,3,2]
+    if (STEP == 1) return dpp<0x4E>(x);   // quad_perm [2,3,0,1]
+    if (STEP == 2) return dpp<0x141>(x);  // row_half_mirror
+    if (STEP == 3) return dpp<0x140>(x);  // row_mirror
+    return (uint32_t)__shfl_xor((int)x, STEP == 4 ? 16 : 32);
+}
+template <int STEP>
+__device__ __forceinline__ float partner(float x) {
+    return __uint_as_float(partner<STEP>(__float_as_uint(x)));
+}
+template <int STEP>
+__device__ __forceinline__ double partner(double x) {
+    const uint64_t b = (uint64_t)__double_as_longlong(x);
+    return __longlong_as_double((long long)((uint64_t)partner<STEP>((uint32_t)(b >> 32)) << 32 | partner<STEP>((uint32_t)b)));
+}
+template <int G>
+__device__ __forceinline__ float group_sum(float x) {
+    x += partner<0>(x);
+    x += partner<1>(x);
+    x += partner<2>(x);
+    x += partner<3>(x);
+    if (G == 64) {
+        x += partner<4>(x);
+        x += partner<5>(x);
+    }
+    return x;
+}
+template <int G>
+__device__ __forceinline__ float group_max(float x) {
+    x = fmaxf(x, partner<0>(x));
+    x = fmaxf(x, partner<1>(x));
+    x = fmaxf(x, partner<2>(x));
+    x = fmaxf(x, partner<3>(x));
+    if (G == 64) {
+        x = fmaxf(x, partner<4>(x));
+        x = fmaxf(x, partner<5>(x));
+    }
+    return x;
+}
+
+// ---- keys: a logit and its expert in one word, larger for the larger logit and then for the lower expert ----
+// 16-bit logits: an unsigned word of the logit's bits in ascending order and the expert's complement.  fp32 logits: the same in the
+// 52 mantissa bits of a double in [1, 2), which v_max_f64 and v_min_f64 compare.  The smallest key (0, or 1.0) stands for
+// a masked expert: no logit that is not masked has it.  -0.0 is 0.0.
+__device__ __forceinline__ uint32_t ascending(uint32_t b, uint32_t sign) { return b & sign ? ~b & (sign | (sign - 1)) : b | sign; }
+__device__ __forceinline__ uint32_t descending_back(uint32_t s, uint32_t sign) { return s & sign ? s & ~sign : ~s & (sign | (sign - 1)); }
+
+template <typename T>
+struct Key {  // _Float16, __bf16
+    typedef uint32_t type;
+    static __device__ __forceinline__ type masked() { return 0; }
+    static __device__ __forceinline__ type make(T x, uint32_t e) {
+        uint32_t b = __builtin_bit_cast(uint16_t, x);
+        b = b == 0x8000u ? 0u : b;
+        return ascending(b, 0x8000u) << 16 | (0xffffu - e);
+    }
+    static __device__ __forceinline__ uint32_t expert(type k) { return 0xffffu - (k & 0xffffu); }
+    static __device__ __forceinline__ float logit(type k) {
+        return (float)__builtin_bit_cast(T, (uint16_t)descending_back(k >> 16, 0x8000u));
+    }
+    static __device__ __forceinline__ type larger(type a, type b) { return a > b ? a : b; }
+    static __device__ __forceinline__ type smaller(type a, type b) { return a < b ? a : b; }
+};
+template <>
+struct Key<float> {
+    typedef double type;
+    static __device__ __forceinline__ type masked() { return 1.0; }
+    static __device__ __forceinline__ type make(float x, uint32_t e) {
+        const uint32_t s = ascending(__float_as_uint(x + 0.0f), 0x80000000u);
+        return __longlong_as_double((long long)((uint64_t)(0x3ff00000u | s >> 12) << 32 | (s << 20 | (0xfffffu - e))));
+    }
+    static __device__ __forceinline__ uint32_t expert(type k) { return 0xfffffu - ((uint32_t)__double_as_longlong(k) & 0xfffffu); }
+    static __device__ __forceinline__ float logit(type k) {
+        return __uint_as_float(descending_back((uint32_t)((uint64_t)__double_as_longlong(k) >> 20), 0x80000000u));
+    }
+    // (the instructions themselves: around fmax and fmin the compiler quiets NaNs that no key is)
+    static __device__ __forceinline__ type larger(type a, type b) {
+        type r;
+        asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+        return r;
+    }
+    static __device__ __forceinline__ type smaller(type a, type b) {
+        type r;
+        asm("v_min_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+        return r;
+    }
+};
+
+// Batcher's odd-even merge sort, largest first, all indices known at compile time.
+template <typename K, int N>
+__device__ __forceinline__ void sort_largest_first(typename K::type *a) {
+#pragma unroll
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+        for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+            for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; ++i)
+                    if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                        const typename K::type x = a[i + j], y = a[i + j + k];
+                        a[i + j] = K::larger(x, y);
+                        a[i + j + k] = K::smaller(x, y);
+                    }
+}
+// The N largest of two sorted lists, sorted: one list against the other backwards leaves them, rising and then falling.
+template <typename K, int N>
+__device__ __forceinline__ void keep_largest(typename K::type *a, const typename K::type *b) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] = K::larger(a[i], b[N - 1 - i]);
+#pragma unroll
+    for (int s = N / 2; s >= 1; s /= 2)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (!(i & s)) {
+                const typename K::type x = a[i], y = a[i + s];
+                a[i] = K::larger(x, y);
+                a[i + s] = K::smaller(x, y);
+            }
+}
+template <typename K, int N, int STEP>
+__device__ __forceinline__ void keep_largest_of_pair(typename K::type *a) {
+    typename K::type b[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) b[i] = partner<STEP>(a[i]);
+    keep_largest<K, N>(a, b);
+}
+
+// ---- a lane's V logits of a token: loads of W neighbouring ones, G lanes side by side ----
+template <typename T, int G, int V>
+struct Slots {
+    static constexpr int W = V < chunk_elems<T>() ? V : chunk_elems<T>();
+    typedef T vec __attribute__((ext_vector_type(W)));
+    typedef vec vec_unaligned __attribute__((aligned(sizeof(T))));
+    static __device__ __forceinline__ unsigned expert(int u, unsigned sub) { return (unsigned)(u / W * G + sub) * W + u % W; }
+    static __device__ __forceinline__ void load(T *x, const T *row, unsigned experts, unsigned sub) {
+#pragma unroll
+        for (int u = 0; u < V; u += W) {
+            const unsigned e = expert(u, sub);
+            if (e + W <= experts) {
+                const vec v = *reinterpret_cast<const vec_unaligned *>(row + e);
+#pragma unroll
+                for (int i = 0; i < W; ++i) x[u + i] = v[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < W; ++i) x[u + i] = e + i < experts ? row[e + i] : (T)-__builtin_inff();
+            }
+        }
+    }
+    static __device__ __forceinline__ void store(T *row, const T *x, unsigned experts, unsigned sub) {
+#pragma unroll
+        for (int u = 0; u < V; u += W) {
+            const unsigned e = expert(u, sub);
+            if (e + W <= experts) {
+                vec v;
+#pragma unroll
+                for (int i = 0; i < W; ++i) v[i] = x[u + i];
+                *reinterpret_cast<vec_unaligned *>(row + e) = v;
+            } else {
+#pragma unroll
+                for (int i = 0; i < W; ++i)
+                    if (e + i < experts) row[e + i] = x[u + i];
+            }
+        }
+    }
+};
+
+// exp(l - m) for l <= m; two infinities of a sign differ by nothing.
+__device__ __forceinline__ float exp_below(float l, float m) { return __expf(l == m ? 0.0f : l - m); }
+
+struct RouteArgs {
+    uint64_t stride;
+    int32_t *expert;
+    float *gate;
+    int64_t *counts;  // written by the blocks themselves where a PE has one block, and no loss is asked for
+    char *work;
+    uint64_t hist, psum, rows, ticket;
+    unsigned tokens, per_block, blocks, experts, topk;
+    int normalise, loss;
+    float scale;
+};
+
+constexpr int kRouteThreads = 256;
+
+template <typename T, int G, int V, int KP>
+__global__ __launch_bounds__(kRouteThreads) void route_kernel(const T *logits, RouteArgs a) {
+    typedef Key<T> K;
+    constexpr int kGroups = kRouteThreads / G, kWaves = kRouteThreads / kLanes;
+    extern __shared__ uint32_t lds[];  // hist[experts], float psum[kWaves][experts], rows
+    uint32_t *hist = lds;
+    float *psum = (float *)(lds + a.experts);
+    uint32_t *rows = lds + a.experts * (1 + (a.loss ? kWaves : 0));
+    const unsigned pe = blockIdx.z, sub = threadIdx.x % G, group = threadIdx.x / G;
+    for (unsigned e = threadIdx.x; e < a.experts; e += kRouteThreads) hist[e] = 0;
+    if (threadIdx.x == 0) rows[0] = 0;
+    __syncthreads();
+    if (a.loss && blockIdx.x == 0 && pe == 0 && threadIdx.x == 0) *(uint32_t *)(a.work + a.ticket) = 0;
+
+    const T *my_logits = copy_of(logits, pe, a.stride);
+    int32_t *my_expert = copy_of(a.expert, pe, a.stride);
+    float *my_gate = copy_of(a.gate, pe, a.stride);
+    const unsigned begin = blockIdx.x * a.per_block, end = a.tokens - begin > a.per_block ? begin + a.per_block : a.tokens;
+    float mass[V] = {};
+    unsigned live = 0;
+    for (unsigned t0 = begin; t0 < end; t0 += kGroups) {  // (all lanes take part in every exchange)
+        const unsigned t = t0 + group;
+        T x[V];
+        Slots<T, G, V>::load(x, my_logits + (uint64_t)(t < end ? t : begin) * a.experts, a.experts, sub);
+        typename K::type key[V < KP ? KP : V];
+#pragma unroll
+        for (int u = 0; u < V; ++u)
+            key[u] = (float)x[u] > -__builtin_inff() ? K::make(x[u], Slots<T, G, V>::expert(u, sub)) : K::masked();
+        if (V < KP) {
+            sort_largest_first<K, V>(key);
+#pragma unroll
+            for (int u = V; u < KP; ++u) key[u] = K::masked();
+        } else {
+#pragma unroll
+            for (int u = 0; u < V; u += KP) {
+                sort_largest_first<K, KP>(key + u);
+                if (u) keep_largest<K, KP>(key, key + u);
+            }
+        }
+        keep_largest_of_pair<K, KP, 0>(key);
+        keep_largest_of_pair<K, KP, 1>(key);
+        keep_largest_of_pair<K, KP, 2>(key);
+        keep_largest_of_pair<K, KP, 3>(key);
+        if (G == 64) {
+            keep_largest_of_pair<K, KP, 4>(key);
+            keep_largest_of_pair<K, KP, 5>(key);
+        }
+        const bool some = key[0] != K::masked();
+        const float m = K::logit(key[0]);
+        float z = 1.0f;
+        if (a.loss || !a.normalise) {
+            float p[V], sum = 0.0f;
+#pragma unroll
+            for (int u = 0; u < V; ++u) {
+                p[u] = (float)x[u] > -__builtin_inff() ? exp_below((float)x[u], m) : 0.0f;
+                sum += p[u];
+            }
+            z = group_sum<G>(sum);
+            const float r = some && t < end ? 1.0f / z : 0.0f;
+#pragma unroll
+            for (int u = 0; u < V; ++u) mass[u] = __builtin_fmaf(p[u], r, mass[u]);
+        }
+        typename K::type own = K::masked();
+#pragma unroll
+        for (int k = 0; k < KP; ++k)
+            if (sub == (unsigned)k) own = key[k];
+        const bool chosen = sub < a.topk && own != K::masked();
+        const float p = chosen ? exp_below(K::logit(own), m) : 0.0f;
+        const float s = group_sum<G>(p);
+        if (t < end) {
+            live += some && sub == 0;
+            if (sub < a.topk) {
+                const uint32_t e = K::expert(own);
+                my_expert[(uint64_t)t * a.topk + sub] = chosen ? (int32_t)e : -1;
+                my_gate[(uint64_t)t * a.topk + sub] = chosen ? a.scale * (p / (a.normalise ? s : z)) : 0.0f;
+                if (chosen) atomicAdd(&hist[e], 1u);
+            }
+        }
+    }
+    if (live) atomicAdd(rows, live);
+    if (a.loss) {
+#pragma unroll
+        for (int u = 0; u < V; ++u) {
+            if (G == 16) {
+                mass[u] += partner<4>(mass[u]);
+                mass[u] += partner<5>(mass[u]);
+            }
+            const unsigned e = Slots<T, G, V>::expert(u, sub);
+            if (threadIdx.x % kLanes < G && e < a.experts) psum[threadIdx.x / kLanes * a.experts + e] = mass[u];
+        }
+    }
+    __syncthreads();
+    char *work = copy_of(a.work, pe, a.stride);
+    for (unsigned e = threadIdx.x; e < a.experts; e += kRouteThreads) {
+        if (a.counts) copy_of(a.counts, pe, a.stride)[e] = hist[e];
+        else ((uint32_t *)(work + a.hist))[(uint64_t)blockIdx.x * a.experts + e] = hist[e];
+        if (a.loss) {
+            float s = 0.0f;
+            for (int w = 0; w < kWaves; ++w) s += psum[w * a.experts + e];
+            ((float *)(work + a.psum))[(uint64_t)blockIdx.x * a.experts + e] = s;
+        }
+    }
+    if (a.loss) {
+        if (threadIdx.x == 0) ((uint32_t *)(work + a.rows))[2 * blockIdx.x] = rows[0];
+        // copies of this block
+        __syncthreads();
+        if (threadIdx.x < kLanes) {
+            uint32_t n = 0;
+            for (unsigned e = threadIdx.x; e < a.experts; e += kLanes) n += hist[e];
+            for (int s = 32; s; s >>= 1) n += __shfl_xor((int)n, s);
+            if (threadIdx.x == 0) ((uint32_t *)(work + a.rows))[2 * blockIdx.x + 1] = n;
+        }
+    }
+}
+
+// Counts, loss and its derivative from what the blocks of all PEs left: 32 experts a block, 32 rows at a time.
+constexpr unsigned kFinishExperts = 32, kFinishRows = 32;
+
+__global__ __launch_bounds__(kFinishExperts *kFinishRows) void route_finish_kernel(int64_t *counts, float *loss, float *balance,
+                                                                                    char *work, uint64_t stride, uint64_t hist,
+                                                                                    uint64_t psum, uint64_t rows, uint64_t ticket,
+                                                                                    unsigned blocks, unsigned experts, unsigned npes) {
+    __shared__ uint32_t c_part[kFinishRows][kFinishExperts];
+    __shared__ double s_part[kFinishRows][kFinishExperts];
+    __shared__ double value[kFinishExperts];
+    __shared__ unsigned long long totals[2];
+    __shared__ unsigned last;
+    const unsigned x = threadIdx.x % kFinishExperts, y = threadIdx.x / kFinishExperts;
+    const unsigned e = blockIdx.x * kFinishExperts + x;
+    if (threadIdx.x < 2) totals[threadIdx.x] = 0;
+    double s = 0.0;
+    unsigned long long all = 0;
+    for (unsigned pe = 0; pe < npes; ++pe) {
+        const char *w = copy_of(work, pe, stride);
+        uint32_t c = 0;
+        if (e < experts)
+            for (unsigned r = y; r < blocks; r += kFinishRows) {
+                c += ((const uint32_t *)(w + hist))[(uint64_t)r * experts + e];
+                if (loss) s += ((const float *)(w + psum))[(uint64_t)r * experts + e];
+            }
+        c_part[y][x] = c;
+        __syncthreads();
+        if (y == 0 && e < experts) {
+            c = 0;
+            for (unsigned i = 0; i < kFinishRows; ++i) c += c_part[i][x];
+            copy_of(counts, pe, stride)[e] = c;
+            all += c;
+        }
+        __syncthreads();
+    }
+    if (!loss) return;
+    s_part[y][x] = s;
+    // rows and copies of all PEs
+    unsigned long long n = 0, m = 0;
+    for (unsigned i = threadIdx.x; i < npes * blocks; i += kFinishExperts * kFinishRows) {
+        const uint32_t *r = (const uint32_t *)(copy_of(work, i / blocks, stride) + rows) + 2 * (i % blocks);
+        n += r[0];
+        m += r[1];
+    }
+    if (n) atomicAdd(&totals[0], n);
+    if (m) atomicAdd(&totals[1], m);
+    __syncthreads();
+    if (y == 0) {
+        double total = 0.0;
+        for (unsigned i = 0; i < kFinishRows; ++i) total += s_part[i][x];
+        const double b = totals[1] ? (double)experts * (double)all / ((double)totals[1] * (double)totals[0]) : 0.0;
+        value[x] = e < experts ? b * total : 0.0;
+        if (e < experts)
+            for (unsigned pe = 0; pe < npes; ++pe) copy_of(balance, pe, stride)[e] = (float)b;
+    }
+    __syncthreads();
+    // the block that comes last adds up what each block found, in their order
+    double *found = (double *)(work + ticket + 64);
+    if (threadIdx.x == 0) {
+        double v = 0.0;
+        for (unsigned i = 0; i < kFinishExperts; ++i) v += value[i];
+        __hip_atomic_store(found + blockIdx.x, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = __hip_atomic_fetch_add((uint32_t *)(work + ticket), 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) + 1 == gridDim.x;
+    }
+    __syncthreads();
+    if (!last) return;
+    if (threadIdx.x < npes) {
+        double v = 0.0;
+        for (unsigned i = 0; i < gridDim.x; ++i) v += __hip_atomic_load(found + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        copy_of(loss, threadIdx.x, stride)[0] = (float)v;
+    }
+}
+
+template <typename T, int G, int V>
+__global__ __launch_bounds__(kRouteThreads) void route_grad_kernel(T *dlogits, const T *logits, const int32_t *expert,
+                                                                   const float *dgate, const float *balance, const float *dloss,
+                                                                   uint64_t stride, unsigned tokens, unsigned experts, unsigned topk,
+                                                                   int normalise, float scale) {
+    constexpr int kGroups = kRouteThreads / G;
+    __shared__ float chosen_part[kGroups][G * V];  // what only the chosen experts get, by expert
+    const unsigned pe = blockIdx.z, sub = threadIdx.x % G, group = threadIdx.x / G;
+    const T *my_logits = copy_of(logits, pe, stride);
+    T *my_dlogits = copy_of(dlogits, pe, stride);
+    const int32_t *my_expert = copy_of(expert, pe, stride);
+    const float *my_dgate = copy_of(dgate, pe, stride);
+    float *part = chosen_part[group];
+#pragma unroll
+    for (int u = 0; u < V; ++u) part[u * G + sub] = 0.0f;
+    float b[V];
+    const float up = balance ? copy_of(dloss, pe, stride)[0] : 0.0f;
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+        const unsigned e = Slots<T, G, V>::expert(u, sub);
+        b[u] = balance && e < experts ? up * copy_of(balance, pe, stride)[e] : 0.0f;
+    }
+    for (unsigned t0 = blockIdx.x * kGroups; t0 < tokens; t0 += gridDim.x * kGroups) {
+        const bool here = t0 + group < tokens;
+        const unsigned t = here ? t0 + group : t0;
+        const T *row = my_logits + (uint64_t)t * experts;
+        T x[V];
+        Slots<T, G, V>::load(x, row, experts, sub);
+        int32_t e = -1;
+        float g = 0.0f, l = -__builtin_inff();
+        if (sub < topk) {
+            e = my_expert[(uint64_t)t * topk + sub];
+            if ((unsigned)e < experts) {
+                g = scale * my_dgate[(uint64_t)t * topk + sub];
+                l = (float)row[e];
+            }
+        }
+        const bool chosen = (unsigned)e < experts && l > -__builtin_inff();
+        float p[V], m = -__builtin_inff();
+#pragma unroll
+        for (int u = 0; u < V; ++u) m = fmaxf(m, (float)x[u]);  // (fmax passes NaN over)
+        m = group_max<G>(m);
+        float z = 0.0f, bp = 0.0f;
+#pragma unroll
+        for (int u = 0; u < V; ++u) {
+            p[u] = (float)x[u] > -__builtin_inff() ? exp_below((float)x[u], m) : 0.0f;
+            z += p[u];
+            bp = __builtin_fmaf(p[u], b[u], bp);
+        }
+        z = group_sum<G>(z);
+        const float r = z > 0.0f ? 1.0f / z : 0.0f;
+        bp = group_sum<G>(bp) * r;
+        if (!chosen) g = 0.0f;
+        // the gates' own softmax is taken against the largest chosen logit, whatever else the row holds
+        const float top = normalise ? group_max<G>(chosen ? l : -__builtin_inff()) : m;
+        const float pk = chosen ? exp_below(l, top) * (normalise ? 1.0f : r) : 0.0f;
+        const float s = group_sum<G>(pk), gs = group_sum<G>(pk * g);
+        if (chosen) part[e] = normalise ? pk / s * (g - gs / s) : g;
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        T d[V];
+#pragma unroll
+        for (int u = 0; u < V; ++u) {
+            const unsigned at = Slots<T, G, V>::expert(u, sub);
+            const float c = part[at], pr = p[u] * r;
+            d[u] = (T)(normalise ? __builtin_fmaf(pr, b[u] - bp, c) : pr * (b[u] + c - (bp + gs)));
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (chosen) part[e] = 0.0f;
+        if (here) Slots<T, G, V>::store(my_dlogits + (uint64_t)t * experts, d, experts, sub);
+    }
+}
+
+// ---- the shuffle's tables ----
+// A stable counting sort of the copies by expert: rows of a destination PE lie in the order (expert, source PE, token, k).
+constexpr unsigned kPlaceThreads = 1024, kPlaceRounds = 8, kPlaceCopies = kPlaceThreads * kPlaceRounds;
+constexpr unsigned kPlaceWaves = kPlaceThreads / kLanes;
+
+__global__ __launch_bounds__(kPlaceThreads) void place_count_kernel(uint32_t *hist, const int32_t *expert, uint64_t stride,
+                                                                    unsigned copies, unsigned experts) {
+    __shared__ uint32_t count[kMostExperts];
+    const unsigned pe = blockIdx.z;
+    count[threadIdx.x] = 0;
+    __syncthreads();
+    const int32_t *mine = copy_of(expert, pe, stride);
+    for (unsigned i = 0; i < kPlaceRounds; ++i) {
+        const unsigned c = blockIdx.x * kPlaceCopies + i * kPlaceThreads + threadIdx.x;
+        if (c < copies && (unsigned)mine[c] < experts) atomicAdd(&count[mine[c]], 1u);
+    }
+    __syncthreads();
+    if (threadIdx.x < experts) copy_of(hist, pe, stride)[(uint64_t)blockIdx.x * experts + threadIdx.x] = count[threadIdx.x];
+}
+
+__global__ __launch_bounds__(kPlaceThreads) void place_kernel(int32_t *dest_pe, int64_t *dest_row, uint64_t *expected,
+                                                              int64_t *expert_row, const uint32_t *hist, const int32_t *expert,
+                                                              const int64_t *counts, uint64_t stride, unsigned copies,
+                                                              unsigned experts, unsigned npes, uint64_t cap) {
+    extern __shared__ uint32_t lds[];  // next[kPlaceWaves][experts]: where a wavefront's next copy to an expert goes
+    __shared__ uint32_t scan[kMostExperts + 1], wave_sum[kPlaceWaves], arriving[NVSHMEMI_AMD_MAX_PES];
+    uint32_t *next = lds;
+    const unsigned pe = blockIdx.z, wave = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+    const unsigned per_pe = experts / npes;
+    const int32_t *mine = copy_of(expert, pe, stride);
+    // this wavefront's copies, consecutive
+    const unsigned c0 = blockIdx.x * kPlaceCopies + wave * (kPlaceRounds * kLanes) + lane;
+    int32_t to[kPlaceRounds];
+#pragma unroll
+    for (unsigned i = 0; i < kPlaceRounds; ++i) to[i] = c0 + i * kLanes < copies ? mine[c0 + i * kLanes] : -1;
+    for (unsigned i = threadIdx.x; i < kPlaceWaves * experts; i += kPlaceThreads) next[i] = 0;
+    if (threadIdx.x < NVSHMEMI_AMD_MAX_PES) arriving[threadIdx.x] = 0;
+
+    // rows of every expert from all sources, from the sources before this one, and from the blocks before this one
+    const unsigned e = threadIdx.x;
+    uint32_t total = 0, before = 0;
+    if (e < experts) {
+        for (unsigned src = 0; src < npes; ++src) {
+            const uint32_t c = (uint32_t)copy_of(counts, src, stride)[e];
+            if (src < pe) before += c;
+            total += c;
+        }
+        const uint32_t *h = hist ? copy_of(hist, pe, stride) : nullptr;
+        for (unsigned b = 0; b < blockIdx.x; ++b) before += h[(uint64_t)b * experts + e];
+    }
+    uint32_t sum = total;
+    for (int s = 1; s < kLanes; s <<= 1) {
+        const uint32_t up = (uint32_t)__shfl_up((int)sum, s);
+        if ((int)lane >= s) sum += up;
+    }
+    if (lane == kLanes - 1) wave_sum[wave] = sum;
+    __syncthreads();
+    for (unsigned w = 0; w < wave; ++w) sum += wave_sum[w];
+    scan[e + 1] = sum;
+    if (e == 0) scan[0] = 0;
+#pragma unroll
+    for (unsigned i = 0; i < kPlaceRounds; ++i)
+        if ((unsigned)to[i] < experts) atomicAdd(&next[wave * experts + to[i]], 1u);
+    __syncthreads();
+    if (e < experts) {
+        const uint32_t start = scan[e] - scan[e / per_pe * per_pe];
+        uint32_t run = start + before;
+        for (unsigned w = 0; w < kPlaceWaves; ++w) {
+            const uint32_t n = next[w * experts + e];
+            next[w * experts + e] = run;
+            run += n;
+        }
+        if (blockIdx.x == 0 && e / per_pe == pe) {  // what arrives here
+            uint32_t at = start;
+            for (unsigned src = 0; src < npes; ++src) {
+                const uint32_t n = (uint32_t)copy_of(counts, src, stride)[e];
+                const uint64_t room = at < cap ? cap - at : 0;
+                atomicAdd(&arriving[src], n < room ? n : (uint32_t)room);
+                at += n;
+            }
+            int64_t *row = copy_of(expert_row, pe, stride);
+            row[e - pe * per_pe] = start < cap ? start : (int64_t)cap;
+            if (e + 1 == (pe + 1) * per_pe) row[per_pe] = at < cap ? at : (int64_t)cap;
+        }
+    }
+    __syncthreads();
+    if (blockIdx.x == 0 && threadIdx.x < npes) copy_of(expected, pe, stride)[threadIdx.x] = arriving[threadIdx.x];
+    int32_t *out_pe = copy_of(dest_pe, pe, stride);
+    int64_t *out_row = copy_of(dest_row, pe, stride);
+    const unsigned bits = 32 - __builtin_clz(experts);
+    uint32_t *place = next + wave * experts;
+#pragma unroll
+    for (unsigned i = 0; i < kPlaceRounds; ++i) {
+        const bool some = (unsigned)to[i] < experts;
+        // the lanes that send to the same expert
+        uint64_t same = __builtin_amdgcn_ballot_w64(some);
+        for (unsigned b = 0; b < bits; ++b) {
+            const uint64_t set = __builtin_amdgcn_ballot_w64((unsigned)to[i] >> b & 1);
+            same &= (unsigned)to[i] >> b & 1 ? set : ~set;
+        }
+        const unsigned rank = (unsigned)__builtin_popcountll(same & ((1ull << lane) - 1)), n = (unsigned)__builtin_popcountll(same);
+        uint32_t row = 0;
+        if (some) row = place[to[i]] + rank;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (some && rank + 1 == n) place[to[i]] = row + 1;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const unsigned c = c0 + i * kLanes;
+        if (c < copies) {
+            const bool kept = some && row < cap;
+            out_pe[c] = kept ? (int32_t)((unsigned)to[i] / per_pe) : -1;
+            out_row[c] = kept ? (int64_t)row : -1;
+        }
+    }
+}
+
+// ---- host ----
+// Blocks of a PE: enough of them over all PEs to fill the GPU, and no more, as the second kernel reads what each one leaves.
+struct RouteShape {
+    unsigned groups, per_block, blocks;
+    uint64_t hist, psum, rows, ticket, bytes;
+    RouteShape(size_t tokens, int experts, int npes) {
+        groups = kRouteThreads / (experts > 256 ? 64 : 16);
+        const uint64_t steps = ((uint64_t)tokens * npes + groups - 1) / groups;
+        per_block = groups * (unsigned)(steps <= 1024 ? 1 : (steps + 1023) / 1024);
+        blocks = tokens ? div_up(tokens, per_block) : 1;
+        const uint64_t table = ((uint64_t)blocks * experts * 4 + 63) / 64 * 64;
+        hist = 0;
+        psum = table;
+        rows = 2 * table;
+        ticket = rows + ((uint64_t)blocks * 8 + 63) / 64 * 64;
+        bytes = ticket + 64 + (kMostExperts / kFinishExperts) * sizeof(double);
+    }
+};
+
+int check_routing(Runtime &rt, const char *what, size_t tokens, int experts, int topk) {
+    NVSHMEM_AMD_REFUSE(experts < 1 || experts > kMostExperts, "%s: %d experts, outside [1, %d]", what, experts, kMostExperts);
+    NVSHMEM_AMD_REFUSE(topk < 1 || topk > kMostTopk || topk > experts, "%s: top-%d of %d experts, outside [1, %d]", what, topk, experts,
+                       kMostTopk < experts ? kMostTopk : experts);
+    NVSHMEM_AMD_REFUSE(tokens > 0x7fffffffull / (size_t)rt.npes / (size_t)topk, "%s: %zu tokens x %d copies on %d PEs, at most 2^31 - 1 in all",
+                       what, tokens, topk, rt.npes);
+    return 0;
+}
+
+template <typename T, int G, int V>
+void launch_route(const T *logits, const RouteArgs &a, unsigned npes, hipStream_t stream) {
+    const dim3 grid(a.blocks, 1, npes);
+    const size_t lds = ((size_t)a.experts * (1 + (a.loss ? kRouteThreads / kLanes : 0)) + 1) * 4;
+    if (a.topk <= 2) launch_kernel(route_kernel<T, G, V, 2>, grid, dim3(kRouteThreads), lds, stream, logits, a);
+    else if (a.topk <= 8) launch_kernel(route_kernel<T, G, V, 8>, grid, dim3(kRouteThreads), lds, stream, logits, a);
+    else launch_kernel(route_kernel<T, G, V, 16>, grid, dim3(kRouteThreads), lds, stream, logits, a);
+}
+
+template <typename API>
+int route_on_stream(int32_t *expert, float *gate, int64_t *counts, float *loss, float *balance, void *workspace, const API *logits,
+                    size_t tokens, int experts, int topk, int normalise, float scale, hipStream_t stream) {
+    typedef typename element<API>::type T;
+    Runtime &rt = Runtime::get();
+    std::lock_guard<std::recursive_mutex> lock(rt.mu);
+    if (!ready(rt, "moe_route")) return NVSHMEMX_ERROR_INVALID_VALUE;
+    if (int rc = check_routing(rt, "moe_route", tokens, experts, topk)) return rc;
+    NVSHMEM_AMD_REFUSE(!loss != !balance, "moe_route: loss and balance come together");
+    NVSHMEM_AMD_REFUSE(!(scale - scale == 0.0f), "moe_route: the scale must be finite");
+    const RouteShape shape(tokens, experts, rt.npes);
+    const uint64_t copies = (uint64_t)tokens * topk;
+    Operands ops(rt, "moe_route");
+    const T *in = (const T *)ops.in("logits", logits, (uint64_t)tokens * experts);
+    RouteArgs a{};
+    a.stride = rt.heap_size;
+    a.expert = ops.out("expert", expert, copies);
+    a.gate = ops.out("gate", gate, copies);
+    int64_t *count = ops.out("counts", counts, (uint64_t)experts);
+    float *l = loss ? ops.out("loss", loss, 1) : nullptr, *b = loss ? ops.out("balance", balance, (uint64_t)experts) : nullptr;
+    a.work = ops.out("workspace", (char *)workspace, shape.bytes, 64);
+    if (!ops.ok()) return NVSHMEMX_ERROR_INVALID_VALUE;
+    const bool alone = shape.blocks == 1 && !loss;
+    a.counts = alone ? count : nullptr;
+    a.hist = shape.hist, a.psum = shape.psum, a.rows = shape.rows, a.ticket = shape.ticket;
+    a.tokens = (unsigned)tokens, a.per_block = shape.per_block, a.blocks = shape.blocks;
+    a.experts = (unsigned)experts, a.topk = (unsigned)topk;
+    a.normalise = normalise != 0, a.loss = loss != nullptr, a.scale = scale;
+    if (experts <= 64) launch_route<T, 16, 4>(in, a, rt.npes, stream);
+    else if (experts <= 256) launch_route<T, 16, 16>(in, a, rt.npes, stream);
+    else launch_route<T, 64, 16>(in, a, rt.npes, stream);
+    if (!alone)
+        launch_kernel(route_finish_kernel, dim3(div_up(experts, kFinishExperts)), dim3(kFinishExperts * kFinishRows), 0, stream, count, l,
+                      b, a.work, a.stride, a.hist, a.psum, a.rows, a.ticket, a.blocks, a.experts, (unsigned)rt.npes);
+    return launched("moe_route");
+}
+
+template <typename API>
+int route_grad_on_stream(API *dlogits, const API *logits, const int32_t *expert, const float *dgate, const float *balance,
+                         const float *dloss, size_t tokens, int experts, int topk, int normalise, float scale, hipStream_t stream) {
+    typedef typename element<API>::type T;
+    Runtime &rt = Runtime::get();
+    std::lock_guard<std::recursive_mutex> lock(rt.mu);
+    if (!ready(rt, "moe_route_grad")) return NVSHMEMX_ERROR_INVALID_VALUE;
+    if (int rc = check_routing(rt, "moe_route_grad", tokens, experts, topk)) return rc;
+    NVSHMEM_AMD_REFUSE(!dloss != !balance, "moe_route_grad: dloss and balance come together");
+    NVSHMEM_AMD_REFUSE(!(scale - scale == 0.0f), "moe_route_grad: the scale must be finite");
+    const uint64_t copies = (uint64_t)tokens * topk, values = (uint64_t)tokens * experts;
+    Operands ops(rt, "moe_route_grad");
+    const T *in = (const T *)ops.in("logits", logits, values);
+    const int32_t *to = ops.in("expert", expert, copies);
+    const float *dg = ops.in("dgate", dgate, copies);
+    const float *b = balance ? ops.in("balance", balance, (uint64_t)experts) : nullptr;
+    const float *dl = balance ? ops.in("dloss", dloss, 1) : nullptr;
+    T *out = (T *)ops.out("dlogits", dlogits, values);
+    if (!ops.ok()) return NVSHMEMX_ERROR_INVALID_VALUE;
+    if (tokens == 0) return 0;
+#define NVSHMEM_AMD_LAUNCH_GRAD(G, V)                                                                                             \
+    {                                                                                                                             \
+        const unsigned steps = div_up(tokens, kRouteThreads / G), most = 4096 / (unsigned)rt.npes;                                \
+        launch_kernel(route_grad_kernel<T, G, V>, dim3(steps < most ? steps : most, 1, rt.npes), dim3(kRouteThreads), 0, stream,  \
+                      out, in, to, dg, b, dl, rt.heap_size, (unsigned)tokens, (unsigned)experts, (unsigned)topk, normalise != 0, scale); \
+    }
+    if (experts <= 64) NVSHMEM_AMD_LAUNCH_GRAD(16, 4)
+    else if (experts <= 256) NVSHMEM_AMD_LAUNCH_GRAD(16, 16)
+    else NVSHMEM_AMD_LAUNCH_GRAD(64, 16)
+#undef NVSHMEM_AMD_LAUNCH_GRAD
+    return launched("moe_route_grad");
+}
+
+int place_on_stream(int32_t *dest_pe, int64_t *dest_row, uint64_t *expected, int64_t *expert_row, void *workspace,
+                    const int32_t *expert, const int64_t *counts, size_t tokens, int topk, int experts, size_t recv_cap_rows,
+                    hipStream_t stream) {
+    Runtime &rt = Runtime::get();
+    std::lock_guard<std::recursive_mutex> lock(rt.mu);
+    if (!ready(rt, "moe_place")) return NVSHMEMX_ERROR_INVALID_VALUE;
+    if (int rc = check_routing(rt, "moe_place", tokens, experts, topk)) return rc;
+    NVSHMEM_AMD_REFUSE(experts % rt.npes, "moe_place: %d experts on %d PEs, not the same number on each", experts, rt.npes);
+    const uint64_t copies = (uint64_t)tokens * topk;
+    const unsigned blocks = copies ? div_up(copies, kPlaceCopies) : 1;
+    Operands ops(rt, "moe_place");
+    const int32_t *in = ops.in("expert", expert, copies);
+    const int64_t *count = ops.in("counts", counts, (uint64_t)experts);
+    int32_t *to = ops.out("dest_pe", dest_pe, copies);
+    int64_t *row = ops.out("dest_row", dest_row, copies);
+    uint64_t *exp = ops.out("expected", expected, (uint64_t)rt.npes);
+    int64_t *first = ops.out("expert_row", expert_row, (uint64_t)(experts / rt.npes + 1));
+    uint32_t *hist = blocks > 1 ? ops.out("workspace", (uint32_t *)workspace, (uint64_t)blocks * experts, 64) : nullptr;
+    if (!ops.ok()) return NVSHMEMX_ERROR_INVALID_VALUE;
+    if (blocks > 1)
+        launch_kernel(place_count_kernel, dim3(blocks, 1, rt.npes), dim3(kPlaceThreads), 0, stream, hist, in, rt.heap_size,
+                      (unsigned)copies, (unsigned)experts);
+    launch_kernel(place_kernel, dim3(blocks, 1, rt.npes), dim3(kPlaceThreads), (size_t)kPlaceWaves * experts * 4, stream, to, row, exp,
+                  first, hist, in, count, rt.heap_size, (unsigned)copies, (unsigned)experts, (unsigned)rt.npes, (uint64_t)recv_cap_rows);
+    return launched("moe_place");
+}
+
+}  // namespace
+}  // namespace tokens
+}  // namespace nvshmem_amd
+
+using namespace nvshmem_amd;
+
+extern "C" {
+
+#define NVSHMEM_AMD_ROUTE(NAME, TYPE)                                                                                              \
+    int nvshmemx_amd_##NAME##_moe_route_on_stream(int32_t *expert, float *gate, int64_t *counts, float *loss, float *balance,      \
+                                                  void *workspace, const TYPE *logits, size_t tokens, int experts, int topk,       \
+                                                  int normalise, float scale, nvshmemx_stream_t stream) {                          \
+        return tokens::route_on_stream(expert, gate, counts, loss, balance, workspace, logits, tokens, experts, topk, normalise,   \
+                                       scale, (hipStream_t)stream);                                                                \
+    }                                                                                                                              \
+    int nvshmemx_amd_##NAME##_moe_route_grad_on_stream(TYPE *dlogits, const TYPE *logits, const int32_t *expert,                   \
+                                                       const float *dgate, const float *balance, const float *dloss,               \
+                                                       size_t tokens, int experts, int topk, int normalise, float scale,           \
+                                                       nvshmemx_stream_t stream) {                                                 \
+        return tokens::route_grad_on_stream(dlogits, logits, expert, dgate, balance, dloss, tokens, experts, topk, normalise,      \
+                                            scale, (hipStream_t)stream);                                                           \
+    }
+NVSHMEMI_AMD_REPT_FOR_TOKEN_TYPES(NVSHMEM_AMD_ROUTE)
+#undef NVSHMEM_AMD_ROUTE
+
+size_t nvshmemx_amd_moe_route_workspace(size_t tokens, int experts) {
+    const int npes = Runtime::get().npes;
+    if (npes < 1 || experts < 1 || experts > tokens::kMostExperts) return 0;
+    return tokens::RouteShape(tokens, experts, npes).bytes;
+}
+
+int nvshmemx_amd_moe_place_on_stream(int32_t *dest_pe, int64_t *dest_row, uint64_t *expected, int64_t *expert_row, void *workspace,
+                                     const int32_t *expert, const int64_t *counts, size_t tokens, int topk, int experts,
+                                     size_t recv_cap_rows, nvshmemx_stream_t stream) {
+    return tokens::place_on_stream(dest_pe, dest_row, expected, expert_row, workspace, expert, counts, tokens, topk, experts,
+                                   recv_cap_rows, (hipStream_t)stream);
+}
+size_t nvshmemx_amd_moe_place_workspace(size_t tokens, int topk, int experts) {
+    if (Runtime::get().npes < 1 || topk < 1 || experts < 1) return 0;
+    return ((uint64_t)tokens * topk + tokens::kPlaceCopies - 1) / tokens::kPlaceCopies * (uint64_t)experts * sizeof(uint32_t);
+}
+
+}  // extern "C"

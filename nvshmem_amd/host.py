@@ -213,6 +213,46 @@ class Runtime:
             self._check(self.lib.nvshmemx_alltoallmem_on_stream(team, dest, src, nbytes,
                                                                 stream.ptr), "alltoallmem_on_stream")
 
+    # -- rows of tokens: in front of and behind the token shuffle ------------------------------
+    def workspace_bytes(self, op, *sizes):
+        """Bytes per PE of a call's workspace: ("embedding_grad", tokens, vocab, dim), ("moe_route", tokens, experts) or
+        ("moe_place", tokens, topk, experts)."""
+        return getattr(self.lib, "nvshmemx_amd_%s_workspace" % op)(*sizes)
+
+    def _tokens(self, name, *args, stream=None):
+        self._check(getattr(self.lib, name)(*args, stream.ptr if stream is not None else None), name)
+
+    def embedding(self, type_name, out, table, ids, tokens, vocab, dim, scale=1.0, stream=None):
+        self._tokens("nvshmemx_amd_%s_embedding_on_stream" % type_name, out, table, ids, tokens, vocab, dim, scale, stream=stream)
+
+    def embedding_grad(self, type_name, dtable, dout, ids, workspace, tokens, vocab, dim, scale=1.0, stream=None):
+        self._tokens("nvshmemx_amd_%s_embedding_grad_on_stream" % type_name, dtable, dout, ids, workspace, tokens, vocab, dim,
+                     scale, stream=stream)
+
+    def moe_route(self, type_name, expert, gate, counts, workspace, logits, tokens, experts, topk, loss=None, balance=None,
+                  normalise=True, scale=1.0, stream=None):
+        self._tokens("nvshmemx_amd_%s_moe_route_on_stream" % type_name, expert, gate, counts, loss, balance, workspace, logits,
+                     tokens, experts, topk, int(normalise), scale, stream=stream)
+
+    def moe_route_grad(self, type_name, dlogits, logits, expert, dgate, tokens, experts, topk, balance=None, dloss=None,
+                       normalise=True, scale=1.0, stream=None):
+        self._tokens("nvshmemx_amd_%s_moe_route_grad_on_stream" % type_name, dlogits, logits, expert, dgate, balance, dloss,
+                     tokens, experts, topk, int(normalise), scale, stream=stream)
+
+    def moe_place(self, dest_pe, dest_row, expected, expert_row, workspace, expert, counts, tokens, topk, experts, recv_cap_rows,
+                  stream=None):
+        self._tokens("nvshmemx_amd_moe_place_on_stream", dest_pe, dest_row, expected, expert_row, workspace, expert, counts,
+                     tokens, topk, experts, recv_cap_rows, stream=stream)
+
+    def moe_combine_sum(self, type_name, out, recv, recv_cap_rows, gate, dest_pe, dest_row, tokens, topk, dim, stream=None):
+        self._tokens("nvshmemx_amd_%s_moe_combine_sum_on_stream" % type_name, out, recv, recv_cap_rows, gate, dest_pe, dest_row,
+                     tokens, topk, dim, stream=stream)
+
+    def moe_combine_grad(self, type_name, drecv, dgate, dout, recv, recv_cap_rows, gate, dest_pe, dest_row, tokens, topk, dim,
+                         stream=None):
+        self._tokens("nvshmemx_amd_%s_moe_combine_grad_on_stream" % type_name, drecv, dgate, dout, recv, recv_cap_rows, gate,
+                     dest_pe, dest_row, tokens, topk, dim, stream=stream)
+
     def read_timeout(self, pe):
         rec = (C.c_uint64 * 4)()
         flag = self.lib.nvshmemx_amd_read_timeout(pe, rec)
