@@ -4,6 +4,7 @@
 //   dtable@(v / R)[v % R] = scale * sum dout@p[t]     over all (p, t) with ids@p[t] = v, in the order of (p, t)
 //
 // An id outside [0, vocab) is padding: a row of zeros, no gradient.
+#include "counting_sort.hpp"
 #include "token_common.hpp"
 
 namespace nvshmem_amd {
@@ -45,40 +46,119 @@ __global__ __launch_bounds__(64) void embedding_kernel(T *out, const T *table, c
 // (`carry`), and a kernel behind it adds those up, in order: nothing depends on which block comes first.
 constexpr unsigned kPart = 32;
 
-// Place of every token in the sorted order, by counting the smaller ones.
-__global__ __launch_bounds__(256) void embedding_rank_kernel(uint32_t *key_out, uint32_t *pos_out, const int64_t *ids,
-                                                             uint64_t stride, unsigned tokens, unsigned n, unsigned vocab) {
-    __shared__ uint32_t tile[256];
-    const unsigned i = blockIdx.x * 256 + threadIdx.x;
-    auto key_of = [&](unsigned j) -> uint32_t {
-        if (j >= n) return 0xffffffffu;
-        const uint64_t id = (uint64_t)copy_of(ids, j / tokens, stride)[j % tokens];
-        return id < vocab ? (uint32_t)id : vocab;
-    };
-    const uint32_t mine = key_of(i);
-    unsigned rank = 0;
-    for (unsigned base = 0; base < n; base += 256) {
-        __syncthreads();
-        tile[threadIdx.x] = key_of(base + threadIdx.x);
-        __syncthreads();
-        for (unsigned j = 0; j < 256 && base + j < n; ++j)
-            rank += (tile[j] < mine || (tile[j] == mine && base + j < i)) ? 1u : 0u;
-    }
-    if (i < n) {
-        key_out[rank] = mine;
-        pos_out[rank] = i;
-    }
+// A token: its id (vocab: padding, sorted behind all ids) and its number pe * tokens + t.
+struct Item {
+    uint32_t key, pos;
+};
+__device__ __forceinline__ uint32_t key_of(const int64_t *ids, uint64_t stride, unsigned tokens, unsigned vocab, unsigned i) {
+    const uint64_t id = (uint64_t)copy_of(ids, i / tokens, stride)[i % tokens];
+    return id < vocab ? (uint32_t)id : vocab;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void embedding_zero_kernel(T *dtable, uint64_t stride, unsigned vocab, unsigned rows,
-                                                             unsigned dim) {
-    const unsigned owner = blockIdx.z;
-    const uint64_t first = (uint64_t)owner * rows;
-    if (first >= vocab) return;
-    const uint64_t elems = (uint64_t)(vocab - first < rows ? vocab - first : rows) * dim;
-    T *mine = copy_of(dtable, owner, stride);
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < elems; i += (uint64_t)gridDim.x * 256) mine[i] = (T)0.0f;
+// Up to kRankTokens tokens: a token's place in the sorted order is the number of smaller ones, and a block of 16 wavefronts counts
+// it for 64 tokens, a lane each, a sixteenth of all tokens a wavefront.  Quadratic, but one launch.
+constexpr unsigned kRankTokens = 8192;
+
+__global__ __launch_bounds__(kSortThreads) void embedding_rank_kernel(Item *sorted, const int64_t *ids, uint64_t stride,
+                                                                      unsigned tokens, unsigned n, unsigned vocab) {
+    __shared__ __align__(16) uint32_t all[kRankTokens];
+    __shared__ uint32_t smaller[kLanes];
+    const unsigned wave = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+    const unsigned padded = (n + 63) / 64 * 64, block = blockIdx.x * kLanes;
+#pragma unroll
+    for (unsigned k = 0; k < kRankTokens / kSortThreads; ++k) {
+        const unsigned i = k * kSortThreads + threadIdx.x;
+        if (i < padded) all[i] = i < n ? key_of(ids, stride, tokens, vocab, i) : 0xffffffffu;
+    }
+    if (threadIdx.x < kLanes) smaller[lane] = 0;
+    __syncthreads();
+    const uint32_t mine = all[block + lane];
+    unsigned rank = 0;
+    // 64 keys at a time; those in front of this block's count when they are equal
+    for (unsigned j0 = wave * kLanes; j0 < padded; j0 += kSortThreads) {
+        if (j0 == block) {
+            for (unsigned j = 0; j < kLanes; ++j) rank += all[block + j] < mine + (j < lane);
+            continue;
+        }
+        const uint32_t limit = mine + (j0 < block);
+#pragma unroll
+        for (unsigned j = 0; j < kLanes; j += 4) {
+            const uint4 k = *(const uint4 *)(all + j0 + j);
+            rank += (k.x < limit) + (k.y < limit) + (k.z < limit) + (k.w < limit);
+        }
+    }
+    atomicAdd(&smaller[lane], rank);
+    __syncthreads();
+    if (wave == 0 && block + lane < n) sorted[smaller[lane]] = {mine, block + lane};
+}
+
+// More tokens: counting sorts by kDigit bits of the id at a time, lowest first, of at most kSortBlocks blocks of consecutive tokens.
+constexpr unsigned kDigit = 9, kBins = 1u << kDigit, kSortBlocks = 64, kSortRounds = 4, kSortTile = kSortThreads * kSortRounds;
+
+template <bool FIRST>
+__device__ __forceinline__ Item item_of(const Item *in, const int64_t *ids, uint64_t stride, unsigned tokens, unsigned vocab,
+                                        unsigned i) {
+    if (FIRST) return {key_of(ids, stride, tokens, vocab, i), i};
+    return in[i];
+}
+
+template <bool FIRST>
+__global__ __launch_bounds__(kSortThreads) void embedding_count_kernel(uint32_t *hist, const Item *in, const int64_t *ids,
+                                                                       uint64_t stride, unsigned tokens, unsigned n, unsigned vocab,
+                                                                       unsigned per_block, unsigned shift) {
+    __shared__ uint32_t count[kBins];
+    if (threadIdx.x < kBins) count[threadIdx.x] = 0;
+    __syncthreads();
+    const uint64_t begin = (uint64_t)blockIdx.x * per_block, end = begin + per_block < n ? begin + per_block : n;
+    for (uint64_t i = begin + threadIdx.x; i < end; i += kSortThreads)
+        atomicAdd(&count[item_of<FIRST>(in, ids, stride, tokens, vocab, (unsigned)i).key >> shift & (kBins - 1)], 1u);
+    __syncthreads();
+    if (threadIdx.x < kBins) hist[blockIdx.x * kBins + threadIdx.x] = count[threadIdx.x];
+}
+
+template <bool FIRST>
+__global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(Item *out, const uint32_t *hist, const Item *in,
+                                                                      const int64_t *ids, uint64_t stride, unsigned tokens, unsigned n,
+                                                                      unsigned vocab, unsigned per_block, unsigned shift) {
+    __shared__ uint32_t count[kSortWaves * kBins], run[kBins], wave_sum[kSortWaves], half[2][kBins];
+    // items of each bin in all blocks, and in those before this one: two threads a bin
+    const unsigned bin = threadIdx.x % kBins;
+    uint32_t total = 0, before = 0;
+#pragma unroll 8
+    for (unsigned b = threadIdx.x / kBins; b < gridDim.x; b += kSortThreads / kBins) {
+        const uint32_t c = hist[b * kBins + bin];
+        total += c;
+        before += b < blockIdx.x ? c : 0;
+    }
+    if (threadIdx.x >= kBins) {
+        half[0][bin] = total;
+        half[1][bin] = before;
+    }
+    __syncthreads();
+    const bool first = threadIdx.x < kBins;
+    total = first ? total + half[0][bin] : 0;
+    const uint32_t start = scan_block(total, wave_sum);
+    if (first) run[bin] = start + before + half[1][bin];
+    const uint64_t begin = (uint64_t)blockIdx.x * per_block, end = begin + per_block < n ? begin + per_block : n;
+    for (uint64_t t = begin; t < end; t += kSortTile) {
+        Item item[kSortRounds];
+        uint32_t to[kSortRounds], place[kSortRounds];
+#pragma unroll
+        for (unsigned r = 0; r < kSortRounds; ++r) {
+            const uint64_t i = t + threadIdx.x / kLanes * (kSortRounds * kLanes) + r * kLanes + threadIdx.x % kLanes;
+            to[r] = kBins;
+            if (i < end) {
+                item[r] = item_of<FIRST>(in, ids, stride, tokens, vocab, (unsigned)i);
+                to[r] = item[r].key >> shift & (kBins - 1);
+            }
+        }
+        __syncthreads();
+        stable_places<kSortRounds>(place, to, kBins, run, count);
+#pragma unroll
+        for (unsigned r = 0; r < kSortRounds; ++r)
+            if (to[r] < kBins) out[place[r]] = item[r];
+        __syncthreads();
+    }
 }
 
 template <typename T>
@@ -90,62 +170,169 @@ __device__ __forceinline__ void write_row(T *dtable, uint64_t stride, uint32_t k
     else chunk_store_part(dst, y, left);
 }
 
+struct SumArgs {
+    const Item *sorted;
+    float *carry;
+    uint64_t stride;
+    unsigned tokens, n, vocab, rows, dim, pitch, pieces, sum_blocks, zero_rows;
+    float scale;
+};
+
+// `elems` zeros at p by a wavefront: elements up to a 16-byte boundary, vectors, elements.
 template <typename T>
-__global__ __launch_bounds__(64) void embedding_sum_kernel(T *dtable, float *carry, const T *dout, const uint32_t *key,
-                                                           const uint32_t *pos, uint64_t stride, unsigned tokens, unsigned n,
-                                                           unsigned vocab, unsigned rows, unsigned dim, unsigned pitch,
-                                                           float scale) {
+__device__ __forceinline__ void zero_fill(T *p, uint64_t elems) {
+    const unsigned lane = threadIdx.x;
+    const uint64_t head = ((16 - (uintptr_t)p % 16) % 16) / sizeof(T);
+    if (elems < head + Chunk<T>::N) {
+        for (uint64_t i = lane; i < elems; i += kLanes) p[i] = (T)0.0f;
+        return;
+    }
+    if (lane < head) p[lane] = (T)0.0f;
+    typedef typename Chunk<T>::vec vec;
+    vec *v = (vec *)(p + head);
+    const uint64_t n = (elems - head) / Chunk<T>::N, tail = head + n * Chunk<T>::N;
+    for (uint64_t i = lane; i < n; i += kLanes) __builtin_nontemporal_store(vec{}, v + i);
+    if (lane < elems - tail) p[tail + lane] = (T)0.0f;
+}
+
+// Loads of a wavefront's rows that are in flight together.
+constexpr unsigned kAhead = 8;
+
+template <typename T>
+__device__ __forceinline__ void embedding_sum_part(T *dtable, const T *dout, const SumArgs &a, unsigned part, unsigned piece) {
     constexpr unsigned N = Chunk<T>::N;
     typedef typename Chunk<T>::facc facc;
-    const unsigned first = (blockIdx.x * kLanes + threadIdx.x) * N, left = first < dim ? dim - first : 0;
-    for (unsigned part = blockIdx.y; (uint64_t)part * kPart < n; part += gridDim.y) {
-    const unsigned begin = part * kPart, end = n - begin > kPart ? begin + kPart : n;
+    const unsigned lane = threadIdx.x, first = (piece * kLanes + lane) * N, left = first < a.dim ? a.dim - first : 0;
+    const unsigned begin = part * kPart, here = a.n - begin < kPart ? a.n - begin : kPart;
+    // lane j looks at item j: where its row is, and whether it is the last of its id
+    Item item = {a.vocab, 0};
+    uint32_t after = a.vocab, prior = a.vocab;
+    if (lane < here) item = a.sorted[begin + lane];
+    if (begin + here < a.n) after = a.sorted[begin + here].key;  // the item behind the part, and the one in front
+    if (begin > 0) prior = a.sorted[begin - 1].key;
+    const uint64_t off = (uint64_t)(item.pos / a.tokens) * a.stride + (uint64_t)(item.pos % a.tokens) * a.dim * sizeof(T);
+    const uint32_t next = (uint32_t)__shfl_down((int)item.key, 1);
+    const bool padding = item.key >= a.vocab;
+    const uint64_t last = __builtin_amdgcn_ballot_w64(!padding && (lane + 1 >= here || next != item.key));
+    const unsigned count = kLanes - __builtin_clzll(last | 1);  // items up to the last that is no padding
+    if (!last) return;
+    const bool goes_on = count == here && after == (uint32_t)__builtin_amdgcn_readlane((int)item.key, here - 1);
+    const bool came = prior == (uint32_t)__builtin_amdgcn_readlane((int)item.key, 0);
+    const bool whole = left >= N;
     facc sum = {};
-    unsigned run = begin;  // where the run being added up begins, or begins in this part
-    for (unsigned j = begin; j < end; ++j) {
-        const uint32_t k = key[j];
-        if (k >= vocab) break;
-        if (left) {
-            const uint32_t i = pos[j];
-            const T *src = copy_of(dout, i / tokens, stride) + (uint64_t)(i % tokens) * dim + first;
-            sum += chunk_to_float<T>(left >= N ? chunk_load(src) : chunk_load_part(src, left));
+    bool from_before = came;
+    for (unsigned j0 = 0; j0 < count; j0 += kAhead) {
+        typename Chunk<T>::vec x[kAhead];
+#pragma unroll
+        for (unsigned u = 0; u < kAhead; ++u) {
+            if (j0 + u >= count) break;
+            const uint64_t o = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(off >> 32), j0 + u) << 32 |
+                               (uint32_t)__builtin_amdgcn_readlane((int)off, j0 + u);
+            const T *src = (const T *)((const char *)dout + o) + first;
+            if (whole) x[u] = chunk_load_stream(src);
+            else x[u] = chunk_load_part(src, left);
         }
-        const bool last = j + 1 == end;
-        if (!last && key[j + 1] == k) continue;
-        const bool from_before = run == begin && begin > 0 && key[begin - 1] == k;
-        const bool goes_on = last && end < n && key[end] == k;
-        if (left) {
-            if (!from_before && !goes_on) {
-                write_row(dtable, stride, k, rows, dim, first, left, sum, scale);
-            } else {
+#pragma unroll
+        for (unsigned u = 0; u < kAhead; ++u) {
+            if (j0 + u >= count) break;
+            sum += chunk_to_float<T>(x[u]);
+            if (!(last >> (j0 + u) & 1)) continue;
+            const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)item.key, j0 + u);
+            if (from_before || (goes_on && j0 + u + 1 == count)) {
                 // slot 0: a sum that came from the part before, slot 1: one that begins here
-                float *c = carry + ((uint64_t)part * 2 + (from_before ? 0 : 1)) * pitch + first;
-                *(facc *)c = sum;
+                if (left) *(facc *)(a.carry + ((uint64_t)part * 2 + (from_before ? 0 : 1)) * a.pitch + first) = sum;
+            } else if (left) {
+                write_row(dtable, a.stride, key, a.rows, a.dim, first, left, sum, a.scale);
             }
+            sum = facc{};
+            from_before = false;
         }
-        sum = facc{};
-        run = j + 1;
-    }
     }
 }
 
+// Zeros for those of kLanes rows that no token names: each lane looks for one of them among the sorted ids.
 template <typename T>
-__global__ __launch_bounds__(64) void embedding_join_kernel(T *dtable, const float *carry, const uint32_t *key, uint64_t stride,
-                                                            unsigned n, unsigned vocab, unsigned rows, unsigned dim,
-                                                            unsigned pitch, float scale) {
+__device__ __forceinline__ void embedding_zero_rows(T *dtable, const SumArgs &a, unsigned group) {
+    const unsigned lane = threadIdx.x;
+    const uint64_t base = (uint64_t)group * a.zero_rows, row = base + lane;
+    const bool mine = lane < a.zero_rows && row < a.vocab;
+    unsigned low = 0, high = a.n;  // the first item whose key is row or more
+    while (low < high) {
+        const unsigned mid = low + (high - low) / 2;
+        if (a.sorted[mid].key < row) low = mid + 1;
+        else high = mid;
+    }
+    const bool named = low < a.n && a.sorted[low].key == row;
+    uint64_t todo = __builtin_amdgcn_ballot_w64(mine && !named);
+    while (todo) {
+        const unsigned from = __builtin_ctzll(todo);
+        const uint64_t rest = ~(todo >> from);
+        unsigned run = rest ? __builtin_ctzll(rest) : kLanes;
+        if (run > kLanes - from) run = kLanes - from;
+        // a PE's rows end where the next one's begin
+        const uint64_t v = base + from;
+        const unsigned owner = (unsigned)(v / a.rows), at = (unsigned)(v % a.rows);
+        if (run > a.rows - at) run = a.rows - at;
+        zero_fill(copy_of(dtable, owner, a.stride) + (uint64_t)at * a.dim, (uint64_t)run * a.dim);
+        todo &= run >= kLanes ? 0 : ~(((1ull << run) - 1) << from);
+    }
+}
+
+// The first sum_blocks blocks add up, the others fill with zeros.
+template <typename T>
+__global__ __launch_bounds__(64) void embedding_sum_kernel(T *dtable, const T *dout, SumArgs a) {
+    if (blockIdx.x < a.sum_blocks) {
+        const uint64_t items = ((uint64_t)a.n + kPart - 1) / kPart * a.pieces;
+        for (uint64_t i = blockIdx.x; i < items; i += a.sum_blocks)
+            embedding_sum_part<T>(dtable, dout, a, (unsigned)(i / a.pieces), (unsigned)(i % a.pieces));
+    } else {
+        embedding_zero_rows<T>(dtable, a, blockIdx.x - a.sum_blocks);
+    }
+}
+
+// A block per part in which a sum begins that goes on behind it; its wavefronts share the parts that the sum goes through.
+constexpr unsigned kJoinWaves = 4;
+
+template <typename T>
+__global__ __launch_bounds__(kJoinWaves *kLanes) void embedding_join_kernel(T *dtable, SumArgs a) {
     constexpr unsigned N = Chunk<T>::N;
     typedef typename Chunk<T>::facc facc;
-    const unsigned first = (blockIdx.x * kLanes + threadIdx.x) * N;
-    if (first >= dim) return;
-    for (unsigned part = blockIdx.y; ((uint64_t)part + 1) * kPart < n; part += gridDim.y) {
-    const unsigned begin = part * kPart, end = begin + kPart;
-    const uint32_t k = key[end - 1];
-    // a run that begins in this part and goes on
-    if (k >= vocab || key[end] != k || (begin > 0 && key[begin - 1] == k)) continue;
-    facc sum = *(const facc *)(carry + ((uint64_t)part * 2 + 1) * pitch + first);
-    for (unsigned q = part + 1; (uint64_t)q * kPart < n && key[q * kPart] == k; ++q)
-        sum += *(const facc *)(carry + (uint64_t)q * 2 * pitch + first);
-    write_row(dtable, stride, k, rows, dim, first, dim - first, sum, scale);
+    __shared__ facc partial[kJoinWaves - 1][kLanes];
+    const unsigned wave = wave_of_block(), lane = threadIdx.x % kLanes;
+    const unsigned parts = (unsigned)(((uint64_t)a.n + kPart - 1) / kPart);
+    for (unsigned part = blockIdx.x; part + 1 < parts; part += gridDim.x) {
+        const unsigned begin = part * kPart, end = begin + kPart;
+        const uint32_t k = a.sorted[end - 1].key;
+        if (k >= a.vocab || a.sorted[end].key != k || (begin > 0 && a.sorted[begin - 1].key == k)) continue;
+        unsigned stop = part + 1;  // the first part that does not begin with k
+        for (;;) {
+            const unsigned q = stop + lane;
+            const uint64_t other = __builtin_amdgcn_ballot_w64(q >= parts || a.sorted[(uint64_t)q * kPart].key != k);
+            if (other) {
+                stop += __builtin_ctzll(other);
+                break;
+            }
+            stop += kLanes;
+        }
+        const unsigned share = (stop - part - 1 + kJoinWaves - 1) / kJoinWaves;
+        const unsigned from = part + 1 + wave * share, to = from + share < stop ? from + share : stop;
+        for (unsigned base = 0; base < a.dim; base += kLanes * N) {
+            const unsigned first = base + lane * N;
+            facc sum = {};
+            if (wave == 0 && first < a.dim) sum = *(const facc *)(a.carry + ((uint64_t)part * 2 + 1) * a.pitch + first);
+            if (first < a.dim) {
+#pragma unroll 8
+                for (unsigned q = from; q < to; ++q) sum += *(const facc *)(a.carry + (uint64_t)q * 2 * a.pitch + first);
+            }
+            if (wave) partial[wave - 1][lane] = sum;
+            __syncthreads();
+            if (wave == 0 && first < a.dim) {
+#pragma unroll
+                for (unsigned w = 0; w < kJoinWaves - 1; ++w) sum += partial[w][lane];
+                write_row(dtable, a.stride, k, a.rows, a.dim, first, a.dim - first, sum, a.scale);
+            }
+            __syncthreads();
+        }
     }
 }
 
@@ -187,16 +374,20 @@ int embedding_on_stream(API *out, const API *table, const int64_t *ids, size_t t
     return launched("embedding");
 }
 
-// The gradient's workspace, in PE 0's copy: keys and positions in sorted order, and two partial sums for every part.
+// The gradient's workspace, in PE 0's copy: the sorted items, twice where they are sorted digit by digit, with the blocks' counts,
+// and two partial sums for every part.
 struct GradSpace {
-    uint64_t key, pos, carry, bytes;
-    unsigned pitch;
-    GradSpace(uint64_t n, uint64_t dim) {
-        const uint64_t list = (n * 4 + 63) / 64 * 64;
+    uint64_t items, hist, carry, bytes;
+    unsigned pitch, passes;
+    GradSpace(uint64_t n, uint64_t vocab, uint64_t dim) {
+        unsigned bits = 1;
+        while (bits < 32 && vocab >> bits) ++bits;  // (vocab itself is the key of padding)
+        passes = n <= kRankTokens ? 0 : (bits + kDigit - 1) / kDigit;
+        const uint64_t list = (n * sizeof(Item) + 63) / 64 * 64;
         pitch = (unsigned)((dim + 7) / 8 * 8);
-        key = 0;
-        pos = list;
-        carry = 2 * list;
+        items = list;
+        hist = passes > 1 ? 2 * list : list;
+        carry = hist + (passes ? kSortBlocks * kBins * sizeof(uint32_t) : 0);
         bytes = carry + (n + kPart - 1) / kPart * 2 * pitch * sizeof(float);
     }
 };
@@ -210,26 +401,46 @@ int embedding_grad_on_stream(API *dtable, const API *dout, const int64_t *ids, v
     if (!ready(rt, "embedding_grad")) return NVSHMEMX_ERROR_INVALID_VALUE;
     if (int rc = check_sizes(rt, "embedding_grad", tokens, vocab, dim, scale)) return rc;
     const size_t rows = (vocab + rt.npes - 1) / rt.npes, n = tokens * rt.npes;
-    const GradSpace space(n, dim);
+    const GradSpace space(n, vocab, dim);
     Operands ops(rt, "embedding_grad");
     const T *src = (const T *)ops.in("dout", dout, (uint64_t)tokens * dim);
     const int64_t *id = ops.in("ids", ids, tokens);
     T *tab = (T *)ops.out("dtable", dtable, (uint64_t)rows * dim);
     char *ws = ops.out("workspace", (char *)workspace, n ? space.bytes : 0, 64);
     if (!ops.ok()) return NVSHMEMX_ERROR_INVALID_VALUE;
-    launch_kernel(embedding_zero_kernel<T>, dim3(1024, 1, rt.npes), dim3(256), 0, stream, tab, rt.heap_size, (unsigned)vocab,
-                  (unsigned)rows, (unsigned)dim);
-    if (n) {
-        uint32_t *key = (uint32_t *)(ws + space.key), *pos = (uint32_t *)(ws + space.pos);
-        float *carry = (float *)(ws + space.carry);
-        const unsigned pieces = div_up(dim, Chunk<T>::N * kLanes), parts = div_up(n, kPart) < 65535 ? div_up(n, kPart) : 65535;
-        launch_kernel(embedding_rank_kernel, dim3(div_up(n, 256)), dim3(256), 0, stream, key, pos, id, rt.heap_size,
+    Item *sorted = (Item *)ws, *other = (Item *)(ws + space.items);
+    if (n && !space.passes) {
+        launch_kernel(embedding_rank_kernel, dim3(div_up(n, kLanes)), dim3(kSortThreads), 0, stream, sorted, id, rt.heap_size,
                       (unsigned)tokens, (unsigned)n, (unsigned)vocab);
-        launch_kernel(embedding_sum_kernel<T>, dim3(pieces, parts), dim3(kLanes), 0, stream, tab, carry, src, key, pos,
-                      rt.heap_size, (unsigned)tokens, (unsigned)n, (unsigned)vocab, (unsigned)rows, (unsigned)dim, space.pitch, scale);
-        launch_kernel(embedding_join_kernel<T>, dim3(pieces, parts), dim3(kLanes), 0, stream, tab, carry, key, rt.heap_size,
-                      (unsigned)n, (unsigned)vocab, (unsigned)rows, (unsigned)dim, space.pitch, scale);
+    } else if (n) {
+        uint32_t *hist = (uint32_t *)(ws + space.hist);
+        const uint64_t tiles = div_up(n, kSortTile);
+        const unsigned per_block = (unsigned)((tiles + kSortBlocks - 1) / kSortBlocks) * kSortTile;
+        const dim3 grid(div_up(n, per_block));
+        Item *out = space.passes % 2 ? sorted : other, *in = space.passes % 2 ? other : sorted;
+        for (unsigned p = 0; p < space.passes; ++p) {
+#define NVSHMEM_AMD_SORT(FIRST)                                                                                                          launch_kernel(embedding_count_kernel<FIRST>, grid, dim3(kSortThreads), 0, stream, hist, in, id, rt.heap_size, (unsigned)tokens,                    (unsigned)n, (unsigned)vocab, per_block, p * kDigit);                                                                  launch_kernel(embedding_sort_kernel<FIRST>, grid, dim3(kSortThreads), 0, stream, out, hist, in, id, rt.heap_size,                                  (unsigned)tokens, (unsigned)n, (unsigned)vocab, per_block, p * kDigit)
+            if (p == 0) {
+                NVSHMEM_AMD_SORT(true);
+            } else {
+                NVSHMEM_AMD_SORT(false);
+            }
+#undef NVSHMEM_AMD_SORT
+            Item *swap = in;
+            in = out, out = swap;
+        }
     }
+    SumArgs a{};
+    a.sorted = sorted, a.carry = (float *)(ws + space.carry), a.stride = rt.heap_size;
+    a.tokens = (unsigned)tokens, a.n = (unsigned)n, a.vocab = (unsigned)vocab, a.rows = (unsigned)rows, a.dim = (unsigned)dim;
+    a.pitch = space.pitch, a.pieces = div_up(dim, Chunk<T>::N * kLanes), a.scale = scale;
+    const uint64_t items = (uint64_t)div_up(n, kPart) * a.pieces;
+    a.sum_blocks = (unsigned)(items < (1u << 22) ? items : 1u << 22);
+    a.zero_rows = kLanes;
+    launch_kernel(embedding_sum_kernel<T>, dim3(a.sum_blocks + div_up(vocab, a.zero_rows)), dim3(kLanes), 0, stream, tab, src, a);
+    if (n > kPart)
+        launch_kernel(embedding_join_kernel<T>, dim3(div_up(n, kPart) < (1u << 20) ? div_up(n, kPart) : 1u << 20), dim3(kJoinWaves * kLanes),
+                      0, stream, tab, a);
     return launched("embedding_grad");
 }
 
@@ -255,9 +466,8 @@ NVSHMEMI_AMD_REPT_FOR_TOKEN_TYPES(NVSHMEM_AMD_EMBEDDING)
 #undef NVSHMEM_AMD_EMBEDDING
 
 size_t nvshmemx_amd_embedding_grad_workspace(size_t tokens, size_t vocab, size_t dim) {
-    (void)vocab;
     const int npes = Runtime::get().npes;
-    return npes < 1 ? 0 : tokens::GradSpace((uint64_t)tokens * npes, dim).bytes;
+    return npes < 1 ? 0 : tokens::GradSpace((uint64_t)tokens * npes, vocab, dim).bytes;
 }
 
 }  // extern "C"

@@ -9,6 +9,7 @@
 //
 // Backward, for upstream dgate and dloss:  q_e = dloss balance_e + (normalise ? 0 : scale dgate_e on S)
 //   dl = p (q - sum q p) + (normalise ? w scale (dgate - sum_S w dgate) on S, w = p / sum_S p : 0)
+#include "counting_sort.hpp"
 #include "token_common.hpp"
 
 namespace nvshmem_amd {
@@ -473,117 +474,99 @@ __global__ __launch_bounds__(kRouteThreads) void route_grad_kernel(T *dlogits, c
 }
 
 // ---- the shuffle's tables ----
-// A stable counting sort of the copies by expert: rows of a destination PE lie in the order (expert, source PE, token, k).
-constexpr unsigned kPlaceThreads = 1024, kPlaceRounds = 8, kPlaceCopies = kPlaceThreads * kPlaceRounds;
-constexpr unsigned kPlaceWaves = kPlaceThreads / kLanes;
+// A stable counting sort of the copies by expert: rows of a destination PE lie in the order (expert, source PE, token, k).  Nothing
+// here is much data; what it costs is waiting, so a block asks for all that it needs from memory at once, at its start.
+constexpr unsigned kPlaceRounds = 8, kPlaceCopies = kSortThreads * kPlaceRounds;
 
-__global__ __launch_bounds__(kPlaceThreads) void place_count_kernel(uint32_t *hist, const int32_t *expert, uint64_t stride,
-                                                                    unsigned copies, unsigned experts) {
+__global__ __launch_bounds__(kSortThreads) void place_count_kernel(uint32_t *hist, const int32_t *expert, uint64_t stride,
+                                                                   unsigned copies, unsigned experts) {
     __shared__ uint32_t count[kMostExperts];
     const unsigned pe = blockIdx.z;
+    const int32_t *mine = copy_of(expert, pe, stride);
+    unsigned to[kPlaceRounds];
+#pragma unroll
+    for (unsigned i = 0; i < kPlaceRounds; ++i) {
+        const unsigned c = blockIdx.x * kPlaceCopies + i * kSortThreads + threadIdx.x;
+        to[i] = c < copies ? (unsigned)mine[c] : ~0u;
+    }
     count[threadIdx.x] = 0;
     __syncthreads();
-    const int32_t *mine = copy_of(expert, pe, stride);
-    for (unsigned i = 0; i < kPlaceRounds; ++i) {
-        const unsigned c = blockIdx.x * kPlaceCopies + i * kPlaceThreads + threadIdx.x;
-        if (c < copies && (unsigned)mine[c] < experts) atomicAdd(&count[mine[c]], 1u);
-    }
+#pragma unroll
+    for (unsigned i = 0; i < kPlaceRounds; ++i)
+        if (to[i] < experts) atomicAdd(&count[to[i]], 1u);
     __syncthreads();
     if (threadIdx.x < experts) copy_of(hist, pe, stride)[(uint64_t)blockIdx.x * experts + threadIdx.x] = count[threadIdx.x];
 }
 
-__global__ __launch_bounds__(kPlaceThreads) void place_kernel(int32_t *dest_pe, int64_t *dest_row, uint64_t *expected,
-                                                              int64_t *expert_row, const uint32_t *hist, const int32_t *expert,
-                                                              const int64_t *counts, uint64_t stride, unsigned copies,
-                                                              unsigned experts, unsigned npes, uint64_t cap) {
-    extern __shared__ uint32_t lds[];  // next[kPlaceWaves][experts]: where a wavefront's next copy to an expert goes
-    __shared__ uint32_t scan[kMostExperts + 1], wave_sum[kPlaceWaves], arriving[NVSHMEMI_AMD_MAX_PES];
-    uint32_t *next = lds;
-    const unsigned pe = blockIdx.z, wave = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
-    const unsigned per_pe = experts / npes;
+__global__ __launch_bounds__(kSortThreads) void place_kernel(int32_t *dest_pe, int64_t *dest_row, uint64_t *expected,
+                                                             int64_t *expert_row, const uint32_t *hist, const int32_t *expert,
+                                                             const int64_t *counts, uint64_t stride, unsigned copies,
+                                                             unsigned experts, unsigned npes, uint64_t cap, unsigned column_log) {
+    extern __shared__ uint32_t lds[];  // stable_places' counts
+    __shared__ uint32_t total[kMostExperts], before[kMostExperts], run[kMostExperts], scan[kMostExperts + 1], wave_sum[kSortWaves];
+    __shared__ uint32_t arriving[NVSHMEMI_AMD_MAX_PES], from[kMostExperts];
+    const unsigned pe = blockIdx.z, per_pe = experts / npes;
     const int32_t *mine = copy_of(expert, pe, stride);
-    // this wavefront's copies, consecutive
-    const unsigned c0 = blockIdx.x * kPlaceCopies + wave * (kPlaceRounds * kLanes) + lane;
-    int32_t to[kPlaceRounds];
+    const unsigned c0 = blockIdx.x * kPlaceCopies + threadIdx.x / kLanes * (kPlaceRounds * kLanes) + threadIdx.x % kLanes;
+    uint32_t to[kPlaceRounds], place[kPlaceRounds];
 #pragma unroll
-    for (unsigned i = 0; i < kPlaceRounds; ++i) to[i] = c0 + i * kLanes < copies ? mine[c0 + i * kLanes] : -1;
-    for (unsigned i = threadIdx.x; i < kPlaceWaves * experts; i += kPlaceThreads) next[i] = 0;
-    if (threadIdx.x < NVSHMEMI_AMD_MAX_PES) arriving[threadIdx.x] = 0;
-
-    // rows of every expert from all sources, from the sources before this one, and from the blocks before this one
-    const unsigned e = threadIdx.x;
-    uint32_t total = 0, before = 0;
+    for (unsigned i = 0; i < kPlaceRounds; ++i) to[i] = c0 + i * kLanes < copies ? (uint32_t)mine[c0 + i * kLanes] : ~0u;
+    // (own expert, source PE), what arrives from there: one pair a thread
+    const unsigned own = threadIdx.x / npes, source = threadIdx.x % npes;
+    const bool pair = blockIdx.x == 0 && own < per_pe;
+    if (pair) from[threadIdx.x] = (uint32_t)copy_of(counts, source, stride)[pe * per_pe + own];
+    // copies to every expert from all sources, and from the sources and blocks in front of this one; threads beyond the experts
+    // share the sources and blocks with those below (column_log: log2 of the experts, rounded up)
+    const unsigned e = threadIdx.x & ((1u << column_log) - 1), share = threadIdx.x >> column_log, shares = kSortThreads >> column_log;
+    uint32_t all = 0, ahead = 0;
     if (e < experts) {
-        for (unsigned src = 0; src < npes; ++src) {
+#pragma unroll 8
+        for (unsigned src = share; src < npes; src += shares) {
             const uint32_t c = (uint32_t)copy_of(counts, src, stride)[e];
-            if (src < pe) before += c;
-            total += c;
+            ahead += src < pe ? c : 0;
+            all += c;
         }
-        const uint32_t *h = hist ? copy_of(hist, pe, stride) : nullptr;
-        for (unsigned b = 0; b < blockIdx.x; ++b) before += h[(uint64_t)b * experts + e];
+        const uint32_t *h = copy_of(hist, pe, stride) + e;
+#pragma unroll 8
+        for (unsigned b = share; b < blockIdx.x; b += shares) ahead += h[(uint64_t)b * experts];
     }
-    uint32_t sum = total;
-    for (int s = 1; s < kLanes; s <<= 1) {
-        const uint32_t up = (uint32_t)__shfl_up((int)sum, s);
-        if ((int)lane >= s) sum += up;
-    }
-    if (lane == kLanes - 1) wave_sum[wave] = sum;
-    __syncthreads();
-    for (unsigned w = 0; w < wave; ++w) sum += wave_sum[w];
-    scan[e + 1] = sum;
-    if (e == 0) scan[0] = 0;
-#pragma unroll
-    for (unsigned i = 0; i < kPlaceRounds; ++i)
-        if ((unsigned)to[i] < experts) atomicAdd(&next[wave * experts + to[i]], 1u);
+    total[threadIdx.x] = before[threadIdx.x] = 0;
+    if (threadIdx.x < NVSHMEMI_AMD_MAX_PES) arriving[threadIdx.x] = 0;
     __syncthreads();
     if (e < experts) {
-        const uint32_t start = scan[e] - scan[e / per_pe * per_pe];
-        uint32_t run = start + before;
-        for (unsigned w = 0; w < kPlaceWaves; ++w) {
-            const uint32_t n = next[w * experts + e];
-            next[w * experts + e] = run;
-            run += n;
-        }
-        if (blockIdx.x == 0 && e / per_pe == pe) {  // what arrives here
-            uint32_t at = start;
-            for (unsigned src = 0; src < npes; ++src) {
-                const uint32_t n = (uint32_t)copy_of(counts, src, stride)[e];
-                const uint64_t room = at < cap ? cap - at : 0;
-                atomicAdd(&arriving[src], n < room ? n : (uint32_t)room);
-                at += n;
-            }
-            int64_t *row = copy_of(expert_row, pe, stride);
-            row[e - pe * per_pe] = start < cap ? start : (int64_t)cap;
-            if (e + 1 == (pe + 1) * per_pe) row[per_pe] = at < cap ? at : (int64_t)cap;
+        atomicAdd(&total[e], all);
+        atomicAdd(&before[e], ahead);
+    }
+    __syncthreads();
+    const uint32_t in_front = scan_block(total[threadIdx.x], wave_sum);
+    scan[threadIdx.x] = in_front;
+    if (threadIdx.x == kSortThreads - 1) scan[kSortThreads] = in_front + total[threadIdx.x];
+    __syncthreads();
+    if (threadIdx.x < experts) run[threadIdx.x] = in_front - scan[threadIdx.x / per_pe * per_pe] + before[threadIdx.x];
+    if (pair) {
+        uint32_t at = scan[pe * per_pe + own] - scan[pe * per_pe];
+        if (source == 0) copy_of(expert_row, pe, stride)[own] = at < cap ? at : (int64_t)cap;
+        for (unsigned s = 0; s < source; ++s) at += from[own * npes + s];
+        const uint32_t n = from[threadIdx.x];
+        const uint64_t room = at < cap ? cap - at : 0;
+        atomicAdd(&arriving[source], n < room ? n : (uint32_t)room);
+        if (threadIdx.x == 0) {
+            const uint32_t rows = scan[(pe + 1) * per_pe] - scan[pe * per_pe];
+            copy_of(expert_row, pe, stride)[per_pe] = rows < cap ? rows : (int64_t)cap;
         }
     }
     __syncthreads();
     if (blockIdx.x == 0 && threadIdx.x < npes) copy_of(expected, pe, stride)[threadIdx.x] = arriving[threadIdx.x];
+    stable_places<kPlaceRounds>(place, to, experts, run, lds);
     int32_t *out_pe = copy_of(dest_pe, pe, stride);
     int64_t *out_row = copy_of(dest_row, pe, stride);
-    const unsigned bits = 32 - __builtin_clz(experts);
-    uint32_t *place = next + wave * experts;
 #pragma unroll
     for (unsigned i = 0; i < kPlaceRounds; ++i) {
-        const bool some = (unsigned)to[i] < experts;
-        // the lanes that send to the same expert
-        uint64_t same = __builtin_amdgcn_ballot_w64(some);
-        for (unsigned b = 0; b < bits; ++b) {
-            const uint64_t set = __builtin_amdgcn_ballot_w64((unsigned)to[i] >> b & 1);
-            same &= (unsigned)to[i] >> b & 1 ? set : ~set;
-        }
-        const unsigned rank = (unsigned)__builtin_popcountll(same & ((1ull << lane) - 1)), n = (unsigned)__builtin_popcountll(same);
-        uint32_t row = 0;
-        if (some) row = place[to[i]] + rank;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (some && rank + 1 == n) place[to[i]] = row + 1;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         const unsigned c = c0 + i * kLanes;
-        if (c < copies) {
-            const bool kept = some && row < cap;
-            out_pe[c] = kept ? (int32_t)((unsigned)to[i] / per_pe) : -1;
-            out_row[c] = kept ? (int64_t)row : -1;
-        }
+        if (c >= copies) continue;
+        const bool kept = to[i] < experts && place[i] < cap;
+        out_pe[c] = kept ? (int32_t)(to[i] / per_pe) : -1;
+        out_row[c] = kept ? (int64_t)place[i] : -1;
     }
 }
 
@@ -713,11 +696,14 @@ int place_on_stream(int32_t *dest_pe, int64_t *dest_row, uint64_t *expected, int
     int64_t *first = ops.out("expert_row", expert_row, (uint64_t)(experts / rt.npes + 1));
     uint32_t *hist = blocks > 1 ? ops.out("workspace", (uint32_t *)workspace, (uint64_t)blocks * experts, 64) : nullptr;
     if (!ops.ok()) return NVSHMEMX_ERROR_INVALID_VALUE;
+    unsigned column_log = 0;
+    while ((1u << column_log) < (unsigned)experts) ++column_log;
     if (blocks > 1)
-        launch_kernel(place_count_kernel, dim3(blocks, 1, rt.npes), dim3(kPlaceThreads), 0, stream, hist, in, rt.heap_size,
+        launch_kernel(place_count_kernel, dim3(blocks, 1, rt.npes), dim3(kSortThreads), 0, stream, hist, in, rt.heap_size,
                       (unsigned)copies, (unsigned)experts);
-    launch_kernel(place_kernel, dim3(blocks, 1, rt.npes), dim3(kPlaceThreads), (size_t)kPlaceWaves * experts * 4, stream, to, row, exp,
-                  first, hist, in, count, rt.heap_size, (unsigned)copies, (unsigned)experts, (unsigned)rt.npes, (uint64_t)recv_cap_rows);
+    launch_kernel(place_kernel, dim3(blocks, 1, rt.npes), dim3(kSortThreads), (size_t)kSortWaves * experts * 4, stream, to, row, exp,
+                  first, hist, in, count, rt.heap_size, (unsigned)copies, (unsigned)experts, (unsigned)rt.npes, (uint64_t)recv_cap_rows,
+                  column_log);
     return launched("moe_place");
 }
 
