@@ -11,49 +11,68 @@ namespace nvshmem_amd {
 namespace tokens {
 namespace {
 
-// Copies of a token whose loads are in flight together.
+// Most copies of a token whose loads are in flight together.
 constexpr int kCopies = 8;
 
-// One wavefront per piece of 64 chunks of a token's row; shorter rows share a wavefront (2^lanes_log lanes each).  Reads every copy
-// once and writes a row: bound by memory.
-template <typename T>
-__global__ __launch_bounds__(64) void combine_sum_kernel(T *out, const T *recv, const float *gate, const int32_t *dest_pe,
-                                                         const int64_t *dest_row, uint64_t stride, uint64_t cap, unsigned tokens,
-                                                         unsigned topk, unsigned dim, unsigned npes, unsigned lanes_log) {
-    constexpr unsigned N = Chunk<T>::N;
-    const unsigned lane = threadIdx.x, pe = blockIdx.z;
-    const unsigned first = (blockIdx.x * kLanes + (lane & ((1u << lanes_log) - 1))) * N;
-    if (first >= dim) return;
-    const unsigned left = dim - first, per_wave = kLanes >> lanes_log;
+// One wavefront per piece of 64 chunks of a token's row, or rows of fewer chunks that share a wavefront, 2^lanes_log lanes each.
+// Reads every copy once and writes a row: bound by memory.  All K loads of a lane leave before the first is used, so neither their
+// addresses nor whether a copy was dropped may be waited for in between: a dropped copy's load goes to the row to be written.
+// Where a wavefront has one token, its entries are scalar loads and its rows scalar addresses.
+template <typename T, int K, int MODE>
+__global__ __launch_bounds__(64) void combine_sum_kernel(T *__restrict__ out, const T *__restrict__ recv, const float *__restrict__ gate,
+                                                         const int32_t *__restrict__ dest_pe, const int64_t *__restrict__ dest_row,
+                                                         uint64_t stride, uint64_t cap, unsigned tokens, unsigned topk, unsigned dim,
+                                                         unsigned npes, unsigned lanes_log) {
+    const unsigned lane = threadIdx.x, pe = blockIdx.z, log = MODE == kWhole ? 6 : lanes_log, per_wave = kLanes >> log;
+    const unsigned c = blockIdx.x * kLanes + (lane & ((1u << log) - 1));
+    if (c * Chunk<T>::N >= dim) return;
+    const unsigned first = chunk_first<T>(c, dim);
     const int32_t *my_pe = copy_of(dest_pe, pe, stride);
     const int64_t *my_row = copy_of(dest_row, pe, stride);
     const float *my_gate = gate ? copy_of(gate, pe, stride) : nullptr;
     T *my_out = copy_of(out, pe, stride);
-    for (uint64_t t = (uint64_t)blockIdx.y * per_wave + (lane >> lanes_log); t < tokens; t += (uint64_t)gridDim.y * per_wave) {
+    for (uint64_t t = (uint64_t)blockIdx.y * per_wave + (MODE == kWhole ? 0 : lane >> log); t < tokens;
+         t += (uint64_t)gridDim.y * per_wave) {
+        T *dst = my_out + t * dim;
         typename Chunk<T>::facc sum = {};
-        for (unsigned k0 = 0; k0 < topk; k0 += kCopies) {
-            typename Chunk<T>::vec x[kCopies];
-            float w[kCopies];
+        for (unsigned k0 = 0; k0 < topk; k0 += K) {
+            // the entries first, all of them; behind the last copy (K is topk where that is less than kCopies) it stands in
+            unsigned d[K];
+            uint64_t r[K];
+            float w[K];
+            uint32_t bits[K];
 #pragma unroll
-            for (unsigned k = 0; k < kCopies; ++k) {
-                w[k] = 0.0f;
-                x[k] = {};
-                if (k0 + k >= topk) continue;
-                const uint64_t c = t * topk + k0 + k;
-                const unsigned d = (unsigned)my_pe[c];
-                const uint64_t r = (uint64_t)my_row[c];
-                if (d >= npes || r >= cap) continue;
-                const T *src = copy_of(recv, d, stride) + r * dim + first;
-                w[k] = my_gate ? my_gate[c] : 1.0f;
-                x[k] = left >= N ? chunk_load_stream(src) : chunk_load_part(src, left);
+            for (unsigned k = 0; k < K; ++k) {
+                const uint64_t e = t * topk + (K < kCopies || k0 + k < topk ? k0 + k : topk - 1);
+                d[k] = (unsigned)my_pe[e];
+                r[k] = (uint64_t)my_row[e];
+                w[k] = 1.0f;
             }
+            if (my_gate) {
 #pragma unroll
-            for (unsigned k = 0; k < kCopies; ++k) sum += chunk_to_float<T>(x[k]) * w[k];
+                for (unsigned k = 0; k < K; ++k) w[k] = my_gate[t * topk + (K < kCopies || k0 + k < topk ? k0 + k : topk - 1)];
+            }
+            const T *src[K];
+#pragma unroll
+            for (unsigned k = 0; k < K; ++k) {
+                const bool ok = (K < kCopies | k0 + k < topk) & (d[k] < npes) & (r[k] < cap);
+                const T *from = copy_of(recv, d[k], stride) + r[k] * dim;
+                src[k] = ok ? from : dst;
+                bits[k] = ok ? ~0u : 0u;
+            }
+            typename Chunk<T>::vec x[K];
+#pragma unroll
+            for (unsigned k = 0; k < K; ++k) x[k] = MODE == kTiny ? chunk_load_part(src[k], dim) : chunk_load_stream(src[k] + first);
+#pragma unroll
+            for (unsigned k = 0; k < K; ++k) {
+                // (a selection would become a branch around the load, with a wait behind it)
+                const nvshmemi_v4u v = __builtin_bit_cast(nvshmemi_v4u, x[k]) & bits[k];
+                sum += chunk_to_float<T>(__builtin_bit_cast(typename Chunk<T>::vec, v)) * w[k];
+            }
         }
-        T *dst = my_out + t * dim + first;
         const typename Chunk<T>::vec y = chunk_from_float<T>(sum);
-        if (left >= N) chunk_store_stream(dst, y);
-        else chunk_store_part(dst, y, left);
+        if (MODE == kTiny) chunk_store_part(dst, y, dim);
+        else chunk_store_stream(dst + first, y);
     }
 }
 
@@ -111,12 +130,6 @@ __global__ __launch_bounds__(256) void combine_grad_kernel(T *drecv, float *dgat
     }
 }
 
-unsigned lanes_log2(size_t chunks) {
-    unsigned l = 0;
-    while (l < 6 && ((size_t)1 << l) < chunks) ++l;
-    return l;
-}
-
 int check_sizes(Runtime &rt, const char *what, size_t tokens, int topk, size_t dim) {
     NVSHMEM_AMD_REFUSE(topk < 1 || topk > 1024, "%s: %d copies of a token, outside [1, 1024]", what, topk);
     NVSHMEM_AMD_REFUSE(tokens > ((size_t)1 << 31) / (size_t)rt.npes, "%s: %zu tokens on %d PEs, at most 2^31 in all", what, tokens, rt.npes);
@@ -143,10 +156,28 @@ int combine_sum_on_stream(API *out, const API *recv, size_t recv_cap_rows, const
     if (!ops.ok()) return NVSHMEMX_ERROR_INVALID_VALUE;
     if (tokens == 0) return 0;
     const size_t chunks = (dim + Chunk<T>::N - 1) / Chunk<T>::N;
-    const unsigned log = lanes_log2(chunks), groups = div_up(tokens, kLanes >> log);
-    launch_kernel(combine_sum_kernel<T>, dim3(div_up(chunks, kLanes), groups < 65535 ? groups : 65535, rt.npes), dim3(kLanes), 0,
-                  stream, dst, src, w, to, at, rt.heap_size, (uint64_t)recv_cap_rows, (unsigned)tokens, (unsigned)topk,
-                  (unsigned)dim, (unsigned)rt.npes, log);
+    const unsigned log = row_lanes_log2(chunks), groups = div_up(tokens, kLanes >> log);
+    const unsigned rows = groups < 65535 ? groups : 65535;
+#define NVSHMEM_AMD_LAUNCH_SUM(K, MODE)                                                                                             \
+    launch_kernel((combine_sum_kernel<T, K, MODE>), dim3(div_up(chunks, kLanes), rows, rt.npes), dim3(kLanes), 0, stream, dst, src, \
+                  w, to, at, rt.heap_size, (uint64_t)recv_cap_rows, (unsigned)tokens, (unsigned)topk, (unsigned)dim,                \
+                  (unsigned)rt.npes, log)
+#define NVSHMEM_AMD_LAUNCH_SUM_OF(MODE)                 \
+    switch (topk) {                                     \
+        case 1: NVSHMEM_AMD_LAUNCH_SUM(1, MODE); break; \
+        case 2: NVSHMEM_AMD_LAUNCH_SUM(2, MODE); break; \
+        case 3: NVSHMEM_AMD_LAUNCH_SUM(3, MODE); break; \
+        case 4: NVSHMEM_AMD_LAUNCH_SUM(4, MODE); break; \
+        case 5: NVSHMEM_AMD_LAUNCH_SUM(5, MODE); break; \
+        case 6: NVSHMEM_AMD_LAUNCH_SUM(6, MODE); break; \
+        case 7: NVSHMEM_AMD_LAUNCH_SUM(7, MODE); break; \
+        default: NVSHMEM_AMD_LAUNCH_SUM(8, MODE);       \
+    }
+    if (dim < (size_t)Chunk<T>::N) NVSHMEM_AMD_LAUNCH_SUM(8, kTiny);
+    else if (log == 6) NVSHMEM_AMD_LAUNCH_SUM_OF(kWhole)
+    else NVSHMEM_AMD_LAUNCH_SUM_OF(kShared)
+#undef NVSHMEM_AMD_LAUNCH_SUM_OF
+#undef NVSHMEM_AMD_LAUNCH_SUM
     return launched("moe_combine_sum");
 }
 

@@ -11,40 +11,57 @@ namespace nvshmem_amd {
 namespace tokens {
 namespace {
 
-// One wavefront per piece of 64 chunks of a row; a row of fewer chunks takes the next power of two lanes and shares its
-// wavefront with others (2^lanes_log lanes a row).  Reads T x dim elements of the table and writes as many: bound by memory.
-template <typename T>
-__global__ __launch_bounds__(64) void embedding_kernel(T *out, const T *table, const int64_t *ids, uint64_t stride,
-                                                       unsigned tokens, unsigned vocab, unsigned rows, unsigned dim,
+// One wavefront per piece of V x 64 chunks of a row; a row of fewer chunks than a wavefront has lanes takes the next power of two of
+// them and shares the wavefront with others (2^lanes_log lanes a row).  Reads a row of the table and writes one: bound by memory.
+// Where a wavefront has one token, its id is a scalar load and its rows are scalar addresses.
+template <typename T, int V, int MODE>
+__global__ __launch_bounds__(64) void embedding_kernel(T *__restrict__ out, const T *__restrict__ table, const int64_t *__restrict__ ids,
+                                                       uint64_t stride, unsigned tokens, unsigned vocab, unsigned rows, unsigned dim,
                                                        unsigned lanes_log, float scale) {
-    constexpr unsigned N = Chunk<T>::N;
-    const unsigned lane = threadIdx.x, pe = blockIdx.z;
-    const unsigned first = (blockIdx.x * kLanes + (lane & ((1u << lanes_log) - 1))) * N;
-    if (first >= dim) return;
-    const unsigned left = dim - first;
+    typedef typename Chunk<T>::vec vec;
+    const unsigned lane = threadIdx.x, pe = blockIdx.z, log = MODE == kWhole ? 6 : lanes_log, per_wave = kLanes >> log;
+    unsigned first[V];
+    bool mine[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const unsigned c = (blockIdx.x * V + v) * kLanes + (lane & ((1u << log) - 1));
+        first[v] = chunk_first<T>(c, dim), mine[v] = c * Chunk<T>::N < dim;
+    }
+    if (!mine[0]) return;
     const int64_t *my_ids = copy_of(ids, pe, stride);
     T *my_out = copy_of(out, pe, stride);
-    const unsigned per_wave = kLanes >> lanes_log;
-    for (uint64_t t = (uint64_t)blockIdx.y * per_wave + (lane >> lanes_log); t < tokens; t += (uint64_t)gridDim.y * per_wave) {
+    for (uint64_t t = (uint64_t)blockIdx.y * per_wave + (MODE == kWhole ? 0 : lane >> log); t < tokens;
+         t += (uint64_t)gridDim.y * per_wave) {
         const uint64_t id = (uint64_t)my_ids[t];
-        typename Chunk<T>::facc x = {};
+        T *dst = my_out + t * dim;
+        vec x[V] = {};
         if (id < vocab) {
             const unsigned owner = (unsigned)id / rows, row = (unsigned)id % rows;
-            const T *src = copy_of(table, owner, stride) + (uint64_t)row * dim + first;
-            x = chunk_to_float<T>(left >= N ? chunk_load(src) : chunk_load_part(src, left));
+            const T *src = copy_of(table, owner, stride) + (uint64_t)row * dim;
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (MODE == kTiny) x[v] = chunk_load_part(src, dim);
+                else if (v == 0 || mine[v]) x[v] = chunk_load(src + first[v]);
         }
-        const typename Chunk<T>::vec y = chunk_from_float<T>(x * scale);
-        T *dst = my_out + t * dim + first;
-        if (left >= N) chunk_store_stream(dst, y);
-        else chunk_store_part(dst, y, left);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const vec y = chunk_from_float<T>(chunk_to_float<T>(x[v]) * scale);
+            if (MODE == kTiny) chunk_store_part(dst, y, dim);
+            else if (v == 0 || mine[v]) chunk_store_stream(dst + first[v], y);
+        }
     }
 }
 
 // ---- gradient ----
-// The tokens of all PEs are sorted by id, stable; a wavefront adds up kPart consecutive ones of a piece of a row, in order, and
+// The tokens of all PEs are sorted by id, stable; a wavefront adds up a part of consecutive ones, of a piece of a row, in order, and
 // writes the sums of the ids that lie in its part as a whole.  A sum that goes on into the next part leaves a partial sum in fp32
 // (`carry`), and a kernel behind it adds those up, in order: nothing depends on which block comes first.
-constexpr unsigned kPart = 32;
+constexpr unsigned kLeastPart = 8, kMostPart = kLanes;
+unsigned part_of(uint64_t n) {
+    unsigned part = kLeastPart;
+    while (part < kMostPart && n / 256 > part) part *= 2;
+    return part;
+}
 
 // A token: its id (vocab: padding, sorted behind all ids) and its number pe * tokens + t.
 struct Item {
@@ -93,7 +110,7 @@ __global__ __launch_bounds__(kSortThreads) void embedding_rank_kernel(Item *sort
 }
 
 // More tokens: counting sorts by kDigit bits of the id at a time, lowest first, of at most kSortBlocks blocks of consecutive tokens.
-constexpr unsigned kDigit = 9, kBins = 1u << kDigit, kSortBlocks = 64, kSortRounds = 4, kSortTile = kSortThreads * kSortRounds;
+constexpr unsigned kDigit = 9, kBins = 1u << kDigit, kSortBlocks = 64, kSortRounds = 2, kSortTile = kSortThreads * kSortRounds;
 
 template <bool FIRST>
 __device__ __forceinline__ Item item_of(const Item *in, const int64_t *ids, uint64_t stride, unsigned tokens, unsigned vocab,
@@ -121,10 +138,22 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(Item *out,
                                                                       const int64_t *ids, uint64_t stride, unsigned tokens, unsigned n,
                                                                       unsigned vocab, unsigned per_block, unsigned shift) {
     __shared__ uint32_t count[kSortWaves * kBins], run[kBins], wave_sum[kSortWaves], half[2][kBins];
+    const uint64_t begin = (uint64_t)blockIdx.x * per_block, end = begin + per_block < n ? begin + per_block : n;
+    Item item[kSortRounds];
+    uint32_t to[kSortRounds], place[kSortRounds];
+    auto fetch = [&](uint64_t tile) {
+#pragma unroll
+        for (unsigned r = 0; r < kSortRounds; ++r) {
+            const uint64_t i = tile + threadIdx.x / kLanes * (kSortRounds * kLanes) + r * kLanes + threadIdx.x % kLanes;
+            item[r] = i < end ? item_of<FIRST>(in, ids, stride, tokens, vocab, (unsigned)i) : Item{0, 0};
+            to[r] = i < end ? item[r].key >> shift & (kBins - 1) : kBins;
+        }
+    };
+    fetch(begin);  // (in flight while the counts are)
     // items of each bin in all blocks, and in those before this one: two threads a bin
     const unsigned bin = threadIdx.x % kBins;
     uint32_t total = 0, before = 0;
-#pragma unroll 8
+#pragma unroll 16
     for (unsigned b = threadIdx.x / kBins; b < gridDim.x; b += kSortThreads / kBins) {
         const uint32_t c = hist[b * kBins + bin];
         total += c;
@@ -139,19 +168,8 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(Item *out,
     total = first ? total + half[0][bin] : 0;
     const uint32_t start = scan_block(total, wave_sum);
     if (first) run[bin] = start + before + half[1][bin];
-    const uint64_t begin = (uint64_t)blockIdx.x * per_block, end = begin + per_block < n ? begin + per_block : n;
-    for (uint64_t t = begin; t < end; t += kSortTile) {
-        Item item[kSortRounds];
-        uint32_t to[kSortRounds], place[kSortRounds];
-#pragma unroll
-        for (unsigned r = 0; r < kSortRounds; ++r) {
-            const uint64_t i = t + threadIdx.x / kLanes * (kSortRounds * kLanes) + r * kLanes + threadIdx.x % kLanes;
-            to[r] = kBins;
-            if (i < end) {
-                item[r] = item_of<FIRST>(in, ids, stride, tokens, vocab, (unsigned)i);
-                to[r] = item[r].key >> shift & (kBins - 1);
-            }
-        }
+    for (uint64_t tile = begin; tile < end; tile += kSortTile) {
+        if (tile != begin) fetch(tile);
         __syncthreads();
         stable_places<kSortRounds>(place, to, kBins, run, count);
 #pragma unroll
@@ -163,18 +181,23 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(Item *out,
 
 template <typename T>
 __device__ __forceinline__ void write_row(T *dtable, uint64_t stride, uint32_t key, unsigned rows, unsigned dim, unsigned first,
-                                          unsigned left, typename Chunk<T>::facc sum, float scale) {
+                                          typename Chunk<T>::facc sum, float scale) {
     T *dst = copy_of(dtable, key / rows, stride) + (uint64_t)(key % rows) * dim + first;
     const typename Chunk<T>::vec y = chunk_from_float<T>(sum * scale);
-    if (left >= (unsigned)Chunk<T>::N) chunk_store_stream(dst, y);
-    else chunk_store_part(dst, y, left);
+    if (dim < (unsigned)Chunk<T>::N) chunk_store_part(dst, y, dim);
+    else chunk_store_stream(dst, y);
 }
+// A partial sum's chunk, at any element.
+template <typename T>
+struct Partial {
+    typedef typename Chunk<T>::facc type __attribute__((aligned(4)));
+};
 
 struct SumArgs {
     const Item *sorted;
     float *carry;
     uint64_t stride;
-    unsigned tokens, n, vocab, rows, dim, pitch, pieces, sum_blocks, zero_rows;
+    unsigned tokens, n, part, parts, vocab, rows, dim, pitch, pieces, sum_blocks, zero_rows;
     float scale;
 };
 
@@ -202,8 +225,9 @@ template <typename T>
 __device__ __forceinline__ void embedding_sum_part(T *dtable, const T *dout, const SumArgs &a, unsigned part, unsigned piece) {
     constexpr unsigned N = Chunk<T>::N;
     typedef typename Chunk<T>::facc facc;
-    const unsigned lane = threadIdx.x, first = (piece * kLanes + lane) * N, left = first < a.dim ? a.dim - first : 0;
-    const unsigned begin = part * kPart, here = a.n - begin < kPart ? a.n - begin : kPart;
+    const unsigned lane = threadIdx.x, c = piece * kLanes + lane, first = chunk_first<T>(c, a.dim);
+    const bool mine = c * N < a.dim, row_part = a.dim < N;
+    const unsigned begin = part * a.part, here = a.n - begin < a.part ? a.n - begin : a.part;
     // lane j looks at item j: where its row is, and whether it is the last of its id
     Item item = {a.vocab, 0};
     uint32_t after = a.vocab, prior = a.vocab;
@@ -218,7 +242,6 @@ __device__ __forceinline__ void embedding_sum_part(T *dtable, const T *dout, con
     if (!last) return;
     const bool goes_on = count == here && after == (uint32_t)__builtin_amdgcn_readlane((int)item.key, here - 1);
     const bool came = prior == (uint32_t)__builtin_amdgcn_readlane((int)item.key, 0);
-    const bool whole = left >= N;
     facc sum = {};
     bool from_before = came;
     for (unsigned j0 = 0; j0 < count; j0 += kAhead) {
@@ -229,8 +252,7 @@ __device__ __forceinline__ void embedding_sum_part(T *dtable, const T *dout, con
             const uint64_t o = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(off >> 32), j0 + u) << 32 |
                                (uint32_t)__builtin_amdgcn_readlane((int)off, j0 + u);
             const T *src = (const T *)((const char *)dout + o) + first;
-            if (whole) x[u] = chunk_load_stream(src);
-            else x[u] = chunk_load_part(src, left);
+            x[u] = row_part ? chunk_load_part(src, a.dim) : chunk_load_stream(src);
         }
 #pragma unroll
         for (unsigned u = 0; u < kAhead; ++u) {
@@ -240,9 +262,9 @@ __device__ __forceinline__ void embedding_sum_part(T *dtable, const T *dout, con
             const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)item.key, j0 + u);
             if (from_before || (goes_on && j0 + u + 1 == count)) {
                 // slot 0: a sum that came from the part before, slot 1: one that begins here
-                if (left) *(facc *)(a.carry + ((uint64_t)part * 2 + (from_before ? 0 : 1)) * a.pitch + first) = sum;
-            } else if (left) {
-                write_row(dtable, a.stride, key, a.rows, a.dim, first, left, sum, a.scale);
+                if (mine) *(typename Partial<T>::type *)(a.carry + ((uint64_t)part * 2 + (from_before ? 0 : 1)) * a.pitch + first) = sum;
+            } else if (mine) {
+                write_row(dtable, a.stride, key, a.rows, a.dim, first, sum, a.scale);
             }
             sum = facc{};
             from_before = false;
@@ -250,31 +272,58 @@ __device__ __forceinline__ void embedding_sum_part(T *dtable, const T *dout, con
     }
 }
 
-// Zeros for those of kLanes rows that no token names: each lane looks for one of them among the sorted ids.
+// The number of items whose key is less than `key`, by a wavefront that looks at 64 places at a time.
+__device__ __forceinline__ unsigned items_below(const Item *sorted, unsigned n, uint64_t key) {
+    const unsigned lane = threadIdx.x % kLanes;
+    unsigned low = 0;  // all items in front of low are less, all from low + left on are not
+    for (unsigned left = n; left;) {
+        const unsigned step = (left + kLanes - 1) / kLanes;
+        // lane l looks at the last item of its `step` ones: if that is less, so are the others
+        const uint64_t at = (uint64_t)(lane + 1) * step - 1;
+        const bool less = at < left && sorted[low + at].key < key;
+        const unsigned steps = __builtin_popcountll(__builtin_amdgcn_ballot_w64(less));
+        low += steps * step;
+        left -= steps * step;
+        // the item that ends the next ones is not less
+        left = left < step - 1 ? left : step - 1;
+    }
+    return low;
+}
+
+// Zeros for those of zero_rows (at most 64) rows that no token names.
 template <typename T>
 __device__ __forceinline__ void embedding_zero_rows(T *dtable, const SumArgs &a, unsigned group) {
     const unsigned lane = threadIdx.x;
-    const uint64_t base = (uint64_t)group * a.zero_rows, row = base + lane;
-    const bool mine = lane < a.zero_rows && row < a.vocab;
-    unsigned low = 0, high = a.n;  // the first item whose key is row or more
-    while (low < high) {
-        const unsigned mid = low + (high - low) / 2;
-        if (a.sorted[mid].key < row) low = mid + 1;
-        else high = mid;
+    const uint64_t base = (uint64_t)group * a.zero_rows;
+    const unsigned rows = a.vocab - base < a.zero_rows ? (unsigned)(a.vocab - base) : a.zero_rows;
+    const unsigned begin = items_below(a.sorted, a.n, base);
+    const uint64_t key = begin + lane < a.n ? a.sorted[begin + lane].key : a.vocab;
+    uint64_t named = 0;
+    if (__builtin_amdgcn_ballot_w64(key >= base + rows)) {  // all of these rows' items are in sight
+        const uint32_t prior = (uint32_t)__shfl_up((int)(uint32_t)key, 1);
+        uint64_t heads = __builtin_amdgcn_ballot_w64(key < base + rows && (lane == 0 || prior != key));
+        for (; heads; heads &= heads - 1)
+            named |= 1ull << ((uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)key, __builtin_ctzll(heads)) - (uint32_t)base);
+    } else {  // many tokens to a row: each lane looks for one row
+        unsigned low = begin, high = a.n;
+        while (low < high) {
+            const unsigned mid = low + (high - low) / 2;
+            if (a.sorted[mid].key < base + lane) low = mid + 1;
+            else high = mid;
+        }
+        named = __builtin_amdgcn_ballot_w64(low < a.n && a.sorted[low].key == base + lane);
     }
-    const bool named = low < a.n && a.sorted[low].key == row;
-    uint64_t todo = __builtin_amdgcn_ballot_w64(mine && !named);
+    uint64_t todo = ~named & (rows < 64 ? (1ull << rows) - 1 : ~0ull);
     while (todo) {
-        const unsigned from = __builtin_ctzll(todo);
-        const uint64_t rest = ~(todo >> from);
+        const unsigned first = __builtin_ctzll(todo);
+        const uint64_t rest = ~(todo >> first);
         unsigned run = rest ? __builtin_ctzll(rest) : kLanes;
-        if (run > kLanes - from) run = kLanes - from;
         // a PE's rows end where the next one's begin
-        const uint64_t v = base + from;
+        const uint64_t v = base + first;
         const unsigned owner = (unsigned)(v / a.rows), at = (unsigned)(v % a.rows);
         if (run > a.rows - at) run = a.rows - at;
         zero_fill(copy_of(dtable, owner, a.stride) + (uint64_t)at * a.dim, (uint64_t)run * a.dim);
-        todo &= run >= kLanes ? 0 : ~(((1ull << run) - 1) << from);
+        todo &= run >= kLanes ? 0 : ~(((1ull << run) - 1) << first);
     }
 }
 
@@ -282,7 +331,7 @@ __device__ __forceinline__ void embedding_zero_rows(T *dtable, const SumArgs &a,
 template <typename T>
 __global__ __launch_bounds__(64) void embedding_sum_kernel(T *dtable, const T *dout, SumArgs a) {
     if (blockIdx.x < a.sum_blocks) {
-        const uint64_t items = ((uint64_t)a.n + kPart - 1) / kPart * a.pieces;
+        const uint64_t items = (uint64_t)a.parts * a.pieces;
         for (uint64_t i = blockIdx.x; i < items; i += a.sum_blocks)
             embedding_sum_part<T>(dtable, dout, a, (unsigned)(i / a.pieces), (unsigned)(i % a.pieces));
     } else {
@@ -295,19 +344,20 @@ constexpr unsigned kJoinWaves = 4;
 
 template <typename T>
 __global__ __launch_bounds__(kJoinWaves *kLanes) void embedding_join_kernel(T *dtable, SumArgs a) {
-    constexpr unsigned N = Chunk<T>::N;
     typedef typename Chunk<T>::facc facc;
+    typedef typename Partial<T>::type stored;
     __shared__ facc partial[kJoinWaves - 1][kLanes];
     const unsigned wave = wave_of_block(), lane = threadIdx.x % kLanes;
-    const unsigned parts = (unsigned)(((uint64_t)a.n + kPart - 1) / kPart);
-    for (unsigned part = blockIdx.x; part + 1 < parts; part += gridDim.x) {
-        const unsigned begin = part * kPart, end = begin + kPart;
-        const uint32_t k = a.sorted[end - 1].key;
-        if (k >= a.vocab || a.sorted[end].key != k || (begin > 0 && a.sorted[begin - 1].key == k)) continue;
+    const unsigned c = blockIdx.y * kLanes + lane, first = chunk_first<T>(c, a.dim);
+    const bool mine = c * Chunk<T>::N < a.dim;
+    for (unsigned part = blockIdx.x; part + 1 < a.parts; part += gridDim.x) {
+        const unsigned begin = part * a.part, end = begin + a.part;
+        const uint32_t k = a.sorted[end - 1].key, after = a.sorted[end].key, prior = a.sorted[begin > 0 ? begin - 1 : 0].key;
+        if (k >= a.vocab || after != k || (begin > 0 && prior == k)) continue;
         unsigned stop = part + 1;  // the first part that does not begin with k
         for (;;) {
             const unsigned q = stop + lane;
-            const uint64_t other = __builtin_amdgcn_ballot_w64(q >= parts || a.sorted[(uint64_t)q * kPart].key != k);
+            const uint64_t other = __builtin_amdgcn_ballot_w64(q >= a.parts || a.sorted[(uint64_t)q * a.part].key != k);
             if (other) {
                 stop += __builtin_ctzll(other);
                 break;
@@ -316,32 +366,26 @@ __global__ __launch_bounds__(kJoinWaves *kLanes) void embedding_join_kernel(T *d
         }
         const unsigned share = (stop - part - 1 + kJoinWaves - 1) / kJoinWaves;
         const unsigned from = part + 1 + wave * share, to = from + share < stop ? from + share : stop;
-        for (unsigned base = 0; base < a.dim; base += kLanes * N) {
-            const unsigned first = base + lane * N;
-            facc sum = {};
-            if (wave == 0 && first < a.dim) sum = *(const facc *)(a.carry + ((uint64_t)part * 2 + 1) * a.pitch + first);
-            if (first < a.dim) {
+        facc sum = {};
+        if (mine) {
+            if (wave == 0) sum = *(const stored *)(a.carry + ((uint64_t)part * 2 + 1) * a.pitch + first);
 #pragma unroll 8
-                for (unsigned q = from; q < to; ++q) sum += *(const facc *)(a.carry + (uint64_t)q * 2 * a.pitch + first);
-            }
-            if (wave) partial[wave - 1][lane] = sum;
-            __syncthreads();
-            if (wave == 0 && first < a.dim) {
-#pragma unroll
-                for (unsigned w = 0; w < kJoinWaves - 1; ++w) sum += partial[w][lane];
-                write_row(dtable, a.stride, k, a.rows, a.dim, first, a.dim - first, sum, a.scale);
-            }
-            __syncthreads();
+            for (unsigned q = from; q < to; ++q) sum += *(const stored *)(a.carry + (uint64_t)q * 2 * a.pitch + first);
         }
+        if (wave) partial[wave - 1][lane] = sum;
+        __syncthreads();
+        if (wave == 0 && mine) {
+#pragma unroll
+            for (unsigned w = 0; w < kJoinWaves - 1; ++w) sum += partial[w][lane];
+            write_row(dtable, a.stride, k, a.rows, a.dim, first, sum, a.scale);
+        }
+        __syncthreads();
     }
 }
 
-unsigned lanes_log2(size_t chunks) {
-    unsigned l = 0;
-    while (l < 6 && ((size_t)1 << l) < chunks) ++l;
-    return l;
-}
-
+#ifndef VV
+#define VV 2
+#endif
 constexpr size_t kMostTokens = (size_t)1 << 31;
 
 int check_sizes(Runtime &rt, const char *what, size_t tokens, size_t vocab, size_t dim, float scale) {
@@ -368,9 +412,16 @@ int embedding_on_stream(API *out, const API *table, const int64_t *ids, size_t t
     if (!ops.ok()) return NVSHMEMX_ERROR_INVALID_VALUE;
     if (tokens == 0) return 0;
     const size_t chunks = (dim + Chunk<T>::N - 1) / Chunk<T>::N;
-    const unsigned log = lanes_log2(chunks), groups = div_up(tokens, kLanes >> log);
-    launch_kernel(embedding_kernel<T>, dim3(div_up(chunks, kLanes), groups < 65535 ? groups : 65535, rt.npes), dim3(kLanes), 0,
-                  stream, dst, tab, id, rt.heap_size, (unsigned)tokens, (unsigned)vocab, (unsigned)rows, (unsigned)dim, log, scale);
+    const unsigned log = row_lanes_log2(chunks), groups = div_up(tokens, kLanes >> log);
+    const unsigned most = groups < 65535 ? groups : 65535;
+#define NVSHMEM_AMD_LAUNCH_EMBEDDING(V, MODE)                                                                                          \
+    launch_kernel((embedding_kernel<T, V, MODE>), dim3(div_up(chunks, kLanes * V), most, rt.npes), dim3(kLanes), 0, stream, dst, tab,  \
+                  id, rt.heap_size, (unsigned)tokens, (unsigned)vocab, (unsigned)rows, (unsigned)dim, log, scale)
+    if (dim < (size_t)Chunk<T>::N) NVSHMEM_AMD_LAUNCH_EMBEDDING(1, kTiny);
+    else if (chunks > kLanes) NVSHMEM_AMD_LAUNCH_EMBEDDING(VV, kWhole);
+    else if (log == 6) NVSHMEM_AMD_LAUNCH_EMBEDDING(1, kWhole);
+    else NVSHMEM_AMD_LAUNCH_EMBEDDING(1, kShared);
+#undef NVSHMEM_AMD_LAUNCH_EMBEDDING
     return launched("embedding");
 }
 
@@ -378,17 +429,18 @@ int embedding_on_stream(API *out, const API *table, const int64_t *ids, size_t t
 // and two partial sums for every part.
 struct GradSpace {
     uint64_t items, hist, carry, bytes;
-    unsigned pitch, passes;
+    unsigned pitch, passes, part;
     GradSpace(uint64_t n, uint64_t vocab, uint64_t dim) {
         unsigned bits = 1;
         while (bits < 32 && vocab >> bits) ++bits;  // (vocab itself is the key of padding)
         passes = n <= kRankTokens ? 0 : (bits + kDigit - 1) / kDigit;
         const uint64_t list = (n * sizeof(Item) + 63) / 64 * 64;
         pitch = (unsigned)((dim + 7) / 8 * 8);
+        part = part_of(n);
         items = list;
         hist = passes > 1 ? 2 * list : list;
         carry = hist + (passes ? kSortBlocks * kBins * sizeof(uint32_t) : 0);
-        bytes = carry + (n + kPart - 1) / kPart * 2 * pitch * sizeof(float);
+        bytes = carry + (n + part - 1) / part * 2 * pitch * sizeof(float);
     }
 };
 
@@ -434,13 +486,14 @@ int embedding_grad_on_stream(API *dtable, const API *dout, const int64_t *ids, v
     a.sorted = sorted, a.carry = (float *)(ws + space.carry), a.stride = rt.heap_size;
     a.tokens = (unsigned)tokens, a.n = (unsigned)n, a.vocab = (unsigned)vocab, a.rows = (unsigned)rows, a.dim = (unsigned)dim;
     a.pitch = space.pitch, a.pieces = div_up(dim, Chunk<T>::N * kLanes), a.scale = scale;
-    const uint64_t items = (uint64_t)div_up(n, kPart) * a.pieces;
+    a.part = space.part, a.parts = div_up(n, space.part);
+    const uint64_t items = (uint64_t)a.parts * a.pieces;
     a.sum_blocks = (unsigned)(items < (1u << 22) ? items : 1u << 22);
     a.zero_rows = kLanes;
     launch_kernel(embedding_sum_kernel<T>, dim3(a.sum_blocks + div_up(vocab, a.zero_rows)), dim3(kLanes), 0, stream, tab, src, a);
-    if (n > kPart)
-        launch_kernel(embedding_join_kernel<T>, dim3(div_up(n, kPart) < (1u << 20) ? div_up(n, kPart) : 1u << 20), dim3(kJoinWaves * kLanes),
-                      0, stream, tab, a);
+    if (a.parts > 1)
+        launch_kernel(embedding_join_kernel<T>, dim3(a.parts < (1u << 20) ? a.parts : 1u << 20, a.pieces), dim3(kJoinWaves * kLanes), 0,
+                      stream, tab, a);
     return launched("embedding_grad");
 }
 

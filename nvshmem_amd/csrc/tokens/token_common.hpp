@@ -57,7 +57,18 @@ template <typename T>
 __device__ __forceinline__ void chunk_store_stream(T *p, typename Chunk<T>::vec v) {
     __builtin_nontemporal_store(v, reinterpret_cast<typename Chunk<T>::vec_unaligned *>(p));
 }
-// The first `n` elements of a chunk that a row ends in (the rest: zeros).
+// How a row's chunks lie on lanes: a wavefront and more to a row, rows that share a wavefront, rows of less than a chunk (which
+// share one as well).
+enum { kWhole, kShared, kTiny };
+
+// Where chunk c of a row begins.  The last one ends with the row and so may share elements with the one in front of it: what is
+// computed for an element depends on the element alone, so both store the same bits, and every access is a whole vector.
+// Rows of less than a chunk have one, of `dim` elements, which the _part functions move.
+template <typename T>
+__device__ __forceinline__ unsigned chunk_first(unsigned c, unsigned dim) {
+    const unsigned first = c * Chunk<T>::N, most = dim < (unsigned)Chunk<T>::N ? 0 : dim - Chunk<T>::N;
+    return first < most ? first : most;
+}
 template <typename T>
 __device__ __forceinline__ typename Chunk<T>::vec chunk_load_part(const T *p, unsigned n) {
     typename Chunk<T>::vec v;
@@ -175,6 +186,12 @@ inline int launched(const char *what) {
         }                                            \
     } while (0)
 
+// The least power of two of lanes (its logarithm, at most a wavefront) that a row of so many chunks fills.
+inline unsigned row_lanes_log2(size_t chunks) {
+    unsigned l = 0;
+    while (l < 6 && ((size_t)1 << l) < chunks) ++l;
+    return l;
+}
 inline unsigned div_up(uint64_t a, uint64_t b) { return (unsigned)((a + b - 1) / b); }
 
 }  // namespace tokens
