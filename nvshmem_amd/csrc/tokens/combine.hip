@@ -11,6 +11,15 @@ namespace nvshmem_amd {
 namespace tokens {
 namespace {
 
+template <int SIZE>
+struct same_size {
+    typedef uint16_t type;
+};
+template <>
+struct same_size<4> {
+    typedef uint32_t type;
+};
+
 // Most copies of a token whose loads are in flight together.
 constexpr int kCopies = 8;
 
@@ -76,55 +85,91 @@ __global__ __launch_bounds__(64) void combine_sum_kernel(T *__restrict__ out, co
     }
 }
 
-// A block per token.  A thread keeps the products of its chunks for up to kCopies gates in registers; the block adds them up at
-// the end, lane by lane and then wavefront by wavefront.
-template <typename T>
-__global__ __launch_bounds__(256) void combine_grad_kernel(T *drecv, float *dgate, const T *dout, const T *recv, const float *gate,
-                                                           const int32_t *dest_pe, const int64_t *dest_row, uint64_t stride,
-                                                           uint64_t cap, unsigned tokens, unsigned topk, unsigned dim,
-                                                           unsigned npes) {
+// A block of up to 8 wavefronts per token.  A lane loads a chunk of all K copies before it uses the first or stores any (drecv may be
+// recv), and keeps the products for the K gates in registers; they are added up lane by lane and then wavefront by wavefront.
+constexpr unsigned kGradWaves = 8;
+
+template <typename T, int K, bool TINY>
+__global__ __launch_bounds__(kGradWaves *kLanes) void combine_grad_kernel(T *drecv, float *__restrict__ dgate, const T *__restrict__ dout,
+                                                                          const T *recv, const float *__restrict__ gate,
+                                                                          const int32_t *__restrict__ dest_pe,
+                                                                          const int64_t *__restrict__ dest_row, uint64_t stride,
+                                                                          uint64_t cap, unsigned tokens, unsigned topk, unsigned dim,
+                                                                          unsigned npes) {
     constexpr unsigned N = Chunk<T>::N;
-    __shared__ float partial[4][kCopies];
-    const unsigned pe = blockIdx.z;
+    typedef typename Chunk<T>::vec vec;
+    typedef typename Chunk<T>::facc facc;
+    __shared__ float partial[kGradWaves][K];
+    const unsigned pe = blockIdx.z, wave = wave_of_block(), waves = blockDim.x / kLanes, lane = threadIdx.x % kLanes;
     const int32_t *my_pe = copy_of(dest_pe, pe, stride);
     const int64_t *my_row = copy_of(dest_row, pe, stride);
     const float *my_gate = copy_of(gate, pe, stride);
     const T *my_dout = copy_of(dout, pe, stride);
     float *my_dgate = copy_of(dgate, pe, stride);
-    for (uint64_t t = (uint64_t)blockIdx.y * gridDim.x + blockIdx.x; t < tokens; t += (uint64_t)gridDim.y * gridDim.x) {
-        for (unsigned k0 = 0; k0 < topk; k0 += kCopies) {
-            float dot[kCopies] = {};
-            for (unsigned first = threadIdx.x * N; first < dim; first += 256 * N) {
-                const unsigned left = dim - first;
-                const T *from = my_dout + t * dim + first;
-                const typename Chunk<T>::facc g = chunk_to_float<T>(left >= N ? chunk_load(from) : chunk_load_part(from, left));
+    for (uint64_t t = blockIdx.x; t < tokens; t += gridDim.x) {
+        const T *from = my_dout + t * dim;
+        for (unsigned k0 = 0; k0 < topk; k0 += K) {
+            // the entries; behind the last copy (K is topk where that is less than kCopies) it stands in
+            unsigned d[K];
+            uint64_t r[K];
+            float w[K];
 #pragma unroll
-                for (unsigned k = 0; k < kCopies; ++k) {
-                    if (k0 + k >= topk) continue;
-                    const uint64_t c = t * topk + k0 + k;
-                    const unsigned d = (unsigned)my_pe[c];
-                    const uint64_t r = (uint64_t)my_row[c];
-                    if (d >= npes || r >= cap) continue;
-                    const uint64_t at = r * dim + first;
-                    const T *src = copy_of(recv, d, stride) + at;
-                    const typename Chunk<T>::facc x = chunk_to_float<T>(left >= N ? chunk_load(src) : chunk_load_part(src, left));
+            for (unsigned k = 0; k < K; ++k) {
+                const uint64_t e = t * topk + (K < kCopies || k0 + k < topk ? k0 + k : topk - 1);
+                d[k] = (unsigned)my_pe[e];
+                r[k] = (uint64_t)my_row[e];
+                w[k] = my_gate[e];
+            }
+            const T *src[K];
+            T *dst[K];
+            unsigned ok = 0;
 #pragma unroll
-                    for (unsigned i = 0; i < N; ++i) dot[k] = __builtin_fmaf(x[i], g[i], dot[k]);
-                    T *dst = copy_of(drecv, d, stride) + at;
-                    const typename Chunk<T>::vec y = chunk_from_float<T>(g * my_gate[c]);
-                    if (left >= N) chunk_store_stream(dst, y);
-                    else chunk_store_part(dst, y, left);
+            for (unsigned k = 0; k < K; ++k) {
+                const bool there = (K < kCopies | k0 + k < topk) & (d[k] < npes) & (r[k] < cap);
+                const T *x = copy_of(recv, d[k], stride) + r[k] * dim;
+                src[k] = there ? x : from;
+                dst[k] = copy_of(drecv, d[k], stride) + r[k] * dim;
+                ok |= there ? 1u << k : 0u;
+            }
+            float dot[K] = {};
+            for (unsigned c = wave * kLanes + lane; c * N < dim; c += waves * kLanes) {
+                const unsigned first = chunk_first<T>(c, dim), shared = c * N - first;
+                vec x[K];
+#pragma unroll
+                for (unsigned k = 0; k < K; ++k) x[k] = TINY ? chunk_load_part(src[k], dim) : chunk_load_stream(src[k] + first);
+                const facc g = chunk_to_float<T>(TINY ? chunk_load_part(from, dim) : chunk_load(from + first));
+                // elements that the chunk in front has too are its: zeros here (their values may be gone by now, in place)
+                vec mask;
+#pragma unroll
+                for (unsigned i = 0; i < N; ++i) {
+                    typedef typename same_size<sizeof(T)>::type bits;
+                    mask[i] = __builtin_bit_cast(T, (bits)(i < shared ? 0 : ~(bits)0));
+                }
+#pragma unroll
+                for (unsigned k = 0; k < K; ++k) {
+                    const facc v = chunk_to_float<T>(__builtin_bit_cast(vec, __builtin_bit_cast(nvshmemi_v4u, x[k]) & __builtin_bit_cast(nvshmemi_v4u, mask)));
+#pragma unroll
+                    for (unsigned i = 0; i < N; ++i) dot[k] = __builtin_fmaf(v[i], g[i], dot[k]);
+                }
+#pragma unroll
+                for (unsigned k = 0; k < K; ++k) {
+                    if (!(ok >> k & 1)) continue;
+                    const vec y = chunk_from_float<T>(g * w[k]);
+                    if (TINY) chunk_store_part(dst[k], y, dim);
+                    else chunk_store_stream(dst[k] + first, y);
                 }
             }
 #pragma unroll
-            for (int k = 0; k < kCopies; ++k) {
-                for (int m = 32; m; m >>= 1) dot[k] += __shfl_xor(dot[k], m);
-                if (threadIdx.x % kLanes == 0) partial[threadIdx.x / kLanes][k] = dot[k];
+            for (int k = 0; k < K; ++k) {
+                dot[k] = group_sum<64>(dot[k]);
+                if (lane == 0) partial[wave][k] = dot[k];
             }
             __syncthreads();
-            if (threadIdx.x < kCopies && k0 + threadIdx.x < topk)
-                my_dgate[t * topk + k0 + threadIdx.x] = (partial[0][threadIdx.x] + partial[1][threadIdx.x]) +
-                                                        (partial[2][threadIdx.x] + partial[3][threadIdx.x]);
+            if (threadIdx.x < K && k0 + threadIdx.x < topk) {
+                float sum = 0.0f;
+                for (unsigned i = 0; i < waves; ++i) sum += partial[i][threadIdx.x];
+                my_dgate[t * topk + k0 + threadIdx.x] = ok >> threadIdx.x & 1 ? sum : 0.0f;
+            }
             __syncthreads();
         }
     }
@@ -202,9 +247,27 @@ int combine_grad_on_stream(API *drecv, float *dgate, const API *dout, const API 
     T *dst = (T *)ops.out("drecv", drecv, (uint64_t)recv_cap_rows * dim);
     if (!ops.ok()) return NVSHMEMX_ERROR_INVALID_VALUE;
     if (tokens == 0) return 0;
-    launch_kernel(combine_grad_kernel<T>, dim3((unsigned)(tokens < (1u << 20) ? tokens : 1u << 20), 1, rt.npes), dim3(256), 0, stream,
-                  dst, dw, from, src, w, to, at, rt.heap_size, (uint64_t)recv_cap_rows, (unsigned)tokens, (unsigned)topk,
-                  (unsigned)dim, (unsigned)rt.npes);
+    // as many wavefronts as make the last of their steps through a row a full one, more or less
+    const unsigned chunks = div_up(dim, Chunk<T>::N), steps = div_up(chunks, kGradWaves * kLanes), waves = div_up(chunks, steps * kLanes);
+#define NVSHMEM_AMD_LAUNCH_GRAD(K, TINY)                                                                                             \
+    launch_kernel((combine_grad_kernel<T, K, TINY>), dim3((unsigned)(tokens < (1u << 20) ? tokens : 1u << 20), 1, rt.npes),          \
+                  dim3(waves * kLanes), 0, stream, dst, dw, from, src, w, to, at, rt.heap_size, (uint64_t)recv_cap_rows,             \
+                  (unsigned)tokens, (unsigned)topk, (unsigned)dim, (unsigned)rt.npes)
+    if (dim < (size_t)Chunk<T>::N) {
+        NVSHMEM_AMD_LAUNCH_GRAD(8, true);
+    } else {
+        switch (topk) {
+            case 1: NVSHMEM_AMD_LAUNCH_GRAD(1, false); break;
+            case 2: NVSHMEM_AMD_LAUNCH_GRAD(2, false); break;
+            case 3: NVSHMEM_AMD_LAUNCH_GRAD(3, false); break;
+            case 4: NVSHMEM_AMD_LAUNCH_GRAD(4, false); break;
+            case 5: NVSHMEM_AMD_LAUNCH_GRAD(5, false); break;
+            case 6: NVSHMEM_AMD_LAUNCH_GRAD(6, false); break;
+            case 7: NVSHMEM_AMD_LAUNCH_GRAD(7, false); break;
+            default: NVSHMEM_AMD_LAUNCH_GRAD(8, false);
+        }
+    }
+#undef NVSHMEM_AMD_LAUNCH_GRAD
     return launched("moe_combine_grad");
 }
 

@@ -14,6 +14,8 @@ namespace {
 // One wavefront per piece of V x 64 chunks of a row; a row of fewer chunks than a wavefront has lanes takes the next power of two of
 // them and shares the wavefront with others (2^lanes_log lanes a row).  Reads a row of the table and writes one: bound by memory.
 // Where a wavefront has one token, its id is a scalar load and its rows are scalar addresses.
+// us for 8 x 4096 rows of 7168 bf16 (0.47 GB written, about a third of that read from memory: 113 us are 5.5 TB/s): one chunk a lane
+// 141, two 120, four (of 14) 130, seven 116; two, written through to memory 113.  8 x 64 rows: 4.4, written through 4.0.
 template <typename T, int V, int MODE>
 __global__ __launch_bounds__(64) void embedding_kernel(T *__restrict__ out, const T *__restrict__ table, const int64_t *__restrict__ ids,
                                                        uint64_t stride, unsigned tokens, unsigned vocab, unsigned rows, unsigned dim,
@@ -47,7 +49,7 @@ __global__ __launch_bounds__(64) void embedding_kernel(T *__restrict__ out, cons
         for (int v = 0; v < V; ++v) {
             const vec y = chunk_from_float<T>(chunk_to_float<T>(x[v]) * scale);
             if (MODE == kTiny) chunk_store_part(dst, y, dim);
-            else if (v == 0 || mine[v]) chunk_store_stream(dst + first[v], y);
+            else if (v == 0 || mine[v]) chunk_store_through(dst + first[v], y);
         }
     }
 }
@@ -214,7 +216,7 @@ __device__ __forceinline__ void zero_fill(T *p, uint64_t elems) {
     typedef typename Chunk<T>::vec vec;
     vec *v = (vec *)(p + head);
     const uint64_t n = (elems - head) / Chunk<T>::N, tail = head + n * Chunk<T>::N;
-    for (uint64_t i = lane; i < n; i += kLanes) __builtin_nontemporal_store(vec{}, v + i);
+    for (uint64_t i = lane; i < n; i += kLanes) chunk_store_stream((T *)(v + i), vec{});
     if (lane < elems - tail) p[tail + lane] = (T)0.0f;
 }
 
@@ -383,9 +385,6 @@ __global__ __launch_bounds__(kJoinWaves *kLanes) void embedding_join_kernel(T *d
     }
 }
 
-#ifndef VV
-#define VV 2
-#endif
 constexpr size_t kMostTokens = (size_t)1 << 31;
 
 int check_sizes(Runtime &rt, const char *what, size_t tokens, size_t vocab, size_t dim, float scale) {
@@ -418,7 +417,7 @@ int embedding_on_stream(API *out, const API *table, const int64_t *ids, size_t t
     launch_kernel((embedding_kernel<T, V, MODE>), dim3(div_up(chunks, kLanes * V), most, rt.npes), dim3(kLanes), 0, stream, dst, tab,  \
                   id, rt.heap_size, (unsigned)tokens, (unsigned)vocab, (unsigned)rows, (unsigned)dim, log, scale)
     if (dim < (size_t)Chunk<T>::N) NVSHMEM_AMD_LAUNCH_EMBEDDING(1, kTiny);
-    else if (chunks > kLanes) NVSHMEM_AMD_LAUNCH_EMBEDDING(VV, kWhole);
+    else if (chunks > kLanes) NVSHMEM_AMD_LAUNCH_EMBEDDING(2, kWhole);
     else if (log == 6) NVSHMEM_AMD_LAUNCH_EMBEDDING(1, kWhole);
     else NVSHMEM_AMD_LAUNCH_EMBEDDING(1, kShared);
 #undef NVSHMEM_AMD_LAUNCH_EMBEDDING

@@ -19,41 +19,6 @@ namespace {
 constexpr int kMostExperts = 1024, kMostTopk = 16;
 
 // ---- lanes: a token belongs to a group of G lanes (16, or the wavefront) ----
-template <int CTRL>
-__device__ __forceinline__ uint32_t dpp(uint32_t x) {
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
-}
-// The value of the lane that step STEP of a reduction over a group pairs with.  Steps 2 and 3 mirror 8 and 16 lanes: after the
-// steps before, all lanes of a quad (a half of the row) hold the same.
-template <int STEP>
-__device__ __forceinline__ uint32_t partner(uint32_t x) {
-    if (STEP == 0) return dpp<0xB1>(x);   // quad_perm [1,0,3,2]
-    if (STEP == 1) return dpp<0x4E>(x);   // quad_perm [2,3,0,1]
-    if (STEP == 2) return dpp<0x141>(x);  // row_half_mirror
-    if (STEP == 3) return dpp<0x140>(x);  // row_mirror
-    return (uint32_t)__shfl_xor((int)x, STEP == 4 ? 16 : 32);
-}
-template <int STEP>
-__device__ __forceinline__ float partner(float x) {
-    return __uint_as_float(partner<STEP>(__float_as_uint(x)));
-}
-template <int STEP>
-__device__ __forceinline__ double partner(double x) {
-    const uint64_t b = (uint64_t)__double_as_longlong(x);
-    return __longlong_as_double((long long)((uint64_t)partner<STEP>((uint32_t)(b >> 32)) << 32 | partner<STEP>((uint32_t)b)));
-}
-template <int G>
-__device__ __forceinline__ float group_sum(float x) {
-    x += partner<0>(x);
-    x += partner<1>(x);
-    x += partner<2>(x);
-    x += partner<3>(x);
-    if (G == 64) {
-        x += partner<4>(x);
-        x += partner<5>(x);
-    }
-    return x;
-}
 template <int G>
 __device__ __forceinline__ float group_max(float x) {
     x = fmaxf(x, partner<0>(x));

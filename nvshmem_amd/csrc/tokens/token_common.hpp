@@ -61,6 +61,11 @@ __device__ __forceinline__ void chunk_store_stream(T *p, typename Chunk<T>::vec 
 // share one as well).
 enum { kWhole, kShared, kTiny };
 
+// ... and written through to memory, past the L2.
+template <typename T>
+__device__ __forceinline__ void chunk_store_through(T *p, typename Chunk<T>::vec v) {
+    asm volatile("global_store_dwordx4 %0, %1, off sc1 nt\n\ts_nop 1" : : "v"(p), "v"(v) : "memory");
+}
 // Where chunk c of a row begins.  The last one ends with the row and so may share elements with the one in front of it: what is
 // computed for an element depends on the element alone, so both store the same bits, and every access is a whole vector.
 // Rows of less than a chunk have one, of `dim` elements, which the _part functions move.
@@ -95,6 +100,42 @@ __device__ __forceinline__ typename Chunk<T>::vec chunk_from_float(typename Chun
 template <typename T>
 __device__ __forceinline__ T *copy_of(T *p, unsigned pe, uint64_t stride) {
     return (T *)((char *)p + pe * stride);  // (pointer arithmetic all the way, or loads become flat ones)
+}
+// ---- lanes that exchange values: groups of G (16, or the wavefront) ----
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
+}
+// The value of the lane that step STEP of a reduction over a group pairs with.  Steps 2 and 3 mirror 8 and 16 lanes: after the
+// steps before, all lanes of a quad (a half of the row) hold the same.
+template <int STEP>
+__device__ __forceinline__ uint32_t partner(uint32_t x) {
+    if (STEP == 0) return dpp<0xB1>(x);   // quad_perm [1,0,3,2]
+    if (STEP == 1) return dpp<0x4E>(x);   // quad_perm [2,3,0,1]
+    if (STEP == 2) return dpp<0x141>(x);  // row_half_mirror
+    if (STEP == 3) return dpp<0x140>(x);  // row_mirror
+    return (uint32_t)__shfl_xor((int)x, STEP == 4 ? 16 : 32);
+}
+template <int STEP>
+__device__ __forceinline__ float partner(float x) {
+    return __uint_as_float(partner<STEP>(__float_as_uint(x)));
+}
+template <int STEP>
+__device__ __forceinline__ double partner(double x) {
+    const uint64_t b = (uint64_t)__double_as_longlong(x);
+    return __longlong_as_double((long long)((uint64_t)partner<STEP>((uint32_t)(b >> 32)) << 32 | partner<STEP>((uint32_t)b)));
+}
+template <int G>
+__device__ __forceinline__ float group_sum(float x) {
+    x += partner<0>(x);
+    x += partner<1>(x);
+    x += partner<2>(x);
+    x += partner<3>(x);
+    if (G == 64) {
+        x += partner<4>(x);
+        x += partner<5>(x);
+    }
+    return x;
 }
 // The wavefront's index in its block as a scalar.
 __device__ __forceinline__ unsigned wave_of_block() { return __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes); }
