@@ -18,39 +18,24 @@ namespace {
 
 constexpr int kMostExperts = 1024, kMostTopk = 16;
 
-// ---- lanes: a token belongs to a group of G lanes (16, or the wavefront) ----
-template <int G>
-__device__ __forceinline__ float group_max(float x) {
-    x = fmaxf(x, partner<0>(x));
-    x = fmaxf(x, partner<1>(x));
-    x = fmaxf(x, partner<2>(x));
-    x = fmaxf(x, partner<3>(x));
-    if (G == 64) {
-        x = fmaxf(x, partner<4>(x));
-        x = fmaxf(x, partner<5>(x));
-    }
-    return x;
-}
-
 // ---- keys: a logit and its expert in one word, larger for the larger logit and then for the lower expert ----
-// 16-bit logits: an unsigned word of the logit's bits in ascending order and the expert's complement.  fp32 logits: the same in the
-// 52 mantissa bits of a double in [1, 2), which v_max_f64 and v_min_f64 compare.  The smallest key (0, or 1.0) stands for
-// a masked expert: no logit that is not masked has it.  -0.0 is 0.0.
-__device__ __forceinline__ uint32_t ascending(uint32_t b, uint32_t sign) { return b & sign ? ~b & (sign | (sign - 1)) : b | sign; }
-__device__ __forceinline__ uint32_t descending_back(uint32_t s, uint32_t sign) { return s & sign ? s & ~sign : ~s & (sign | (sign - 1)); }
+// A logit is cleaned first: NaN becomes -inf, -0.0 becomes 0.0.  Its bits are then put in ascending order, in front of the
+// expert's complement: 16-bit logits in an unsigned word, fp32 logits in the 52 mantissa bits of a double in [1, 2), which v_max_f64
+// and v_min_f64 compare.  A key whose logit is -inf (or that is `none`, whose logit reads as NaN) is a masked expert's.
+__device__ __forceinline__ uint32_t ascending(uint32_t b) { return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u); }
+__device__ __forceinline__ uint32_t ascending_back(uint32_t s) { return s ^ (~(uint32_t)((int32_t)s >> 31) | 0x80000000u); }
+__device__ __forceinline__ float clean(float x) { return fmaxf(x, -__builtin_inff()) + 0.0f; }
 
 template <typename T>
 struct Key {  // _Float16, __bf16
     typedef uint32_t type;
-    static __device__ __forceinline__ type masked() { return 0; }
-    static __device__ __forceinline__ type make(T x, uint32_t e) {
-        uint32_t b = __builtin_bit_cast(uint16_t, x);
-        b = b == 0x8000u ? 0u : b;
-        return ascending(b, 0x8000u) << 16 | (0xffffu - e);
+    static __device__ __forceinline__ type none() { return 0; }
+    static __device__ __forceinline__ type make(float x, uint32_t e) {
+        return (ascending((uint32_t)__builtin_bit_cast(uint16_t, (T)x) << 16) & 0xffff0000u) | (0xffffu - e);
     }
     static __device__ __forceinline__ uint32_t expert(type k) { return 0xffffu - (k & 0xffffu); }
     static __device__ __forceinline__ float logit(type k) {
-        return (float)__builtin_bit_cast(T, (uint16_t)descending_back(k >> 16, 0x8000u));
+        return (float)__builtin_bit_cast(T, (uint16_t)(ascending_back(k) >> 16));
     }
     static __device__ __forceinline__ type larger(type a, type b) { return a > b ? a : b; }
     static __device__ __forceinline__ type smaller(type a, type b) { return a < b ? a : b; }
@@ -58,14 +43,14 @@ struct Key {  // _Float16, __bf16
 template <>
 struct Key<float> {
     typedef double type;
-    static __device__ __forceinline__ type masked() { return 1.0; }
+    static __device__ __forceinline__ type none() { return 1.0; }
     static __device__ __forceinline__ type make(float x, uint32_t e) {
-        const uint32_t s = ascending(__float_as_uint(x + 0.0f), 0x80000000u);
-        return __longlong_as_double((long long)((uint64_t)(0x3ff00000u | s >> 12) << 32 | (s << 20 | (0xfffffu - e))));
+        const uint32_t s = ascending(__float_as_uint(x));
+        return __longlong_as_double((long long)((uint64_t)__builtin_amdgcn_alignbit(0x3ffu, s, 12) << 32 | (s << 20 | (0xfffffu - e))));
     }
     static __device__ __forceinline__ uint32_t expert(type k) { return 0xfffffu - ((uint32_t)__double_as_longlong(k) & 0xfffffu); }
     static __device__ __forceinline__ float logit(type k) {
-        return __uint_as_float(descending_back((uint32_t)((uint64_t)__double_as_longlong(k) >> 20), 0x80000000u));
+        return __uint_as_float(ascending_back((uint32_t)((uint64_t)__double_as_longlong(k) >> 20)));
     }
     // (the instructions themselves: around fmax and fmin the compiler quiets NaNs that no key is)
     static __device__ __forceinline__ type larger(type a, type b) {
@@ -169,23 +154,25 @@ struct RouteArgs {
     int64_t *counts;  // written by the blocks themselves where a PE has one block, and no loss is asked for
     char *work;
     uint64_t hist, psum, rows, ticket;
-    unsigned tokens, per_block, blocks, experts, topk;
+    unsigned tokens, threads, per_block, blocks, experts, topk;
     int normalise, loss;
     float scale;
 };
 
-constexpr int kRouteThreads = 256;
+// Threads of a block: few for few tokens, which then spread over more compute units, many for many, whose second kernel then has
+// fewer rows to read.
+constexpr unsigned kRouteThreads = 256, kRouteMostThreads = 1024;
 
 template <typename T, int G, int V, int KP>
-__global__ __launch_bounds__(kRouteThreads) void route_kernel(const T *logits, RouteArgs a) {
+__global__ __launch_bounds__(kRouteMostThreads) void route_kernel(const T *logits, RouteArgs a) {
     typedef Key<T> K;
-    constexpr int kGroups = kRouteThreads / G, kWaves = kRouteThreads / kLanes;
-    extern __shared__ uint32_t lds[];  // hist[experts], float psum[kWaves][experts], rows
+    const unsigned threads = a.threads, waves = threads / kLanes, groups = threads / G;
+    extern __shared__ uint32_t lds[];  // hist[experts], float psum[waves][experts], rows
     uint32_t *hist = lds;
     float *psum = (float *)(lds + a.experts);
-    uint32_t *rows = lds + a.experts * (1 + (a.loss ? kWaves : 0));
+    uint32_t *rows = lds + a.experts * (1 + (a.loss ? waves : 0));
     const unsigned pe = blockIdx.z, sub = threadIdx.x % G, group = threadIdx.x / G;
-    for (unsigned e = threadIdx.x; e < a.experts; e += kRouteThreads) hist[e] = 0;
+    for (unsigned e = threadIdx.x; e < a.experts; e += threads) hist[e] = 0;
     if (threadIdx.x == 0) rows[0] = 0;
     __syncthreads();
     if (a.loss && blockIdx.x == 0 && pe == 0 && threadIdx.x == 0) *(uint32_t *)(a.work + a.ticket) = 0;
@@ -196,18 +183,21 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(const T *logits, R
     const unsigned begin = blockIdx.x * a.per_block, end = a.tokens - begin > a.per_block ? begin + a.per_block : a.tokens;
     float mass[V] = {};
     unsigned live = 0;
-    for (unsigned t0 = begin; t0 < end; t0 += kGroups) {  // (all lanes take part in every exchange)
+    for (unsigned t0 = begin; t0 < end; t0 += groups) {  // (all lanes take part in every exchange)
         const unsigned t = t0 + group;
-        T x[V];
-        Slots<T, G, V>::load(x, my_logits + (uint64_t)(t < end ? t : begin) * a.experts, a.experts, sub);
+        T raw[V];
+        Slots<T, G, V>::load(raw, my_logits + (uint64_t)(t < end ? t : begin) * a.experts, a.experts, sub);
+        float x[V];
         typename K::type key[V < KP ? KP : V];
 #pragma unroll
-        for (int u = 0; u < V; ++u)
-            key[u] = (float)x[u] > -__builtin_inff() ? K::make(x[u], Slots<T, G, V>::expert(u, sub)) : K::masked();
+        for (int u = 0; u < V; ++u) {
+            x[u] = clean((float)raw[u]);
+            key[u] = K::make(x[u], Slots<T, G, V>::expert(u, sub));
+        }
         if (V < KP) {
             sort_largest_first<K, V>(key);
 #pragma unroll
-            for (int u = V; u < KP; ++u) key[u] = K::masked();
+            for (int u = V; u < KP; ++u) key[u] = K::none();
         } else {
 #pragma unroll
             for (int u = 0; u < V; u += KP) {
@@ -223,27 +213,35 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(const T *logits, R
             keep_largest_of_pair<K, KP, 4>(key);
             keep_largest_of_pair<K, KP, 5>(key);
         }
-        const bool some = key[0] != K::masked();
         const float m = K::logit(key[0]);
+        const bool some = m > -__builtin_inff();
         float z = 1.0f;
         if (a.loss || !a.normalise) {
-            float p[V], sum = 0.0f;
+            // weights against the largest logit; where that is inf, those that are inf weigh 1 and the others nothing
+            const bool endless = m == __builtin_inff();
+            if (__builtin_amdgcn_ballot_w64(endless)) {
+#pragma unroll
+                for (int u = 0; u < V; ++u) x[u] = endless ? (x[u] == m ? 0.0f : -__builtin_inff()) : x[u];
+            }
+            const float top = some && !endless ? m : 0.0f;
+            float sum = 0.0f;
 #pragma unroll
             for (int u = 0; u < V; ++u) {
-                p[u] = (float)x[u] > -__builtin_inff() ? exp_below((float)x[u], m) : 0.0f;
-                sum += p[u];
+                x[u] = __expf(x[u] - top);
+                sum += x[u];
             }
             z = group_sum<G>(sum);
             const float r = some && t < end ? 1.0f / z : 0.0f;
 #pragma unroll
-            for (int u = 0; u < V; ++u) mass[u] = __builtin_fmaf(p[u], r, mass[u]);
+            for (int u = 0; u < V; ++u) mass[u] = __builtin_fmaf(x[u], r, mass[u]);
         }
-        typename K::type own = K::masked();
+        typename K::type own = K::none();
 #pragma unroll
         for (int k = 0; k < KP; ++k)
             if (sub == (unsigned)k) own = key[k];
-        const bool chosen = sub < a.topk && own != K::masked();
-        const float p = chosen ? exp_below(K::logit(own), m) : 0.0f;
+        const float l = K::logit(own);
+        const bool chosen = sub < a.topk && l > -__builtin_inff();
+        const float p = chosen ? exp_below(l, m) : 0.0f;
         const float s = group_sum<G>(p);
         if (t < end) {
             live += some && sub == 0;
@@ -269,12 +267,12 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(const T *logits, R
     }
     __syncthreads();
     char *work = copy_of(a.work, pe, a.stride);
-    for (unsigned e = threadIdx.x; e < a.experts; e += kRouteThreads) {
+    for (unsigned e = threadIdx.x; e < a.experts; e += threads) {
         if (a.counts) copy_of(a.counts, pe, a.stride)[e] = hist[e];
         else ((uint32_t *)(work + a.hist))[(uint64_t)blockIdx.x * a.experts + e] = hist[e];
         if (a.loss) {
             float s = 0.0f;
-            for (int w = 0; w < kWaves; ++w) s += psum[w * a.experts + e];
+            for (unsigned w = 0; w < waves; ++w) s += psum[w * a.experts + e];
             ((float *)(work + a.psum))[(uint64_t)blockIdx.x * a.experts + e] = s;
         }
     }
@@ -291,85 +289,98 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(const T *logits, R
     }
 }
 
-// Counts, loss and its derivative from what the blocks of all PEs left: 32 experts a block, 32 rows at a time.
-constexpr unsigned kFinishExperts = 32, kFinishRows = 32;
+// Counts, loss and its derivative from what the blocks of all PEs left.  A block has 8 experts, a wavefront 8 rows of a PE's at a
+// time, so that no wavefront waits for another until all PEs are added up.
+constexpr unsigned kFinishExperts = 8, kFinishWaves = 16;
 
-__global__ __launch_bounds__(kFinishExperts *kFinishRows) void route_finish_kernel(int64_t *counts, float *loss, float *balance,
-                                                                                    char *work, uint64_t stride, uint64_t hist,
-                                                                                    uint64_t psum, uint64_t rows, uint64_t ticket,
-                                                                                    unsigned blocks, unsigned experts, unsigned npes) {
-    __shared__ uint32_t c_part[kFinishRows][kFinishExperts];
-    __shared__ double s_part[kFinishRows][kFinishExperts];
-    __shared__ double value[kFinishExperts];
-    __shared__ unsigned long long totals[2];
+__global__ __launch_bounds__(kFinishWaves *kLanes) void route_finish_kernel(int64_t *counts, float *loss, float *balance, char *work,
+                                                                            uint64_t stride, uint64_t hist, uint64_t psum,
+                                                                            uint64_t rows, uint64_t ticket, unsigned blocks,
+                                                                            unsigned experts, unsigned npes) {
+    __shared__ double value[kFinishWaves][kFinishExperts];
+    __shared__ unsigned long long copies[kFinishExperts], totals[2];
     __shared__ unsigned last;
-    const unsigned x = threadIdx.x % kFinishExperts, y = threadIdx.x / kFinishExperts;
+    const unsigned wave = wave_of_block(), x = threadIdx.x % kFinishExperts, y = threadIdx.x % kLanes / kFinishExperts;
     const unsigned e = blockIdx.x * kFinishExperts + x;
+    if (threadIdx.x < kFinishExperts) copies[threadIdx.x] = 0;
     if (threadIdx.x < 2) totals[threadIdx.x] = 0;
-    double s = 0.0;
-    unsigned long long all = 0;
-    for (unsigned pe = 0; pe < npes; ++pe) {
-        const char *w = copy_of(work, pe, stride);
-        uint32_t c = 0;
-        if (e < experts)
-            for (unsigned r = y; r < blocks; r += kFinishRows) {
-                c += ((const uint32_t *)(w + hist))[(uint64_t)r * experts + e];
-                if (loss) s += ((const float *)(w + psum))[(uint64_t)r * experts + e];
-            }
-        c_part[y][x] = c;
-        __syncthreads();
-        if (y == 0 && e < experts) {
-            c = 0;
-            for (unsigned i = 0; i < kFinishRows; ++i) c += c_part[i][x];
-            copy_of(counts, pe, stride)[e] = c;
-            all += c;
+    __syncthreads();
+    double mass = 0.0;
+    // tokens and copies of all PEs
+    unsigned long long tokens_here = 0, copies_here = 0;
+    if (loss) {
+        for (unsigned i = threadIdx.x; i < npes * blocks; i += kFinishWaves * kLanes) {
+            const uint32_t *r = (const uint32_t *)(copy_of(work, i / blocks, stride) + rows) + 2 * (i % blocks);
+            tokens_here += r[0];
+            copies_here += r[1];
         }
-        __syncthreads();
+    }
+    for (unsigned pe = wave; pe < npes; pe += kFinishWaves) {
+        const char *w = copy_of(work, pe, stride);
+        const uint32_t *h = (const uint32_t *)(w + hist) + e;
+        const float *s = (const float *)(w + psum) + e;
+        uint32_t c = 0;
+        if (e < experts) {
+            if (loss) {
+#pragma unroll 8
+                for (unsigned r = y; r < blocks; r += kLanes / kFinishExperts) {
+                    c += h[(uint64_t)r * experts];
+                    mass += s[(uint64_t)r * experts];
+                }
+            } else {
+#pragma unroll 8
+                for (unsigned r = y; r < blocks; r += kLanes / kFinishExperts) c += h[(uint64_t)r * experts];
+            }
+        }
+        c += dpp<0x128>(c);  // row_ror:8
+        c += partner<4>(c);
+        c += partner<5>(c);
+        if (y == 0 && e < experts) {
+            copy_of(counts, pe, stride)[e] = c;
+            atomicAdd(&copies[x], (unsigned long long)c);
+        }
     }
     if (!loss) return;
-    s_part[y][x] = s;
-    // rows and copies of all PEs
-    unsigned long long n = 0, m = 0;
-    for (unsigned i = threadIdx.x; i < npes * blocks; i += kFinishExperts * kFinishRows) {
-        const uint32_t *r = (const uint32_t *)(copy_of(work, i / blocks, stride) + rows) + 2 * (i % blocks);
-        n += r[0];
-        m += r[1];
-    }
-    if (n) atomicAdd(&totals[0], n);
-    if (m) atomicAdd(&totals[1], m);
+    for (int s = kFinishExperts; s < kLanes; s <<= 1) mass += __shfl_xor(mass, s);
+    if (y == 0) value[wave][x] = mass;
+    if (tokens_here) atomicAdd(&totals[0], tokens_here);
+    if (copies_here) atomicAdd(&totals[1], copies_here);
     __syncthreads();
-    if (y == 0) {
-        double total = 0.0;
-        for (unsigned i = 0; i < kFinishRows; ++i) total += s_part[i][x];
-        const double b = totals[1] ? (double)experts * (double)all / ((double)totals[1] * (double)totals[0]) : 0.0;
-        value[x] = e < experts ? b * total : 0.0;
-        if (e < experts)
-            for (unsigned pe = 0; pe < npes; ++pe) copy_of(balance, pe, stride)[e] = (float)b;
-    }
-    __syncthreads();
-    // the block that comes last adds up what each block found, in their order
     double *found = (double *)(work + ticket + 64);
-    if (threadIdx.x == 0) {
+    if (wave == 0) {
         double v = 0.0;
-        for (unsigned i = 0; i < kFinishExperts; ++i) v += value[i];
-        __hip_atomic_store(found + blockIdx.x, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        last = __hip_atomic_fetch_add((uint32_t *)(work + ticket), 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) + 1 == gridDim.x;
+        if (y == 0 && e < experts) {
+            const double b = totals[1] ? (double)experts * (double)copies[x] / ((double)totals[1] * (double)totals[0]) : 0.0;
+            for (unsigned w = 0; w < kFinishWaves; ++w) v += value[w][x];
+            v *= b;
+            for (unsigned pe = 0; pe < npes; ++pe) copy_of(balance, pe, stride)[e] = (float)b;
+        }
+        for (int s = 1; s < (int)kFinishExperts; s <<= 1) v += __shfl_xor(v, s);
+        // the block that comes last adds up what each block found, in their order
+        if (threadIdx.x == 0) {
+            __hip_atomic_store(found + blockIdx.x, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            // (agent-scope stores and loads pass the L2s by: that the store has arrived is all that the ticket has to wait for,
+            // and no L2 has to be written back for it)
+            nvshmemi_amd_wait_vm();
+            last = __hip_atomic_fetch_add((uint32_t *)(work + ticket), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == gridDim.x;
+        }
     }
     __syncthreads();
-    if (!last) return;
-    if (threadIdx.x < npes) {
-        double v = 0.0;
-        for (unsigned i = 0; i < gridDim.x; ++i) v += __hip_atomic_load(found + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        copy_of(loss, threadIdx.x, stride)[0] = (float)v;
-    }
+    if (!last || wave != 0) return;
+    double v = 0.0;
+    for (unsigned i = threadIdx.x; i < gridDim.x; i += kLanes) v += __hip_atomic_load(found + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int s = 1; s < kLanes; s <<= 1) v += __shfl_xor(v, s);
+    if (threadIdx.x < npes) copy_of(loss, threadIdx.x, stride)[0] = (float)v;
 }
 
+constexpr int kGradThreads = 256;
+
 template <typename T, int G, int V>
-__global__ __launch_bounds__(kRouteThreads) void route_grad_kernel(T *dlogits, const T *logits, const int32_t *expert,
+__global__ __launch_bounds__(kGradThreads) void route_grad_kernel(T *dlogits, const T *logits, const int32_t *expert,
                                                                    const float *dgate, const float *balance, const float *dloss,
                                                                    uint64_t stride, unsigned tokens, unsigned experts, unsigned topk,
                                                                    int normalise, float scale) {
-    constexpr int kGroups = kRouteThreads / G;
+    constexpr int kGroups = kGradThreads / G;
     __shared__ float chosen_part[kGroups][G * V];  // what only the chosen experts get, by expert
     const unsigned pe = blockIdx.z, sub = threadIdx.x % G, group = threadIdx.x / G;
     const T *my_logits = copy_of(logits, pe, stride);
@@ -441,28 +452,33 @@ __global__ __launch_bounds__(kRouteThreads) void route_grad_kernel(T *dlogits, c
 // ---- the shuffle's tables ----
 // A stable counting sort of the copies by expert: rows of a destination PE lie in the order (expert, source PE, token, k).  Nothing
 // here is much data; what it costs is waiting, so a block asks for all that it needs from memory at once, at its start.
-constexpr unsigned kPlaceRounds = 8, kPlaceCopies = kSortThreads * kPlaceRounds;
+// Copies of a thread: one where a block has room for all of a PE's, two up to kPlaceSpread of them, which then spread over more
+// compute units, eight beyond, as each block adds up what the blocks in front of it counted.
+constexpr uint64_t kPlaceSpread = 1 << 17;
+unsigned place_rounds(uint64_t copies) { return copies <= kSortThreads ? 1 : copies <= kPlaceSpread ? 2 : 8; }
 
+template <unsigned ROUNDS>
 __global__ __launch_bounds__(kSortThreads) void place_count_kernel(uint32_t *hist, const int32_t *expert, uint64_t stride,
                                                                    unsigned copies, unsigned experts) {
     __shared__ uint32_t count[kMostExperts];
     const unsigned pe = blockIdx.z;
     const int32_t *mine = copy_of(expert, pe, stride);
-    unsigned to[kPlaceRounds];
+    unsigned to[ROUNDS];
 #pragma unroll
-    for (unsigned i = 0; i < kPlaceRounds; ++i) {
-        const unsigned c = blockIdx.x * kPlaceCopies + i * kSortThreads + threadIdx.x;
+    for (unsigned i = 0; i < ROUNDS; ++i) {
+        const unsigned c = blockIdx.x * (kSortThreads * ROUNDS) + i * kSortThreads + threadIdx.x;
         to[i] = c < copies ? (unsigned)mine[c] : ~0u;
     }
     count[threadIdx.x] = 0;
     __syncthreads();
 #pragma unroll
-    for (unsigned i = 0; i < kPlaceRounds; ++i)
+    for (unsigned i = 0; i < ROUNDS; ++i)
         if (to[i] < experts) atomicAdd(&count[to[i]], 1u);
     __syncthreads();
     if (threadIdx.x < experts) copy_of(hist, pe, stride)[(uint64_t)blockIdx.x * experts + threadIdx.x] = count[threadIdx.x];
 }
 
+template <unsigned ROUNDS>
 __global__ __launch_bounds__(kSortThreads) void place_kernel(int32_t *dest_pe, int64_t *dest_row, uint64_t *expected,
                                                              int64_t *expert_row, const uint32_t *hist, const int32_t *expert,
                                                              const int64_t *counts, uint64_t stride, unsigned copies,
@@ -472,10 +488,10 @@ __global__ __launch_bounds__(kSortThreads) void place_kernel(int32_t *dest_pe, i
     __shared__ uint32_t arriving[NVSHMEMI_AMD_MAX_PES], from[kMostExperts];
     const unsigned pe = blockIdx.z, per_pe = experts / npes;
     const int32_t *mine = copy_of(expert, pe, stride);
-    const unsigned c0 = blockIdx.x * kPlaceCopies + threadIdx.x / kLanes * (kPlaceRounds * kLanes) + threadIdx.x % kLanes;
-    uint32_t to[kPlaceRounds], place[kPlaceRounds];
+    const unsigned c0 = blockIdx.x * (kSortThreads * ROUNDS) + threadIdx.x / kLanes * (ROUNDS * kLanes) + threadIdx.x % kLanes;
+    uint32_t to[ROUNDS], place[ROUNDS];
 #pragma unroll
-    for (unsigned i = 0; i < kPlaceRounds; ++i) to[i] = c0 + i * kLanes < copies ? (uint32_t)mine[c0 + i * kLanes] : ~0u;
+    for (unsigned i = 0; i < ROUNDS; ++i) to[i] = c0 + i * kLanes < copies ? (uint32_t)mine[c0 + i * kLanes] : ~0u;
     // (own expert, source PE), what arrives from there: one pair a thread
     const unsigned own = threadIdx.x / npes, source = threadIdx.x % npes;
     const bool pair = blockIdx.x == 0 && own < per_pe;
@@ -522,11 +538,11 @@ __global__ __launch_bounds__(kSortThreads) void place_kernel(int32_t *dest_pe, i
     }
     __syncthreads();
     if (blockIdx.x == 0 && threadIdx.x < npes) copy_of(expected, pe, stride)[threadIdx.x] = arriving[threadIdx.x];
-    stable_places<kPlaceRounds>(place, to, experts, run, lds);
+    stable_places<ROUNDS>(place, to, experts, run, lds);
     int32_t *out_pe = copy_of(dest_pe, pe, stride);
     int64_t *out_row = copy_of(dest_row, pe, stride);
 #pragma unroll
-    for (unsigned i = 0; i < kPlaceRounds; ++i) {
+    for (unsigned i = 0; i < ROUNDS; ++i) {
         const unsigned c = c0 + i * kLanes;
         if (c >= copies) continue;
         const bool kept = to[i] < experts && place[i] < cap;
@@ -536,14 +552,18 @@ __global__ __launch_bounds__(kSortThreads) void place_kernel(int32_t *dest_pe, i
 }
 
 // ---- host ----
+constexpr unsigned kFewBlocks = 512, kManyBlocks = 256;
 // Blocks of a PE: enough of them over all PEs to fill the GPU, and no more, as the second kernel reads what each one leaves.
 struct RouteShape {
-    unsigned groups, per_block, blocks;
+    unsigned threads, per_block, blocks;
     uint64_t hist, psum, rows, ticket, bytes;
     RouteShape(size_t tokens, int experts, int npes) {
-        groups = kRouteThreads / (experts > 256 ? 64 : 16);
-        const uint64_t steps = ((uint64_t)tokens * npes + groups - 1) / groups;
-        per_block = groups * (unsigned)(steps <= 1024 ? 1 : (steps + 1023) / 1024);
+        const unsigned group = experts > 256 ? kLanes : 16;
+        const uint64_t all = (uint64_t)tokens * npes;
+        threads = all * group <= kFewBlocks * kRouteThreads ? kRouteThreads : kRouteMostThreads;
+        const unsigned groups = threads / group, most = threads == kRouteThreads ? kFewBlocks : kManyBlocks;
+        const uint64_t steps = (all + groups - 1) / groups;
+        per_block = groups * (unsigned)(steps <= most ? 1 : (steps + most - 1) / most);
         blocks = tokens ? div_up(tokens, per_block) : 1;
         const uint64_t table = ((uint64_t)blocks * experts * 4 + 63) / 64 * 64;
         hist = 0;
@@ -566,10 +586,10 @@ int check_routing(Runtime &rt, const char *what, size_t tokens, int experts, int
 template <typename T, int G, int V>
 void launch_route(const T *logits, const RouteArgs &a, unsigned npes, hipStream_t stream) {
     const dim3 grid(a.blocks, 1, npes);
-    const size_t lds = ((size_t)a.experts * (1 + (a.loss ? kRouteThreads / kLanes : 0)) + 1) * 4;
-    if (a.topk <= 2) launch_kernel(route_kernel<T, G, V, 2>, grid, dim3(kRouteThreads), lds, stream, logits, a);
-    else if (a.topk <= 8) launch_kernel(route_kernel<T, G, V, 8>, grid, dim3(kRouteThreads), lds, stream, logits, a);
-    else launch_kernel(route_kernel<T, G, V, 16>, grid, dim3(kRouteThreads), lds, stream, logits, a);
+    const size_t lds = ((size_t)a.experts * (1 + (a.loss ? a.threads / kLanes : 0)) + 1) * 4;
+    if (a.topk <= 2) launch_kernel(route_kernel<T, G, V, 2>, grid, dim3(a.threads), lds, stream, logits, a);
+    else if (a.topk <= 8) launch_kernel(route_kernel<T, G, V, 8>, grid, dim3(a.threads), lds, stream, logits, a);
+    else launch_kernel(route_kernel<T, G, V, 16>, grid, dim3(a.threads), lds, stream, logits, a);
 }
 
 template <typename API>
@@ -597,14 +617,14 @@ int route_on_stream(int32_t *expert, float *gate, int64_t *counts, float *loss, 
     const bool alone = shape.blocks == 1 && !loss;
     a.counts = alone ? count : nullptr;
     a.hist = shape.hist, a.psum = shape.psum, a.rows = shape.rows, a.ticket = shape.ticket;
-    a.tokens = (unsigned)tokens, a.per_block = shape.per_block, a.blocks = shape.blocks;
+    a.tokens = (unsigned)tokens, a.threads = shape.threads, a.per_block = shape.per_block, a.blocks = shape.blocks;
     a.experts = (unsigned)experts, a.topk = (unsigned)topk;
     a.normalise = normalise != 0, a.loss = loss != nullptr, a.scale = scale;
     if (experts <= 64) launch_route<T, 16, 4>(in, a, rt.npes, stream);
     else if (experts <= 256) launch_route<T, 16, 16>(in, a, rt.npes, stream);
     else launch_route<T, 64, 16>(in, a, rt.npes, stream);
     if (!alone)
-        launch_kernel(route_finish_kernel, dim3(div_up(experts, kFinishExperts)), dim3(kFinishExperts * kFinishRows), 0, stream, count, l,
+        launch_kernel(route_finish_kernel, dim3(div_up(experts, kFinishExperts)), dim3(kFinishWaves * kLanes), 0, stream, count, l,
                       b, a.work, a.stride, a.hist, a.psum, a.rows, a.ticket, a.blocks, a.experts, (unsigned)rt.npes);
     return launched("moe_route");
 }
@@ -631,8 +651,8 @@ int route_grad_on_stream(API *dlogits, const API *logits, const int32_t *expert,
     if (tokens == 0) return 0;
 #define NVSHMEM_AMD_LAUNCH_GRAD(G, V)                                                                                             \
     {                                                                                                                             \
-        const unsigned steps = div_up(tokens, kRouteThreads / G), most = 4096 / (unsigned)rt.npes;                                \
-        launch_kernel(route_grad_kernel<T, G, V>, dim3(steps < most ? steps : most, 1, rt.npes), dim3(kRouteThreads), 0, stream,  \
+        const unsigned steps = div_up(tokens, kGradThreads / G), most = 1024 / (unsigned)rt.npes;                                \
+        launch_kernel(route_grad_kernel<T, G, V>, dim3(steps < most ? steps : most, 1, rt.npes), dim3(kGradThreads), 0, stream,  \
                       out, in, to, dg, b, dl, rt.heap_size, (unsigned)tokens, (unsigned)experts, (unsigned)topk, normalise != 0, scale); \
     }
     if (experts <= 64) NVSHMEM_AMD_LAUNCH_GRAD(16, 4)
@@ -651,7 +671,7 @@ int place_on_stream(int32_t *dest_pe, int64_t *dest_row, uint64_t *expected, int
     if (int rc = check_routing(rt, "moe_place", tokens, experts, topk)) return rc;
     NVSHMEM_AMD_REFUSE(experts % rt.npes, "moe_place: %d experts on %d PEs, not the same number on each", experts, rt.npes);
     const uint64_t copies = (uint64_t)tokens * topk;
-    const unsigned blocks = copies ? div_up(copies, kPlaceCopies) : 1;
+    const unsigned rounds = place_rounds(copies), blocks = copies ? div_up(copies, kSortThreads * rounds) : 1;
     Operands ops(rt, "moe_place");
     const int32_t *in = ops.in("expert", expert, copies);
     const int64_t *count = ops.in("counts", counts, (uint64_t)experts);
@@ -663,12 +683,19 @@ int place_on_stream(int32_t *dest_pe, int64_t *dest_row, uint64_t *expected, int
     if (!ops.ok()) return NVSHMEMX_ERROR_INVALID_VALUE;
     unsigned column_log = 0;
     while ((1u << column_log) < (unsigned)experts) ++column_log;
-    if (blocks > 1)
-        launch_kernel(place_count_kernel, dim3(blocks, 1, rt.npes), dim3(kSortThreads), 0, stream, hist, in, rt.heap_size,
-                      (unsigned)copies, (unsigned)experts);
-    launch_kernel(place_kernel, dim3(blocks, 1, rt.npes), dim3(kSortThreads), (size_t)kSortWaves * experts * 4, stream, to, row, exp,
-                  first, hist, in, count, rt.heap_size, (unsigned)copies, (unsigned)experts, (unsigned)rt.npes, (uint64_t)recv_cap_rows,
-                  column_log);
+#define NVSHMEM_AMD_LAUNCH_PLACE(ROUNDS)                                                                                               \
+    {                                                                                                                                \
+        if (blocks > 1)                                                                                                              \
+            launch_kernel(place_count_kernel<ROUNDS>, dim3(blocks, 1, rt.npes), dim3(kSortThreads), 0, stream, hist, in,             \
+                          rt.heap_size, (unsigned)copies, (unsigned)experts);                                                        \
+        launch_kernel(place_kernel<ROUNDS>, dim3(blocks, 1, rt.npes), dim3(kSortThreads), (size_t)kSortWaves * experts * 4, stream, \
+                      to, row, exp, first, hist, in, count, rt.heap_size, (unsigned)copies, (unsigned)experts, (unsigned)rt.npes,    \
+                      (uint64_t)recv_cap_rows, column_log);                                                                          \
+    }
+    if (rounds == 1) NVSHMEM_AMD_LAUNCH_PLACE(1)
+    else if (rounds == 2) NVSHMEM_AMD_LAUNCH_PLACE(2)
+    else NVSHMEM_AMD_LAUNCH_PLACE(8)
+#undef NVSHMEM_AMD_LAUNCH_PLACE
     return launched("moe_place");
 }
 
@@ -711,7 +738,8 @@ int nvshmemx_amd_moe_place_on_stream(int32_t *dest_pe, int64_t *dest_row, uint64
 }
 size_t nvshmemx_amd_moe_place_workspace(size_t tokens, int topk, int experts) {
     if (Runtime::get().npes < 1 || topk < 1 || experts < 1) return 0;
-    return ((uint64_t)tokens * topk + tokens::kPlaceCopies - 1) / tokens::kPlaceCopies * (uint64_t)experts * sizeof(uint32_t);
+    const uint64_t copies = (uint64_t)tokens * topk, block = (uint64_t)tokens::kSortThreads * tokens::place_rounds(copies);
+    return (copies + block - 1) / block * (uint64_t)experts * sizeof(uint32_t);
 }
 
 }  // extern "C"

@@ -104,7 +104,7 @@ __device__ __forceinline__ T *copy_of(T *p, unsigned pe, uint64_t stride) {
 // ---- lanes that exchange values: groups of G (16, or the wavefront) ----
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp(uint32_t x) {
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, CTRL, 0xf, 0xf, true);
 }
 // The value of the lane that step STEP of a reduction over a group pairs with.  Steps 2 and 3 mirror 8 and 16 lanes: after the
 // steps before, all lanes of a quad (a half of the row) hold the same.
@@ -134,6 +134,18 @@ __device__ __forceinline__ float group_sum(float x) {
     if (G == 64) {
         x += partner<4>(x);
         x += partner<5>(x);
+    }
+    return x;
+}
+template <int G>
+__device__ __forceinline__ float group_max(float x) {
+    x = fmaxf(x, partner<0>(x));
+    x = fmaxf(x, partner<1>(x));
+    x = fmaxf(x, partner<2>(x));
+    x = fmaxf(x, partner<3>(x));
+    if (G == 64) {
+        x = fmaxf(x, partner<4>(x));
+        x = fmaxf(x, partner<5>(x));
     }
     return x;
 }
