@@ -138,7 +138,7 @@ __global__ __launch_bounds__(kGradWaves *kLanes) void combine_grad_kernel(T *dre
 #pragma unroll
                 for (unsigned k = 0; k < K; ++k) x[k] = TINY ? chunk_load_part(src[k], dim) : chunk_load_stream(src[k] + first);
                 const facc g = chunk_to_float<T>(TINY ? chunk_load_part(from, dim) : chunk_load(from + first));
-                // elements that the chunk in front has too are its: zeros here (their values may be gone by now, in place)
+                // elements that the chunk in front has too are its: zeros here (in place, their values may be gone by now)
                 vec mask;
 #pragma unroll
                 for (unsigned i = 0; i < N; ++i) {
@@ -155,8 +155,10 @@ __global__ __launch_bounds__(kGradWaves *kLanes) void combine_grad_kernel(T *dre
                 for (unsigned k = 0; k < K; ++k) {
                     if (!(ok >> k & 1)) continue;
                     const vec y = chunk_from_float<T>(g * w[k]);
+                    // (the elements shared with the chunk in front are stored by its lane, which may still have to read them)
                     if (TINY) chunk_store_part(dst[k], y, dim);
-                    else chunk_store_stream(dst[k] + first, y);
+                    else if (shared == 0) chunk_store_stream(dst[k] + first, y);
+                    else chunk_store_behind(dst[k] + first, y, shared);
                 }
             }
 #pragma unroll

@@ -59,9 +59,10 @@ __global__ __launch_bounds__(64) void embedding_kernel(T *__restrict__ out, cons
 // writes the sums of the ids that lie in its part as a whole.  A sum that goes on into the next part leaves a partial sum in fp32
 // (`carry`), and a kernel behind it adds those up, in order: nothing depends on which block comes first.
 constexpr unsigned kLeastPart = 8, kMostPart = kLanes;
-unsigned part_of(uint64_t n) {
+unsigned part_of(uint64_t n, uint64_t dim) {
+    const uint64_t pieces = (dim + 511) / 512;
     unsigned part = kLeastPart;
-    while (part < kMostPart && n / 256 > part) part *= 2;
+    while (part < kMostPart && n * pieces / 4096 > part) part *= 2;
     return part;
 }
 
@@ -74,41 +75,39 @@ __device__ __forceinline__ uint32_t key_of(const int64_t *ids, uint64_t stride, 
     return id < vocab ? (uint32_t)id : vocab;
 }
 
-// Up to kRankTokens tokens: a token's place in the sorted order is the number of smaller ones, and a block of 16 wavefronts counts
-// it for 64 tokens, a lane each, a sixteenth of all tokens a wavefront.  Quadratic, but one launch.
-constexpr unsigned kRankTokens = 8192;
+// Up to kRankTokens tokens: a token's place in the sorted order is the number of smaller ones.  A block of 16 wavefronts counts it for
+// 32 tokens, two lanes each; a lane goes through a thirty-second of all tokens, four at a time.  Quadratic, but one launch; what bounds
+// it is LDS, which half the keys to a block, in twice the blocks, halves.
+constexpr unsigned kRankTokens = 12288, kRankKeys = kLanes / 2;
 
 __global__ __launch_bounds__(kSortThreads) void embedding_rank_kernel(Item *sorted, const int64_t *ids, uint64_t stride,
                                                                       unsigned tokens, unsigned n, unsigned vocab) {
-    __shared__ __align__(16) uint32_t all[kRankTokens];
-    __shared__ uint32_t smaller[kLanes];
-    const unsigned wave = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
-    const unsigned padded = (n + 63) / 64 * 64, block = blockIdx.x * kLanes;
-#pragma unroll
-    for (unsigned k = 0; k < kRankTokens / kSortThreads; ++k) {
-        const unsigned i = k * kSortThreads + threadIdx.x;
-        if (i < padded) all[i] = i < n ? key_of(ids, stride, tokens, vocab, i) : 0xffffffffu;
-    }
-    if (threadIdx.x < kLanes) smaller[lane] = 0;
+    extern __shared__ __align__(16) uint32_t all[];  // n, rounded up to 64
+    __shared__ uint32_t smaller[kRankKeys];
+    const unsigned wave = threadIdx.x / kLanes, lane = threadIdx.x % kRankKeys, half = threadIdx.x % kLanes / kRankKeys;
+    const unsigned padded = (n + 63) / 64 * 64, block = blockIdx.x * kRankKeys;
+#pragma unroll 8
+    for (unsigned i = threadIdx.x; i < padded; i += kSortThreads) all[i] = i < n ? key_of(ids, stride, tokens, vocab, i) : 0xffffffffu;
+    if (threadIdx.x < kRankKeys) smaller[threadIdx.x] = 0;
     __syncthreads();
     const uint32_t mine = all[block + lane];
     unsigned rank = 0;
-    // 64 keys at a time; those in front of this block's count when they are equal
-    for (unsigned j0 = wave * kLanes; j0 < padded; j0 += kSortThreads) {
+    // 32 keys at a time; those in front of this block's count when they are equal
+    for (unsigned j0 = wave * kLanes + half * kRankKeys; j0 < padded; j0 += kSortThreads) {
         if (j0 == block) {
-            for (unsigned j = 0; j < kLanes; ++j) rank += all[block + j] < mine + (j < lane);
+            for (unsigned j = 0; j < kRankKeys; ++j) rank += all[block + j] < mine + (j < lane);
             continue;
         }
         const uint32_t limit = mine + (j0 < block);
 #pragma unroll
-        for (unsigned j = 0; j < kLanes; j += 4) {
+        for (unsigned j = 0; j < kRankKeys; j += 4) {
             const uint4 k = *(const uint4 *)(all + j0 + j);
             rank += (k.x < limit) + (k.y < limit) + (k.z < limit) + (k.w < limit);
         }
     }
     atomicAdd(&smaller[lane], rank);
     __syncthreads();
-    if (wave == 0 && block + lane < n) sorted[smaller[lane]] = {mine, block + lane};
+    if (threadIdx.x < kRankKeys && block + lane < n) sorted[smaller[lane]] = {mine, block + lane};
 }
 
 // More tokens: counting sorts by kDigit bits of the id at a time, lowest first, of at most kSortBlocks blocks of consecutive tokens.
@@ -216,7 +215,7 @@ __device__ __forceinline__ void zero_fill(T *p, uint64_t elems) {
     typedef typename Chunk<T>::vec vec;
     vec *v = (vec *)(p + head);
     const uint64_t n = (elems - head) / Chunk<T>::N, tail = head + n * Chunk<T>::N;
-    for (uint64_t i = lane; i < n; i += kLanes) chunk_store_stream((T *)(v + i), vec{});
+    for (uint64_t i = lane; i < n; i += kLanes) v[i] = vec{};
     if (lane < elems - tail) p[tail + lane] = (T)0.0f;
 }
 
@@ -435,7 +434,7 @@ struct GradSpace {
         passes = n <= kRankTokens ? 0 : (bits + kDigit - 1) / kDigit;
         const uint64_t list = (n * sizeof(Item) + 63) / 64 * 64;
         pitch = (unsigned)((dim + 7) / 8 * 8);
-        part = part_of(n);
+        part = part_of(n, dim);
         items = list;
         hist = passes > 1 ? 2 * list : list;
         carry = hist + (passes ? kSortBlocks * kBins * sizeof(uint32_t) : 0);
@@ -461,7 +460,7 @@ int embedding_grad_on_stream(API *dtable, const API *dout, const int64_t *ids, v
     if (!ops.ok()) return NVSHMEMX_ERROR_INVALID_VALUE;
     Item *sorted = (Item *)ws, *other = (Item *)(ws + space.items);
     if (n && !space.passes) {
-        launch_kernel(embedding_rank_kernel, dim3(div_up(n, kLanes)), dim3(kSortThreads), 0, stream, sorted, id, rt.heap_size,
+        launch_kernel(embedding_rank_kernel, dim3(div_up(n, kRankKeys)), dim3(kSortThreads), (n + 63) / 64 * 256, stream, sorted, id, rt.heap_size,
                       (unsigned)tokens, (unsigned)n, (unsigned)vocab);
     } else if (n) {
         uint32_t *hist = (uint32_t *)(ws + space.hist);

@@ -134,7 +134,7 @@ struct Slots {
                 vec v;
 #pragma unroll
                 for (int i = 0; i < W; ++i) v[i] = x[u + i];
-                *reinterpret_cast<vec_unaligned *>(row + e) = v;
+                __builtin_nontemporal_store(v, reinterpret_cast<vec_unaligned *>(row + e));
             } else {
 #pragma unroll
                 for (int i = 0; i < W; ++i)
@@ -374,6 +374,7 @@ __global__ __launch_bounds__(kFinishWaves *kLanes) void route_finish_kernel(int6
 }
 
 constexpr int kGradThreads = 256;
+constexpr unsigned kGradBlocks = 1024;  // of all PEs
 
 template <typename T, int G, int V>
 __global__ __launch_bounds__(kGradThreads) void route_grad_kernel(T *dlogits, const T *logits, const int32_t *expert,
@@ -651,7 +652,7 @@ int route_grad_on_stream(API *dlogits, const API *logits, const int32_t *expert,
     if (tokens == 0) return 0;
 #define NVSHMEM_AMD_LAUNCH_GRAD(G, V)                                                                                             \
     {                                                                                                                             \
-        const unsigned steps = div_up(tokens, kGradThreads / G), most = 1024 / (unsigned)rt.npes;                                \
+        const unsigned steps = div_up(tokens, kGradThreads / G), most = kGradBlocks / (unsigned)rt.npes;                                \
         launch_kernel(route_grad_kernel<T, G, V>, dim3(steps < most ? steps : most, 1, rt.npes), dim3(kGradThreads), 0, stream,  \
                       out, in, to, dg, b, dl, rt.heap_size, (unsigned)tokens, (unsigned)experts, (unsigned)topk, normalise != 0, scale); \
     }

@@ -32,6 +32,10 @@ struct element<nvshmem_bfloat16_t> {
 
 constexpr int kLanes = 64;
 
+// How a row's chunks lie on lanes: a wavefront and more to a row, rows that share a wavefront, rows of less than a chunk (which
+// share one as well).
+enum { kWhole, kShared, kTiny };
+
 // A row is handled in chunks of 16 bytes, counted from its first element whatever that is aligned to: gfx950 takes 16-byte
 // accesses at any address (one global_load_dwordx4 either way), so rows of an odd number of elements need no kernel of their own.
 template <typename T>
@@ -57,10 +61,6 @@ template <typename T>
 __device__ __forceinline__ void chunk_store_stream(T *p, typename Chunk<T>::vec v) {
     __builtin_nontemporal_store(v, reinterpret_cast<typename Chunk<T>::vec_unaligned *>(p));
 }
-// How a row's chunks lie on lanes: a wavefront and more to a row, rows that share a wavefront, rows of less than a chunk (which
-// share one as well).
-enum { kWhole, kShared, kTiny };
-
 // ... and written through to memory, past the L2.
 template <typename T>
 __device__ __forceinline__ void chunk_store_through(T *p, typename Chunk<T>::vec v) {
@@ -86,6 +86,13 @@ __device__ __forceinline__ void chunk_store_part(T *p, typename Chunk<T>::vec v,
 #pragma unroll
     for (int i = 0; i < Chunk<T>::N; ++i)
         if (i < (int)n) p[i] = v[i];
+}
+// All but the first `n` elements.
+template <typename T>
+__device__ __forceinline__ void chunk_store_behind(T *p, typename Chunk<T>::vec v, unsigned n) {
+#pragma unroll
+    for (int i = 0; i < Chunk<T>::N; ++i)
+        if (i >= (int)n) p[i] = v[i];
 }
 template <typename T>
 __device__ __forceinline__ typename Chunk<T>::facc chunk_to_float(typename Chunk<T>::vec v) {
@@ -172,28 +179,28 @@ class Operands {
   private:
     void *add(const char *name, const void *p, uint64_t elems, uint64_t size, uint64_t align, bool written) {
         if (!ok_ || elems == 0) return nullptr;
-        char label[96];
-        snprintf(label, sizeof label, "%s %s", what_, name);
         uint64_t off = 0;
-        if (elems > rt_.heap_size / size) {
-            set_error("%s: %llu elements leave the PE's heap slice", label, (unsigned long long)elems);
-            return fail();
-        }
-        if (!check_symmetric_range(rt_, label, p, elems * size, &off)) return fail();
-        if (off % align) {
-            set_error("%s: must be aligned to %llu bytes", label, (unsigned long long)align);
-            return fail();
-        }
+        const bool fits = elems <= rt_.heap_size / size;
+        if (!fits || !rt_.usable(p, elems * size, &off) || off % align) return refuse(name, p, fits, elems, size, align);
         const uint64_t end = off + elems * size;
         for (int i = 0; i < n_; ++i) {
             if (!written && !op_[i].written) continue;
             if (off >= op_[i].end || op_[i].off >= end) continue;
             if (may_be_ && off == op_[i].off && end == op_[i].end && may_be_ == rt_.base + off) continue;
-            set_error("%s: overlaps %s", label, op_[i].name);
+            set_error("%s %s: overlaps %s", what_, name, op_[i].name);
             return fail();
         }
         if (n_ < kMost) op_[n_++] = {name, off, end, written};
         return rt_.base + off;
+    }
+    // (a call that is fine makes no text)
+    void *refuse(const char *name, const void *p, bool fits, uint64_t elems, uint64_t size, uint64_t align) {
+        char label[96];
+        snprintf(label, sizeof label, "%s %s", what_, name);
+        uint64_t off = 0;
+        if (!fits) set_error("%s: %llu elements leave the PE's heap slice", label, (unsigned long long)elems);
+        else if (check_symmetric_range(rt_, label, p, elems * size, &off)) set_error("%s: must be aligned to %llu bytes", label, (unsigned long long)align);
+        return fail();
     }
     void *fail() {
         ok_ = false;

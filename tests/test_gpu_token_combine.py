@@ -22,7 +22,7 @@ def _tables(rng, npes, tokens, topk, cap, dropped=0.15):
 
 SIZES = [  # npes, tokens, topk, dim, shift of the rows' buffers in elements
     (8, 20, 8, 512, 0), (4, 33, 3, 1029, 1), (4, 7, 1, 1, 0), (16, 5, 6, 7168, 0), (2, 65, 9, 63, 3), (3, 10, 17, 2050, 2),
-    (1, 12, 4, 129, 0), (8, 1, 2, 8192, 0)]
+    (1, 12, 4, 129, 0), (8, 1, 2, 8192, 0), (2, 9, 5, 600, 1), (4, 6, 7, 100, 0), (2, 5, 4, 5, 3), (2, 150, 2, 2053, 1)]
 
 
 @pytest.mark.parametrize("npes,tokens,topk,dim,shift", SIZES)

@@ -217,6 +217,43 @@ def test_place(npes, tokens, experts, topk, cap):
         ws.get()
 
 
+@pytest.mark.parametrize("npes,tokens,experts,topk", [(2, 66000, 6, 2), (4, 30000, 1024, 4), (8, 20000, 64, 8)])
+def test_place_many(npes, tokens, experts, topk):
+    """Copies of several blocks, on either side of where a thread takes more of them."""
+    rng = np.random.default_rng(tokens)
+    e = np.argsort(rng.random((npes, tokens, experts), np.float32) if experts < 100 else rng.random((npes, tokens, 8), np.float32),
+                   axis=2)[..., :topk].astype(np.int32)
+    if experts >= 100:
+        e += 8 * rng.integers(0, experts // 8, (npes, tokens, 1), np.int32)
+    e[rng.random(e.shape) < 0.1] = -1
+    cap = tokens * topk * 9 // 10
+    counts_values = np.stack([np.bincount(e[pe][e[pe] >= 0], minlength=experts) for pe in range(npes)])
+    per_pe = experts // npes
+    source = np.broadcast_to(np.arange(npes)[:, None, None], e.shape)
+    key = np.where(e >= 0, e * npes + source, experts * npes).reshape(-1)
+    rank = np.empty(key.size, np.int64)
+    rank[np.argsort(key, kind="stable")] = np.arange(key.size)
+    first = np.searchsorted(np.sort(key), np.arange(npes + 1) * per_pe * npes)
+    pe = np.minimum(key // (per_pe * npes), npes)
+    row = rank - first[pe]
+    ok = (pe < npes) & (row < cap)
+    with runtime(npes, 64 << 20) as rt, Arrays(rt) as new:
+        expert, counts = new("int32", (tokens, topk), e), new("int64", (experts,), counts_values)
+        dest_pe, dest_row = new("int32", (tokens, topk)), new("int64", (tokens, topk))
+        expected, expert_row = new("int64", (npes,)), new("int64", (per_pe + 1,))
+        ws = new.workspace("moe_place", tokens, topk, experts)
+        note("moe_place", npes, tokens, experts, topk)
+        rt.moe_place(dest_pe.address, dest_row.address, expected.address, expert_row.address, ws.address, expert.address,
+                     counts.address, tokens, topk, experts, cap)
+        rt.sync()
+        assert np.array_equal(dest_pe.get().reshape(-1), np.where(ok, pe, -1))
+        assert np.array_equal(dest_row.get().reshape(-1), np.where(ok, row, -1))
+        want = np.zeros((npes, npes), np.int64)
+        np.add.at(want, (pe[ok], source.reshape(-1)[ok]), 1)
+        assert np.array_equal(expected.get(), want)
+        ws.get()
+
+
 def test_place_of_counts_that_are_not_the_experts():
     """Rows may then be given twice, but never outside of what there is."""
     npes, tokens, experts, topk, cap = 4, 300, 16, 2, 50
