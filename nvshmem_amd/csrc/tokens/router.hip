@@ -160,7 +160,14 @@ struct RouteArgs {
 };
 
 // Threads of a block: few for few tokens, which then spread over more compute units, many for many, whose second kernel then has
-// fewer rows to read.
+// fewer rows to read.  us with 256 / 1024, 256 experts, bf16: 1024 tokens in all 6.4 / 9.2, 8192 8.2 / 10.4; from 16384 on 1024 are ahead,
+// with 65536 tokens by what the second kernel saves (14.0 with 1024 blocks, 9.6 with 256).
+//
+// What bounds it in large batches is the vector unit, busy for 78 % of the time: 642 instructions for 4 tokens of 256 experts, of which
+// 236 compare keys, 64 carry them to other lanes, 96 make them and 100 are the softmax.  65536 tokens of 256 fp32 logits: 26.5 us (the
+// 67 MB alone would take 10.5); bf16 23.  8 lanes a token with twice the keys each take as long.  Four tokens to a group, merged
+// so that each quad of lanes ends up with one (5 merges for 4 tokens instead of 16), spill and take 35 us; the next tokens' logits
+// loaded ahead change nothing.
 constexpr unsigned kRouteThreads = 256, kRouteMostThreads = 1024;
 
 template <typename T, int G, int V, int KP>
@@ -290,7 +297,8 @@ __global__ __launch_bounds__(kRouteMostThreads) void route_kernel(const T *logit
 }
 
 // Counts, loss and its derivative from what the blocks of all PEs left.  A block has 8 experts, a wavefront 8 rows of a PE's at a
-// time, so that no wavefront waits for another until all PEs are added up.
+// time, so that no wavefront waits for another until all PEs are added up (32 experts a block, waiting after each PE: 25 us, so
+// 9.6, for 256 rows of 256 experts).  It waits for memory four times in a row: rows, own result, ticket, all results.
 constexpr unsigned kFinishExperts = 8, kFinishWaves = 16;
 
 __global__ __launch_bounds__(kFinishWaves *kLanes) void route_finish_kernel(int64_t *counts, float *loss, float *balance, char *work,
@@ -373,8 +381,10 @@ __global__ __launch_bounds__(kFinishWaves *kLanes) void route_finish_kernel(int6
     if (threadIdx.x < npes) copy_of(loss, threadIdx.x, stride)[0] = (float)v;
 }
 
+// Bound by memory: logits read once, their gradient written once.  us for 65536 tokens of 256 fp32 logits (138 MB): 27.5 are 5.0 TB/s;
+// with stores that stay in the caches 33.7.  Blocks of all PEs: 4096 (a step each) 32.5, 2048 29.3, 1024 27.5.
 constexpr int kGradThreads = 256;
-constexpr unsigned kGradBlocks = 1024;  // of all PEs
+constexpr unsigned kGradBlocks = 1024;
 
 template <typename T, int G, int V>
 __global__ __launch_bounds__(kGradThreads) void route_grad_kernel(T *dlogits, const T *logits, const int32_t *expert,
@@ -453,10 +463,12 @@ __global__ __launch_bounds__(kGradThreads) void route_grad_kernel(T *dlogits, co
 // ---- the shuffle's tables ----
 // A stable counting sort of the copies by expert: rows of a destination PE lie in the order (expert, source PE, token, k).  Nothing
 // here is much data; what it costs is waiting, so a block asks for all that it needs from memory at once, at its start.
-// Copies of a thread: one where a block has room for all of a PE's, two up to kPlaceSpread of them, which then spread over more
-// compute units, eight beyond, as each block adds up what the blocks in front of it counted.
+// Copies of a thread: one where a block has room for all of a PE's, two for fewer than kPlaceSpread of them, which then spread over
+// more compute units, eight beyond, as each block adds up what the blocks in front of it counted.  us with 1 | 2 | 8, 8 PEs, 256 experts:
+// 512 copies a PE 5.4 | 6.2 | 10.7, 65536 11.5 | 8.6 | 11.8, 131072 27.5 | 14.1 | 13.4, 262144 61.7 | 31.0 | 15.7 (and 4.9 for the counts in
+// front of it, from two blocks on).
 constexpr uint64_t kPlaceSpread = 1 << 17;
-unsigned place_rounds(uint64_t copies) { return copies <= kSortThreads ? 1 : copies <= kPlaceSpread ? 2 : 8; }
+unsigned place_rounds(uint64_t copies) { return copies <= kSortThreads ? 1 : copies < kPlaceSpread ? 2 : 8; }
 
 template <unsigned ROUNDS>
 __global__ __launch_bounds__(kSortThreads) void place_count_kernel(uint32_t *hist, const int32_t *expert, uint64_t stride,
@@ -553,7 +565,8 @@ __global__ __launch_bounds__(kSortThreads) void place_kernel(int32_t *dest_pe, i
 }
 
 // ---- host ----
-constexpr unsigned kFewBlocks = 512, kManyBlocks = 256;
+// (a lane adds up at most kMostSteps shares in fp32)
+constexpr unsigned kFewBlocks = 512, kManyBlocks = 256, kMostSteps = 64;
 // Blocks of a PE: enough of them over all PEs to fill the GPU, and no more, as the second kernel reads what each one leaves.
 struct RouteShape {
     unsigned threads, per_block, blocks;
@@ -563,8 +576,8 @@ struct RouteShape {
         const uint64_t all = (uint64_t)tokens * npes;
         threads = all * group <= kFewBlocks * kRouteThreads ? kRouteThreads : kRouteMostThreads;
         const unsigned groups = threads / group, most = threads == kRouteThreads ? kFewBlocks : kManyBlocks;
-        const uint64_t steps = (all + groups - 1) / groups;
-        per_block = groups * (unsigned)(steps <= most ? 1 : (steps + most - 1) / most);
+        const uint64_t steps = (all + groups - 1) / groups, each = (steps + most - 1) / most;
+        per_block = groups * (unsigned)(each < 1 ? 1 : each < kMostSteps ? each : kMostSteps);
         blocks = tokens ? div_up(tokens, per_block) : 1;
         const uint64_t table = ((uint64_t)blocks * experts * 4 + 63) / 64 * 64;
         hist = 0;
