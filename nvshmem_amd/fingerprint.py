@@ -1,4 +1,5 @@
-"""Fingerprint of the sources the GPU kernels are compiled from.
+"""Fingerprint of the sources that the benchmark's GPU kernels are compiled from (the operators under csrc/tokens share no
+code with them and are not among its workloads).
 
 A profile summary under profiles/ records the fingerprint of the tree it was measured on; the benchmark
 quotes a summary's measured HBM traffic only while the fingerprint still matches, so a kernel change
