@@ -47,7 +47,7 @@ __global__ __launch_bounds__(64) void embedding_kernel(T *__restrict__ out, cons
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const vec y = chunk_from_float<T>(chunk_to_float<T>(x[v]) * scale);
+            const vec y = chunk_from_float<T>(chunk_to_float<T>(x[v]) * (id < vocab ? scale : 0.0f));
             if (MODE == kTiny) chunk_store_part(dst, y, dim);
             else if (v == 0 || mine[v]) chunk_store_through(dst + first[v], y);
         }
@@ -356,9 +356,9 @@ __global__ __launch_bounds__(kJoinWaves *kLanes) void embedding_join_kernel(T *d
     typedef typename Partial<T>::type stored;
     __shared__ facc partial[kJoinWaves - 1][kLanes];
     const unsigned wave = wave_of_block(), lane = threadIdx.x % kLanes;
-    const unsigned c = blockIdx.y * kLanes + lane, first = chunk_first<T>(c, a.dim);
+    const unsigned c = blockIdx.x * kLanes + lane, first = chunk_first<T>(c, a.dim);
     const bool mine = c * Chunk<T>::N < a.dim;
-    for (unsigned part = blockIdx.x; part + 1 < a.parts; part += gridDim.x) {
+    for (unsigned part = blockIdx.y; part + 1 < a.parts; part += gridDim.y) {
         const unsigned begin = part * a.part, end = begin + a.part;
         const uint32_t k = a.sorted[end - 1].key, after = a.sorted[end].key, prior = a.sorted[begin > 0 ? begin - 1 : 0].key;
         if (k >= a.vocab || after != k || (begin > 0 && prior == k)) continue;
@@ -476,7 +476,11 @@ int embedding_grad_on_stream(API *dtable, const API *dout, const int64_t *ids, v
         const dim3 grid(div_up(n, per_block));
         Item *out = space.passes % 2 ? sorted : other, *in = space.passes % 2 ? other : sorted;
         for (unsigned p = 0; p < space.passes; ++p) {
-#define NVSHMEM_AMD_SORT(FIRST)                                                                                                          launch_kernel(embedding_count_kernel<FIRST>, grid, dim3(kSortThreads), 0, stream, hist, in, id, rt.heap_size, (unsigned)tokens,                    (unsigned)n, (unsigned)vocab, per_block, p * kDigit);                                                                  launch_kernel(embedding_sort_kernel<FIRST>, grid, dim3(kSortThreads), 0, stream, out, hist, in, id, rt.heap_size,                                  (unsigned)tokens, (unsigned)n, (unsigned)vocab, per_block, p * kDigit)
+#define NVSHMEM_AMD_SORT(FIRST)                                                                                                       \
+    launch_kernel(embedding_count_kernel<FIRST>, grid, dim3(kSortThreads), 0, stream, hist, in, id, rt.heap_size, (unsigned)tokens,  \
+                  (unsigned)n, (unsigned)vocab, per_block, p * kDigit);                                                              \
+    launch_kernel(embedding_sort_kernel<FIRST>, grid, dim3(kSortThreads), 0, stream, out, hist, in, id, rt.heap_size,                \
+                  (unsigned)tokens, (unsigned)n, (unsigned)vocab, per_block, p * kDigit)
             if (p == 0) {
                 NVSHMEM_AMD_SORT(true);
             } else {
@@ -497,8 +501,8 @@ int embedding_grad_on_stream(API *dtable, const API *dout, const int64_t *ids, v
     a.zero_rows = kLanes;
     launch_kernel(embedding_sum_kernel<T>, dim3(a.sum_blocks + div_up(vocab, a.zero_rows)), dim3(kLanes), 0, stream, tab, src, a);
     if (a.parts > 1)
-        launch_kernel(embedding_join_kernel<T>, dim3(a.parts < (1u << 20) ? a.parts : 1u << 20, a.pieces), dim3(kJoinWaves * kLanes), 0,
-                      stream, tab, a);
+        launch_kernel(embedding_join_kernel<T>, dim3(a.pieces, a.parts < 65535 ? a.parts : 65535), dim3(kJoinWaves * kLanes), 0, stream,
+                      tab, a);
     return launched("embedding_grad");
 }
 

@@ -24,7 +24,9 @@ constexpr int kMostExperts = 1024, kMostTopk = 16;
 // and v_min_f64 compare.  A key whose logit is -inf (or that is `none`, whose logit reads as NaN) is a masked expert's.
 __device__ __forceinline__ uint32_t ascending(uint32_t b) { return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u); }
 __device__ __forceinline__ uint32_t ascending_back(uint32_t s) { return s ^ (~(uint32_t)((int32_t)s >> 31) | 0x80000000u); }
-__device__ __forceinline__ float clean(float x) { return fmaxf(x, -__builtin_inff()) + 0.0f; }
+// (the sum first: it quiets a signalling NaN, which a maximum would return; widening a bf16 leaves it one, whatever the compiler
+// takes that for)
+__device__ __forceinline__ float clean(float x) { return fmaxf(x + 0.0f, -__builtin_inff()); }
 
 template <typename T>
 struct Key {  // _Float16, __bf16
@@ -426,12 +428,15 @@ __global__ __launch_bounds__(kGradThreads) void route_grad_kernel(T *dlogits, co
         const bool chosen = (unsigned)e < experts && l > -__builtin_inff();
         float p[V], m = -__builtin_inff();
 #pragma unroll
-        for (int u = 0; u < V; ++u) m = fmaxf(m, (float)x[u]);  // (fmax passes NaN over)
+        for (int u = 0; u < V; ++u) {
+            p[u] = clean((float)x[u]);
+            m = fmaxf(m, p[u]);
+        }
         m = group_max<G>(m);
         float z = 0.0f, bp = 0.0f;
 #pragma unroll
         for (int u = 0; u < V; ++u) {
-            p[u] = (float)x[u] > -__builtin_inff() ? exp_below((float)x[u], m) : 0.0f;
+            p[u] = p[u] > -__builtin_inff() ? exp_below(p[u], m) : 0.0f;
             z += p[u];
             bp = __builtin_fmaf(p[u], b[u], bp);
         }

@@ -82,6 +82,42 @@ def test_route(kind, npes, tokens, experts, topk, shift, how):
             ws.get()
 
 
+@pytest.mark.parametrize("experts", [12, 200, 600])
+@pytest.mark.parametrize("kind,nans", [("float", [0x7F800001, 0xFF800001, 0x7FFFFFFF, 0xFFC00000]), ("half", [0x7C01, 0xFC01, 0x7FFF, 0xFE00]),
+                                       ("bfloat16", [0x7F81, 0xFF81, 0x7FFF, 0xFFC0])])
+def test_every_nan_masks(kind, nans, experts):
+    """Signalling and quiet ones of both signs."""
+    npes, tokens, topk = 2, 9, 4
+    rng = np.random.default_rng(12)
+    x = rounded(rng.standard_normal((npes, tokens, experts)), kind)
+    at = rng.random(x.shape) < 0.3
+    at[0, 0] = True
+    bits = np.uint32 if kind == "float" else np.uint16
+    with runtime(npes, 16 << 20) as rt, Arrays(rt) as new:
+        logits, dlogits = new(kind, (tokens, experts), x), new(kind, (tokens, experts))
+        for pe in range(npes):
+            raw = rt.download(logits.base, pe, (tokens, experts), bits, logits.first)
+            raw[at[pe]] = rng.choice(np.array(nans, bits), at[pe].sum())
+            rt.upload(logits.base, pe, raw, logits.first)
+        x[at] = np.nan
+        expert, gate, counts = new("int32", (tokens, topk)), new("float", (tokens, topk)), new("int64", (experts,))
+        loss, balance, dloss = new("float", (1,)), new("float", (experts,)), new("float", (1,), np.float32(1))
+        ws = new.workspace("moe_route", tokens, experts)
+        for normalise in (True, False):
+            rt.moe_route(kind, expert.address, gate.address, counts.address, ws.address, logits.address, tokens, experts, topk,
+                         loss.address, balance.address, normalise)
+            rt.moe_route_grad(kind, dlogits.address, logits.address, expert.address, gate.address, tokens, experts, topk,
+                              balance.address, dloss.address, normalise)
+            rt.sync()
+            want_expert, want_gate, want_counts, want_loss, b = R.route(x, topk, normalise, 1.0)
+            tol = _exp_tolerance(x)
+            assert np.array_equal(expert.get(), want_expert) and np.array_equal(counts.get(), want_counts)
+            close(gate.get(), want_gate, tol * R.STEP * want_gate + 1e-37, "gate")
+            close(loss.get(), np.full((npes, 1), want_loss), (tol + 72) * R.STEP * want_loss, "loss")
+            want, size = R.route_grad(x, want_expert, gate.get(), balance.get(), np.ones(npes), normalise, 1.0)
+            close(dlogits.get(), want, (3 * tol + 52) * R.STEP * size + EPS[kind] / 2 * np.abs(want) * 1.01 + TINY[kind] + 1e-36, "dlogits")
+
+
 @pytest.mark.parametrize("npes,tokens,experts,topk", [(8, 2100, 256, 8), (2, 17000, 64, 2), (4, 1500, 1024, 3), (8, 0, 16, 2)])
 def test_many_tokens_and_none(npes, tokens, experts, topk):
     rng = np.random.default_rng(tokens)
