@@ -12,11 +12,16 @@ namespace tokens {
 namespace {
 
 // One wavefront per piece of V x 64 chunks of a row; a row of fewer chunks than a wavefront has lanes takes the next power of two of
-// them and shares the wavefront with others (2^lanes_log lanes a row).  Reads a row of the table and writes one: bound by memory.
-// Where a wavefront has one token, its id is a scalar load and its rows are scalar addresses.
+// them and shares the wavefront with others (2^lanes_log lanes a row).  Reads a row of the table and writes one: bound by memory, and
+// for short rows by the rate at which wavefronts start, so there one has TOKENS tokens (or TOKENS for each row's lanes).
+// Where a wavefront has whole tokens, their ids are scalar loads and their rows scalar addresses.
 // us for 8 x 4096 rows of 7168 bf16 (0.47 GB written, about a third of that read from memory: 113 us are 5.5 TB/s): one chunk a lane
 // 141, two 120, four (of 14) 130, seven 116; two, written through to memory 113.  8 x 64 rows: 4.4, written through 4.0.
-template <typename T, int V, int MODE>
+// Rows of up to four pieces of 64 chunks are one wavefront's, against two pieces each: 8 x 20000 rows of 1152 73 / 141, of 2048 118 / 150.
+// One / four tokens a wavefront: 8 x 5970 rows of 512 bf16 (47760 wavefronts of one) 22.2 / 10.8, 8 x 600 (4800) 4.2 / 3.5, 8 x 64 (512)
+// 2.3 / 2.7; 8 x 5970 rows of 64 (5976) 5.0 / 3.8, 8 x 2100 (2104) 3.3 / 3.4.  Two tokens for rows of 900: 14.6 / 15.1, not taken.
+constexpr uint64_t kManyWaves = 4096;
+template <typename T, int V, int TOKENS, int MODE>
 __global__ __launch_bounds__(64) void embedding_kernel(T *__restrict__ out, const T *__restrict__ table, const int64_t *__restrict__ ids,
                                                        uint64_t stride, unsigned tokens, unsigned vocab, unsigned rows, unsigned dim,
                                                        unsigned lanes_log, float scale) {
@@ -32,24 +37,33 @@ __global__ __launch_bounds__(64) void embedding_kernel(T *__restrict__ out, cons
     if (!mine[0]) return;
     const int64_t *my_ids = copy_of(ids, pe, stride);
     T *my_out = copy_of(out, pe, stride);
-    for (uint64_t t = (uint64_t)blockIdx.y * per_wave + (MODE == kWhole ? 0 : lane >> log); t < tokens;
-         t += (uint64_t)gridDim.y * per_wave) {
-        const uint64_t id = (uint64_t)my_ids[t];
-        T *dst = my_out + t * dim;
-        vec x[V] = {};
-        if (id < vocab) {
-            const unsigned owner = (unsigned)id / rows, row = (unsigned)id % rows;
+    for (uint64_t t0 = (uint64_t)blockIdx.y * per_wave * TOKENS + (MODE == kWhole ? 0 : lane >> log); t0 < tokens;
+         t0 += (uint64_t)gridDim.y * per_wave * TOKENS) {
+        uint64_t id[TOKENS];
+#pragma unroll
+        for (int i = 0; i < TOKENS; ++i) id[i] = (uint64_t)my_ids[t0 + i * per_wave < tokens ? t0 + i * per_wave : t0];
+        vec x[TOKENS][V] = {};
+#pragma unroll
+        for (int i = 0; i < TOKENS; ++i) {
+            if (id[i] >= vocab) continue;
+            const unsigned owner = (unsigned)id[i] / rows, row = (unsigned)id[i] % rows;
             const T *src = copy_of(table, owner, stride) + (uint64_t)row * dim;
 #pragma unroll
             for (int v = 0; v < V; ++v)
-                if (MODE == kTiny) x[v] = chunk_load_part(src, dim);
-                else if (v == 0 || mine[v]) x[v] = chunk_load(src + first[v]);
+                if (MODE == kTiny) x[i][v] = chunk_load_part(src, dim);
+                else if (v == 0 || mine[v]) x[i][v] = chunk_load(src + first[v]);
         }
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const vec y = chunk_from_float<T>(chunk_to_float<T>(x[v]) * (id < vocab ? scale : 0.0f));
-            if (MODE == kTiny) chunk_store_part(dst, y, dim);
-            else if (v == 0 || mine[v]) chunk_store_through(dst + first[v], y);
+        for (int i = 0; i < TOKENS; ++i) {
+            const uint64_t t = t0 + i * per_wave;
+            if (t >= tokens) break;
+            T *dst = my_out + t * dim;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const vec y = chunk_from_float<T>(chunk_to_float<T>(x[i][v]) * (id[i] < vocab ? scale : 0.0f));
+                if (MODE == kTiny) chunk_store_part(dst, y, dim);
+                else if (v == 0 || mine[v]) chunk_store_through(dst + first[v], y);
+            }
         }
     }
 }
@@ -417,15 +431,24 @@ int embedding_on_stream(API *out, const API *table, const int64_t *ids, size_t t
     if (!ops.ok()) return NVSHMEMX_ERROR_INVALID_VALUE;
     if (tokens == 0) return 0;
     const size_t chunks = (dim + Chunk<T>::N - 1) / Chunk<T>::N;
-    const unsigned log = row_lanes_log2(chunks), groups = div_up(tokens, kLanes >> log);
-    const unsigned most = groups < 65535 ? groups : 65535;
-#define NVSHMEM_AMD_LAUNCH_EMBEDDING(V, MODE)                                                                                          \
-    launch_kernel((embedding_kernel<T, V, MODE>), dim3(div_up(chunks, kLanes * V), most, rt.npes), dim3(kLanes), 0, stream, dst, tab,  \
-                  id, rt.heap_size, (unsigned)tokens, (unsigned)vocab, (unsigned)rows, (unsigned)dim, log, scale)
-    if (dim < (size_t)Chunk<T>::N) NVSHMEM_AMD_LAUNCH_EMBEDDING(1, kTiny);
-    else if (chunks > kLanes) NVSHMEM_AMD_LAUNCH_EMBEDDING(2, kWhole);
-    else if (log == 6) NVSHMEM_AMD_LAUNCH_EMBEDDING(1, kWhole);
-    else NVSHMEM_AMD_LAUNCH_EMBEDDING(1, kShared);
+    const unsigned log = row_lanes_log2(chunks), per_wave = kLanes >> log;
+    const bool many = (uint64_t)tokens * rt.npes / per_wave >= kManyWaves;
+#define NVSHMEM_AMD_LAUNCH_EMBEDDING(V, TOKENS, MODE)                                                                                  \
+    {                                                                                                                                  \
+        const unsigned groups = div_up(tokens, per_wave * TOKENS);                                                                     \
+        launch_kernel((embedding_kernel<T, V, TOKENS, MODE>), dim3(div_up(chunks, kLanes * V), groups < 65535 ? groups : 65535, rt.npes), \
+                      dim3(kLanes), 0, stream, dst, tab, id, rt.heap_size, (unsigned)tokens, (unsigned)vocab, (unsigned)rows,          \
+                      (unsigned)dim, log, scale);                                                                                      \
+    }
+    if (dim < (size_t)Chunk<T>::N) NVSHMEM_AMD_LAUNCH_EMBEDDING(1, 1, kTiny)
+    else if (chunks > 4 * kLanes) NVSHMEM_AMD_LAUNCH_EMBEDDING(2, 1, kWhole)
+    else if (chunks > 3 * kLanes) NVSHMEM_AMD_LAUNCH_EMBEDDING(4, 1, kWhole)
+    else if (chunks > 2 * kLanes) NVSHMEM_AMD_LAUNCH_EMBEDDING(3, 1, kWhole)
+    else if (chunks > kLanes) NVSHMEM_AMD_LAUNCH_EMBEDDING(2, 1, kWhole)
+    else if (log == 6 && many) NVSHMEM_AMD_LAUNCH_EMBEDDING(1, 4, kWhole)
+    else if (log == 6) NVSHMEM_AMD_LAUNCH_EMBEDDING(1, 1, kWhole)
+    else if (many) NVSHMEM_AMD_LAUNCH_EMBEDDING(1, 4, kShared)
+    else NVSHMEM_AMD_LAUNCH_EMBEDDING(1, 1, kShared)
 #undef NVSHMEM_AMD_LAUNCH_EMBEDDING
     return launched("embedding");
 }

@@ -54,6 +54,26 @@ def test_lookup(kind, npes, tokens, vocab, dim, shift):
                 assert np.array_equal(got, want) and not np.signbit(got[~ok]).any()
 
 
+@pytest.mark.parametrize("npes,tokens,vocab,dim,shift", [  # wavefronts with four tokens, and with three or four chunks a lane
+    (8, 700, 999, 509, 1), (8, 513, 999, 252, 0), (3, 1367, 100, 511, 0), (8, 4097, 77, 72, 2), (16, 4099, 1000, 20, 0),
+    (1, 4096, 5, 256, 0), (4, 77, 130, 769, 1), (4, 77, 130, 1021, 0), (4, 77, 130, 1531, 3), (2, 90, 7, 1544, 0), (2, 90, 7, 2045, 1)])
+@pytest.mark.parametrize("kind", ["float", "half", "bfloat16"])
+def test_lookup_of_many_and_of_wider_rows(kind, npes, tokens, vocab, dim, shift):
+    rng = np.random.default_rng(dim)
+    with runtime(npes, 64 << 20) as rt, Arrays(rt) as new:
+        table_values = rounded(rng.standard_normal((npes, -(-vocab // npes), dim)), kind)
+        table = new(kind, table_values.shape[1:], table_values, shift)
+        ids_values = _ids(rng, npes, tokens, vocab, "padding")
+        ids, out = new("int64", (tokens,), ids_values), new(kind, (tokens, dim), shift=shift)
+        note("embedding", kind, npes, tokens, vocab, dim)
+        rt.embedding(kind, out.address, table.address, ids.address, tokens, vocab, dim, 0.5)
+        rt.sync()
+        ok = (ids_values >= 0) & (ids_values < vocab)
+        found = table_values.reshape(-1, dim)[np.where(ok, ids_values, 0)]
+        # half of a value is exact but for fp16's subnormals, which round once
+        assert np.array_equal(out.get(), rounded(np.where(ok[..., None], found * np.float32(0.5), np.float32(0)), kind))
+
+
 @pytest.mark.parametrize("how", ["any", "padding", "one", "none", "zipf"])
 @pytest.mark.parametrize("npes,tokens,vocab,dim,shift", SIZES)
 @pytest.mark.parametrize("kind", ["float", "half", "bfloat16"])
