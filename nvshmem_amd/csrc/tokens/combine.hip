@@ -70,6 +70,7 @@ __global__ __launch_bounds__(64) void combine_sum_kernel(T *__restrict__ out, co
                 const T *from = copy_of(recv, d[k], stride) + r[k] * dim;
                 src[k] = ok ? from : dst;
                 bits[k] = ok ? ~0u : 0u;
+                w[k] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, w[k]) & bits[k]);  // (it may be infinite or a NaN)
             }
             typename Chunk<T>::vec x[K];
 #pragma unroll

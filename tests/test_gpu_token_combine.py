@@ -100,6 +100,34 @@ def test_long_rows_are_added_up_in_parts():
         close(dgate.get(), want, (128 + 10 + 1) * R.STEP * size, "dgate")
 
 
+@pytest.mark.parametrize("topk", [1, 3, 8, 11])
+@pytest.mark.parametrize("kind,dim", [("float", 3), ("bfloat16", 100), ("half", 520)])
+def test_a_dropped_copy_s_gate_adds_nothing(kind, dim, topk):
+    rng = np.random.default_rng(dim + topk)
+    npes, tokens, cap = 2, 9, 9 * topk
+    with runtime(npes, 16 << 20) as rt, Arrays(rt) as new:
+        recv_values = rounded(np.abs(rng.standard_normal((npes, cap, dim))) + 0.5, kind)
+        pe_values, row_values = _tables(rng, npes, tokens, topk, cap, 0.9)
+        pe_values[0, 0], pe_values[1, 0, 0] = -1, npes
+        ok = R.kept(pe_values, row_values, npes, cap)
+        gate_values = rng.random((npes, tokens, topk)).astype(np.float32)
+        gate_values[~ok] = rng.choice([np.nan, np.inf, -np.inf], np.count_nonzero(~ok))
+        pe_values[1, 1, -1], row_values[1, 1, -1] = 0, 0
+        gate_values[1, 1, -1], ok[1, 1, -1] = np.inf, True         # one that counts, and is a token's last
+        recv, gate = new(kind, (cap, dim), recv_values), new("float", (tokens, topk), gate_values)
+        dest_pe, dest_row = new("int32", (tokens, topk), pe_values), new("int64", (tokens, topk), row_values)
+        out = new(kind, (tokens, dim))
+        note("moe_combine_sum", kind, npes, tokens, topk, dim)
+        rt.moe_combine_sum(kind, out.address, recv.address, cap, gate.address, dest_pe.address, dest_row.address, tokens, topk, dim)
+        rt.sync()
+        gate_values[~ok], gate_values[1, 1, -1] = 0, 1
+        want, size = R.combine_sum(recv_values, gate_values, pe_values, row_values)
+        got = out.get()
+        assert (got[1, 1] == np.inf).all()
+        got[1, 1] = want[1, 1]
+        close(got, want, 2 * topk * R.STEP * size + EPS[kind] / 2 * np.abs(want) * 1.01 + TINY[kind], "out")
+
+
 def test_infinities_and_nan_stay_with_their_token():
     with runtime(2, 16 << 20) as rt, Arrays(rt) as new:
         tokens, topk, dim = 6, 2, 40
