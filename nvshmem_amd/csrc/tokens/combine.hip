@@ -142,14 +142,16 @@ __global__ __launch_bounds__(kGradWaves *kLanes) void combine_grad_kernel(T *dre
                 vec x[K];
 #pragma unroll
                 for (unsigned k = 0; k < K; ++k) x[k] = TINY ? chunk_load_part(src[k], dim) : chunk_load_stream(src[k] + first);
-                const facc g = chunk_to_float<T>(TINY ? chunk_load_part(from, dim) : chunk_load(from + first));
-                // elements that the chunk in front has too are its: zeros here (in place, their values may be gone by now)
+                const vec raw = TINY ? chunk_load_part(from, dim) : chunk_load(from + first);
+                // elements that the chunk in front has too are its: zeros here, of both (in place, a copy's values may be gone by now, and an
+                // infinity of dout's times a zero is a NaN)
                 vec mask;
 #pragma unroll
                 for (unsigned i = 0; i < N; ++i) {
                     typedef typename same_size<sizeof(T)>::type bits;
                     mask[i] = __builtin_bit_cast(T, (bits)(i < shared ? 0 : ~(bits)0));
                 }
+                const facc g = chunk_to_float<T>(__builtin_bit_cast(vec, __builtin_bit_cast(nvshmemi_v4u, raw) & __builtin_bit_cast(nvshmemi_v4u, mask)));
 #pragma unroll
                 for (unsigned k = 0; k < K; ++k) {
                     const facc v = chunk_to_float<T>(__builtin_bit_cast(vec, __builtin_bit_cast(nvshmemi_v4u, x[k]) & __builtin_bit_cast(nvshmemi_v4u, mask)));

@@ -128,6 +128,27 @@ def test_a_dropped_copy_s_gate_adds_nothing(kind, dim, topk):
         close(got, want, 2 * topk * R.STEP * size + EPS[kind] / 2 * np.abs(want) * 1.01 + TINY[kind], "out")
 
 
+@pytest.mark.parametrize("kind,dim", [("float", 1029), ("bfloat16", 101), ("half", 9), ("bfloat16", 512), ("float", 3)])
+def test_an_infinite_gradient_is_counted_once(kind, dim):
+    npes, tokens, cap = 2, dim, dim
+    with runtime(npes, 64 << 20) as rt, Arrays(rt) as new:
+        pe_values = np.repeat(np.arange(npes, dtype=np.int32)[:, None, None], tokens, 1)
+        row_values = np.broadcast_to(np.arange(tokens)[None, :, None], (npes, tokens, 1))
+        dout_values = np.ones((npes, tokens, dim), np.float32)
+        dout_values[0, np.arange(dim), np.arange(dim)] = np.inf       # another element of each token
+        recv = new(kind, (cap, dim), np.full((npes, cap, dim), 0.5, np.float32))
+        dout, gate = new(kind, (tokens, dim), dout_values), new("float", (tokens, 1), np.ones((npes, tokens, 1)))
+        dest_pe, dest_row = new("int32", (tokens, 1), pe_values), new("int64", (tokens, 1), row_values)
+        drecv, dgate = new(kind, (cap, dim)), new("float", (tokens, 1))
+        note("moe_combine_grad", kind, npes, tokens, dim)
+        rt.moe_combine_grad(kind, drecv.address, dgate.address, dout.address, recv.address, cap, gate.address, dest_pe.address,
+                            dest_row.address, tokens, 1, dim)
+        rt.sync()
+        got = dgate.get()
+        assert (got[0] == np.inf).all() and (got[1] == dim / 2).all()
+        assert np.array_equal(drecv.get(), dout_values)
+
+
 def test_infinities_and_nan_stay_with_their_token():
     with runtime(2, 16 << 20) as rt, Arrays(rt) as new:
         tokens, topk, dim = 6, 2, 40
