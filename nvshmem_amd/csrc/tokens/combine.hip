@@ -88,6 +88,54 @@ __global__ __launch_bounds__(64) void combine_sum_kernel(T *__restrict__ out, co
     }
 }
 
+// The sum of one copy.  TOKENS tokens for each row's lanes, as wavefronts of one piece of two rows start too slowly to keep memory busy.
+// us for 8 x t rows of d bf16, one token / four: 6000 of 512 23.4 / 17.4, 6000 of 2048 86.7 / 61.6 (6.4 TB/s), 4096 of 7168 146 / 144, 600 of
+// 512 (4800 wavefronts of one) 4.9 / 4.4, 64 of 512 (512) 2.8 / 3.3; 8000 of 64 (8000) 7.4 / 6.4, 2100 of 64 (2104) 3.9 / 4.3.
+constexpr uint64_t kManyPieces = 4096;
+constexpr unsigned kTokens = 4;
+
+template <typename T, int MODE>
+__global__ __launch_bounds__(64) void combine_one_kernel(T *__restrict__ out, const T *__restrict__ recv, const float *__restrict__ gate,
+                                                         const int32_t *__restrict__ dest_pe, const int64_t *__restrict__ dest_row,
+                                                         uint64_t stride, uint64_t cap, unsigned tokens, unsigned dim, unsigned npes,
+                                                         unsigned lanes_log) {
+    typedef typename Chunk<T>::facc facc;
+    const unsigned lane = threadIdx.x, pe = blockIdx.z, log = MODE == kWhole ? 6 : lanes_log, per_wave = kLanes >> log;
+    const unsigned c = blockIdx.x * kLanes + (lane & ((1u << log) - 1));
+    if (c * Chunk<T>::N >= dim) return;
+    const unsigned first = chunk_first<T>(c, dim);
+    const int32_t *my_pe = copy_of(dest_pe, pe, stride);
+    const int64_t *my_row = copy_of(dest_row, pe, stride);
+    const float *my_gate = gate ? copy_of(gate, pe, stride) : nullptr;
+    T *my_out = copy_of(out, pe, stride);
+    for (uint64_t t0 = (uint64_t)blockIdx.y * per_wave * kTokens + (MODE == kWhole ? 0 : lane >> log); t0 < tokens;
+         t0 += (uint64_t)gridDim.y * per_wave * kTokens) {
+        unsigned d[kTokens];
+        uint64_t r[kTokens];
+        float w[kTokens];
+#pragma unroll
+        for (unsigned i = 0; i < kTokens; ++i) {
+            const uint64_t t = t0 + i * per_wave < tokens ? t0 + i * per_wave : t0;
+            d[i] = (unsigned)my_pe[t], r[i] = (uint64_t)my_row[t], w[i] = 1.0f;
+        }
+        if (my_gate) {
+#pragma unroll
+            for (unsigned i = 0; i < kTokens; ++i) w[i] = my_gate[t0 + i * per_wave < tokens ? t0 + i * per_wave : t0];
+        }
+        typename Chunk<T>::vec x[kTokens] = {};
+#pragma unroll
+        for (unsigned i = 0; i < kTokens; ++i)
+            if (d[i] < npes && r[i] < cap) x[i] = chunk_load_stream(copy_of(recv, d[i], stride) + r[i] * dim + first);
+            else w[i] = 0.0f;
+#pragma unroll
+        for (unsigned i = 0; i < kTokens; ++i) {
+            facc sum = {};
+            sum += chunk_to_float<T>(x[i]) * w[i];
+            if (t0 + i * per_wave < tokens) chunk_store_stream(my_out + (t0 + i * per_wave) * dim + first, chunk_from_float<T>(sum));
+        }
+    }
+}
+
 // A block of up to 8 wavefronts per token.  A lane loads a chunk of all K copies before it uses the first or stores any (drecv may be
 // recv), and keeps the products for the K gates in registers; they are added up lane by lane and then wavefront by wavefront.
 // Bound by memory: 8 x 2048 rows of 7168 bf16, top-8 (3.99 GB) take 651 us, 6.1 TB/s; one copy after the other 674 to 696.  4 x 501 rows of
@@ -228,6 +276,16 @@ int combine_sum_on_stream(API *out, const API *recv, size_t recv_cap_rows, const
         default: NVSHMEM_AMD_LAUNCH_SUM(8, MODE);       \
     }
     if (dim < (size_t)Chunk<T>::N) NVSHMEM_AMD_LAUNCH_SUM(8, kTiny);
+    else if (topk == 1 && (uint64_t)tokens * rt.npes / (kLanes >> log) * div_up(chunks, kLanes) >= kManyPieces) {
+        const unsigned fours = div_up(tokens, (kLanes >> log) * kTokens);
+        const dim3 grid(div_up(chunks, kLanes), fours < 65535 ? fours : 65535, rt.npes);
+        if (log == 6)
+            launch_kernel((combine_one_kernel<T, kWhole>), grid, dim3(kLanes), 0, stream, dst, src, w, to, at, rt.heap_size,
+                          (uint64_t)recv_cap_rows, (unsigned)tokens, (unsigned)dim, (unsigned)rt.npes, log);
+        else
+            launch_kernel((combine_one_kernel<T, kShared>), grid, dim3(kLanes), 0, stream, dst, src, w, to, at, rt.heap_size,
+                          (uint64_t)recv_cap_rows, (unsigned)tokens, (unsigned)dim, (unsigned)rt.npes, log);
+    }
     else if (log == 6) NVSHMEM_AMD_LAUNCH_SUM_OF(kWhole)
     else NVSHMEM_AMD_LAUNCH_SUM_OF(kShared)
 #undef NVSHMEM_AMD_LAUNCH_SUM_OF

@@ -48,6 +48,29 @@ def test_sum(kind, npes, tokens, topk, dim, shift):
             close(out.get(), want, 2 * topk * R.STEP * size + EPS[kind] / 2 * np.abs(want) * 1.01 + TINY[kind], "out")
 
 
+@pytest.mark.parametrize("npes,tokens,dim,shift", [(8, 700, 509, 1), (3, 1367, 256, 0), (8, 4099, 72, 2), (16, 4097, 20, 0),
+                                                   (4, 99, 5000, 1), (1, 4096, 257, 0)])
+@pytest.mark.parametrize("kind", ["float", "half", "bfloat16"])
+def test_sum_of_one_copy_of_many_tokens(kind, npes, tokens, dim, shift):
+    rng = np.random.default_rng(dim)
+    cap = tokens + 5
+    with runtime(npes, 64 << 20) as rt, Arrays(rt) as new:
+        recv_values = rounded(rng.standard_normal((npes, cap, dim)), kind)
+        pe_values, row_values = _tables(rng, npes, tokens, 1, cap, 0.5)
+        gate_values = rng.random((npes, tokens, 1)).astype(np.float32)
+        gate_values[~R.kept(pe_values, row_values, npes, cap)] = np.nan
+        recv, gate = new(kind, (cap, dim), recv_values, shift), new("float", (tokens, 1), gate_values)
+        dest_pe, dest_row = new("int32", (tokens, 1), pe_values), new("int64", (tokens, 1), row_values)
+        for weights in (gate, None):
+            out = new(kind, (tokens, dim), shift=shift)
+            note("moe_combine_sum", kind, npes, tokens, dim, weights is not None)
+            rt.moe_combine_sum(kind, out.address, recv.address, cap, weights and weights.address, dest_pe.address,
+                               dest_row.address, tokens, 1, dim)
+            rt.sync()
+            want, size = R.combine_sum(recv_values, weights and np.nan_to_num(gate_values), pe_values, row_values)
+            close(out.get(), want, 2 * R.STEP * size + EPS[kind] / 2 * np.abs(want) * 1.01 + TINY[kind], "out")
+
+
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("npes,tokens,topk,dim,shift", SIZES)
 @pytest.mark.parametrize("kind", ["float", "half", "bfloat16"])
