@@ -436,7 +436,7 @@ __global__ __launch_bounds__(kGradThreads) void route_grad_kernel(T *dlogits, co
         float z = 0.0f, bp = 0.0f;
 #pragma unroll
         for (int u = 0; u < V; ++u) {
-            p[u] = p[u] > -__builtin_inff() ? exp_below(p[u], m) : 0.0f;
+            p[u] = p[u] > -__builtin_inff() ? exp_below(p[u], m) : -0.0f;  // (the sign says that it is masked)
             z += p[u];
             bp = __builtin_fmaf(p[u], b[u], bp);
         }
@@ -456,7 +456,8 @@ __global__ __launch_bounds__(kGradThreads) void route_grad_kernel(T *dlogits, co
         for (int u = 0; u < V; ++u) {
             const unsigned at = Slots<T, G, V>::expert(u, sub);
             const float c = part[at], pr = p[u] * r;
-            d[u] = (T)(normalise ? __builtin_fmaf(pr, b[u] - bp, c) : pr * (b[u] + c - (bp + gs)));
+            const float v = normalise ? __builtin_fmaf(pr, b[u] - bp, c) : pr * (b[u] + c - (bp + gs));
+            d[u] = (T)(__builtin_bit_cast(uint32_t, p[u]) != 0x80000000u ? v : 0.0f);  // (a NaN or infinity upstream leaves it at 0, too)
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         __builtin_amdgcn_wave_barrier();

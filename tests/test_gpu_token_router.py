@@ -180,6 +180,33 @@ def test_route_grad(kind, npes, tokens, experts, topk, shift, how):
 
 
 @pytest.mark.parametrize("normalise", [True, False])
+@pytest.mark.parametrize("kind,experts", [("float", 10), ("half", 130), ("bfloat16", 515)])
+def test_masked_logits_get_no_gradient_whatever_comes_from_above(kind, experts, normalise):
+    npes, tokens, topk = 2, 11, 3
+    rng = np.random.default_rng(experts)
+    x = rounded(rng.standard_normal((npes, tokens, experts)), kind)
+    masked = rng.random(x.shape) < 0.4
+    masked[0, 0] = True
+    x[masked] = -np.inf
+    want_expert, gate, _, _, balance_values = R.route(x, topk, normalise, 1.0)
+    with runtime(npes, 16 << 20) as rt, Arrays(rt) as new:
+        logits, dlogits, expert = new(kind, (tokens, experts), x), new(kind, (tokens, experts)), new("int32", (tokens, topk), want_expert)
+        for loss, bad in ((1.0, np.nan), (1.0, np.inf), (np.inf, 1.0), (np.nan, 1.0)):
+            dgate_values = np.ones(gate.shape, np.float32)
+            dgate_values[:, ::2] = bad                      # (every second token's)
+            dgate, dloss = new("float", (tokens, topk), dgate_values), new("float", (1,), np.float32(loss))
+            balance = new("float", (experts,), balance_values)
+            note("moe_route_grad", kind, experts, normalise, loss, bad)
+            rt.moe_route_grad(kind, dlogits.address, logits.address, expert.address, dgate.address, tokens, experts, topk,
+                              balance.address, dloss.address, normalise)
+            rt.sync()
+            got = dlogits.get()
+            assert (got[masked] == 0).all()
+            if loss == 1.0:
+                assert np.isfinite(got[:, 1::2]).all()
+
+
+@pytest.mark.parametrize("normalise", [True, False])
 def test_route_grad_by_differences(normalise):
     """The reference's gradient is the derivative of the reference's value, and the kernel's is the reference's."""
     rng = np.random.default_rng(6)
