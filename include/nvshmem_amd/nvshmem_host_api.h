@@ -347,7 +347,8 @@ NVSHMEMI_REPT_FOR_ALL_REDUCE_TYPES_AND_OPS(NVSHMEMI_DECL_TYPED_REDUCE_HOST)
  * other operands.  Each call returns 0 or an nvshmemx_status (nvshmemx_amd_last_error() has the text); nothing is enqueued by a
  * call that is refused.  No call allocates, and all of them can be captured into a graph; calls that can run at the same time
  * need workspaces of their own.  Workspaces are symmetric memory of the size that the functions named *_workspace give (bytes
- * per PE, 0 before nvshmem_init), aligned to 64 bytes, with nothing to initialise.  Arithmetic is in fp32 and results are
+ * per PE, 0 before nvshmem_init), aligned to 64 bytes, with nothing to initialise.  The size gets smaller with none of its
+ * arguments, so a workspace for the largest batch serves every smaller one.  Arithmetic is in fp32 and results are
  * rounded once; every sum has a fixed order, so that equal inputs give equal bits.
  *
  * <T>_embedding: out[t] = scale * row ids[t] of a table of `vocab` rows that is cut over the PEs: with R = ceil(vocab / npes),

@@ -75,11 +75,11 @@ __global__ __launch_bounds__(64) void embedding_kernel(T *__restrict__ out, cons
 // Parts are short where there are few wavefronts, long where there are many, as sums that go on cost a partial sum per part.  us
 // for sums | partial sums joined, parts of 8 / 32 / 64: 608 tokens of 515 fp32 13.5 / 19.7 / 29.0 | 4; 32768 of 7168 bf16 - / 330 / 330 | - /
 // 16.8 / 10.4; 8192 of 64 bf16 7.6 / 21.0 / - | 4.
-constexpr unsigned kLeastPart = 8, kMostPart = kLanes;
+constexpr unsigned kLeastPart = 8, kMostPart = kLanes, kPiece = 512, kPartPieces = 4096;
 unsigned part_of(uint64_t n, uint64_t dim) {
-    const uint64_t pieces = (dim + 511) / 512;
+    const uint64_t pieces = (dim + kPiece - 1) / kPiece;
     unsigned part = kLeastPart;
-    while (part < kMostPart && n * pieces / 4096 > part) part *= 2;
+    while (part < kMostPart && n * pieces / kPartPieces > part) part *= 2;
     return part;
 }
 
@@ -470,6 +470,16 @@ struct GradSpace {
         carry = hist + (passes ? kSortBlocks * kBins * sizeof(uint32_t) : 0);
         bytes = carry + (n + part - 1) / part * 2 * pitch * sizeof(float);
     }
+    // What a program allocates: enough for these sizes and for all that are no larger, of which some have shorter parts and so more partial
+    // sums (8 PEs, rows of 7168: 329 tokens take 18.9 MB, 1207 take 8.7).  Parts of P < kMostPart items are for n * pieces < kPartPieces *
+    // (P + 1), and rows have at most pieces * kPiece elements: partial sums of that many elements over P, and of one row for the last
+    // part.  That is the most where P is the least.
+    uint64_t space(uint64_t n) const {
+        const uint64_t short_parts = (n + kLeastPart - 1) / kLeastPart * pitch, long_parts = (n + kMostPart - 1) / kMostPart * pitch;
+        const uint64_t shorter = (uint64_t)kPartPieces * (kLeastPart + 1) * kPiece / kLeastPart + pitch;
+        const uint64_t most = long_parts > shorter ? long_parts : shorter;
+        return carry + (short_parts < most ? short_parts : most) * 2 * sizeof(float);
+    }
 };
 
 template <typename API>
@@ -552,7 +562,9 @@ NVSHMEMI_AMD_REPT_FOR_TOKEN_TYPES(NVSHMEM_AMD_EMBEDDING)
 
 size_t nvshmemx_amd_embedding_grad_workspace(size_t tokens, size_t vocab, size_t dim) {
     const int npes = Runtime::get().npes;
-    return npes < 1 ? 0 : tokens::GradSpace((uint64_t)tokens * npes, vocab, dim).bytes;
+    if (npes < 1) return 0;
+    const uint64_t n = (uint64_t)tokens * npes;
+    return tokens::GradSpace(n, vocab, dim).space(n);
 }
 
 }  // extern "C"

@@ -475,6 +475,12 @@ __global__ __launch_bounds__(kGradThreads) void route_grad_kernel(T *dlogits, co
 // front of it, from two blocks on).
 constexpr uint64_t kPlaceSpread = 1 << 17;
 unsigned place_rounds(uint64_t copies) { return copies <= kSortThreads ? 1 : copies < kPlaceSpread ? 2 : 8; }
+// The most blocks of a PE for as many copies or fewer: just below kPlaceSpread there are more than just above.
+uint64_t place_most_blocks(uint64_t copies) {
+    const uint64_t spread = ((copies < kPlaceSpread ? copies : kPlaceSpread) + 2 * kSortThreads - 1) / (2 * kSortThreads);
+    const uint64_t rounds_8 = (copies + 8 * kSortThreads - 1) / (8 * kSortThreads);
+    return spread > rounds_8 ? spread : rounds_8;
+}
 
 template <unsigned ROUNDS>
 __global__ __launch_bounds__(kSortThreads) void place_count_kernel(uint32_t *hist, const int32_t *expert, uint64_t stride,
@@ -594,12 +600,28 @@ struct RouteShape {
         const uint64_t steps = (all + groups - 1) / groups, each = (steps + most - 1) / most;
         per_block = groups * (unsigned)(each < 1 ? 1 : each < kMostSteps ? each : kMostSteps);
         blocks = tokens ? div_up(tokens, per_block) : 1;
+        lay_out(experts);
+    }
+    void lay_out(int experts) {
         const uint64_t table = ((uint64_t)blocks * experts * 4 + 63) / 64 * 64;
         hist = 0;
         psum = table;
         rows = 2 * table;
         ticket = rows + ((uint64_t)blocks * 8 + 63) / 64 * 64;
         bytes = ticket + 64 + (kMostExperts / kFinishExperts) * sizeof(double);
+    }
+    // What a program allocates: enough for these sizes and for all that are no larger, of which some have more blocks (8 PEs, 256 experts:
+    // 64 a PE for 1024 tokens, 32 for 8192).  A block takes at least one step of the smaller one, and there are at most kFewBlocks of
+    // them over all PEs, unless each takes all of its kMostSteps.
+    static uint64_t space(uint64_t tokens, int experts, int npes) {
+        const unsigned group = experts > 256 ? kLanes : 16;
+        const uint64_t least = kRouteThreads / group, full = kRouteMostThreads / group * kMostSteps;
+        const uint64_t one_step = (tokens + least - 1) / least, all_steps = (tokens + full - 1) / full, few = div_up(kFewBlocks, npes);
+        const uint64_t most = few > all_steps ? few : all_steps;
+        RouteShape shape(0, experts, npes, true);
+        if (tokens) shape.blocks = (unsigned)(one_step < most ? one_step : most);
+        shape.lay_out(experts);
+        return shape.bytes;
     }
 };
 
@@ -756,7 +778,7 @@ NVSHMEMI_AMD_REPT_FOR_TOKEN_TYPES(NVSHMEM_AMD_ROUTE)
 size_t nvshmemx_amd_moe_route_workspace(size_t tokens, int experts) {
     const int npes = Runtime::get().npes;
     if (npes < 1 || experts < 1 || experts > tokens::kMostExperts) return 0;
-    return tokens::RouteShape(tokens, experts, npes, true).bytes;  // (what a call without a loss takes is less)
+    return tokens::RouteShape::space(tokens, experts, npes);  // (what a call without a loss takes is less)
 }
 
 int nvshmemx_amd_moe_place_on_stream(int32_t *dest_pe, int64_t *dest_row, uint64_t *expected, int64_t *expert_row, void *workspace,
@@ -767,8 +789,7 @@ int nvshmemx_amd_moe_place_on_stream(int32_t *dest_pe, int64_t *dest_row, uint64
 }
 size_t nvshmemx_amd_moe_place_workspace(size_t tokens, int topk, int experts) {
     if (Runtime::get().npes < 1 || topk < 1 || experts < 1) return 0;
-    const uint64_t copies = (uint64_t)tokens * topk, block = (uint64_t)tokens::kSortThreads * tokens::place_rounds(copies);
-    return (copies + block - 1) / block * (uint64_t)experts * sizeof(uint32_t);
+    return tokens::place_most_blocks((uint64_t)tokens * topk) * (uint64_t)experts * sizeof(uint32_t);
 }
 
 }  // extern "C"

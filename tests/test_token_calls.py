@@ -200,3 +200,64 @@ rt.embedding_grad("half", p[0], p[1], p[2], p[3], 1 << 24, 1 << 30, 1)
 rt.embedding_grad("half", p[0], p[1], p[2], p[3], 1 << 24, (1 << 31) - 1, 1)
 assert len(launches()) > 15
 """)
+
+
+WORKSPACES = """
+import itertools
+from nvshmem_amd import Runtime
+rt = Runtime(npes=%d, symmetric_size=1 << 20)
+
+def never_falls(op, *grids):
+    size = {p: rt.workspace_bytes(op, *p) for p in itertools.product(*grids)}
+    for p, n in size.items():
+        for i, grid in enumerate(grids):
+            at = grid.index(p[i])
+            q = p[:i] + (grid[max(at - 1, 0)],) + p[i + 1:]
+            assert 0 <= size[q] <= n, "%%s of %%r takes %%d bytes, of %%r %%d" %% (op, q, size[q], p, n)
+
+def around(*values):
+    return sorted({v + d for v in values for d in (-1, 0, 1) if v + d >= 0})
+
+tokens = around(0, 2, 16, 64, 100, 128, 151, 329, 1024, 1207, 2048, 4096, 8192, 16129, 16384, 20000, 65536, 131072, 1 << 20,
+                1 << 22, (1 << 31) // rt.npes // 16 - 1)
+experts = around(2, 8, 64, 176, 256, 512, 1023)
+never_falls("moe_route", tokens, experts)
+never_falls("moe_place", tokens, list(range(1, 17)), experts)
+never_falls("embedding_grad", tokens, around(2, 512, 1 << 17, 1 << 18, (1 << 31) - 2), around(2, 8, 512, 1024, 1029, 7168, (1 << 24) - 1))
+"""
+
+
+@pytest.mark.parametrize("npes", [1, 2, 3, 8, 16, 64])
+def test_workspaces_do_not_get_smaller(recorded, npes):  # noqa: F811
+    """So that what a program allocates for its largest batch holds the smaller ones as well."""
+    recorded(WORKSPACES % npes)
+
+
+def test_a_workspace_of_the_largest_batch_serves_smaller_ones(recorded):  # noqa: F811
+    """Workspaces that end where the PE's slice does: a call that needed more would be refused."""
+    recorded("""
+from nvshmem_amd import Runtime
+rt = Runtime(npes=8, symmetric_size=1 << 30)
+p = [rt.malloc(96 << 20) for _ in range(8)]
+end = p[0] + rt.ptr(p[0], 1) - rt.ptr(p[0], 0) - 2048
+launches()
+
+def last(op, *sizes):
+    return (end - rt.workspace_bytes(op, *sizes)) // 64 * 64
+
+ws = last("moe_route", 8192, 256)
+for t in (1, 64, 65, 1000, 1024, 2048, 2049, 5000, 8192):
+    for e in (8, 64, 256):
+        rt.moe_route("bfloat16", p[0], p[1], p[2], ws, p[3], t, e, 4, loss=p[4], balance=p[5])
+ws = last("moe_route", 8192, 300)
+for t in (1, 256, 512, 513, 1024, 4096, 8192):
+    for e in (256, 257, 300):
+        rt.moe_route("bfloat16", p[0], p[1], p[2], ws, p[3], t, e, 4, loss=p[4], balance=p[5])
+ws = last("moe_place", 16384, 8, 256)
+for t in (100, 1000, 8192, 16128, 16129, 16383, 16384):
+    rt.moe_place(p[0], p[1], p[2], p[3], ws, p[4], p[5], t, 8, 256, 100)
+ws = last("embedding_grad", 1207, 10003, 4096)
+for t in (1, 100, 329, 600, 1206, 1207):
+    for d in (1, 512, 1029, 4096):
+        rt.embedding_grad("bfloat16", p[0], p[1], p[2], ws, t, 10003, d)
+""")
