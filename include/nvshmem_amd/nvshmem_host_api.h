@@ -355,8 +355,9 @@ NVSHMEMI_REPT_FOR_ALL_REDUCE_TYPES_AND_OPS(NVSHMEMI_DECL_TYPED_REDUCE_HOST)
  *   row v is row v % R of PE v / R's copy of `table` (R rows of dim elements on each).  An id outside [0, vocab) is padding and
  *   gives a row of zeros.
  * <T>_embedding_grad: the table's gradient, cut the same way: row v becomes scale * the sum of dout[t] over all tokens of all PEs
- *   with ids[t] = v, added up in the order of (PE, t), and zeros where no token names it.  Rows that a PE holds
- *   behind the vocabulary are left as they were.
+ *   with ids[t] = v, and zeros where no token names it.  The terms are taken in the order of (PE, t), in partial sums that end
+ *   where the batch's other ids have it: the same batch gives the same bits, in another one a row's sum may round differently.
+ *   Rows that a PE holds behind the vocabulary are left as they were.
  *
  * <T>_moe_route: for every token the `topk` (at most 16) largest of `experts` (at most 1024) logits, larger ones first, ties
  *   to the lowest expert.  A logit of -inf or NaN masks an expert out: where fewer are left than topk, expert is -1 and gate 0.

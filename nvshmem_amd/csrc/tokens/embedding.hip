@@ -1,8 +1,9 @@
 // Embedding lookup with scaling from a table that is cut by rows over the PEs, and the table's gradient.
 //
 //   out@p[t] = scale * table@(v / R)[v % R]           v = ids@p[t], R = ceil(vocab / npes) rows of the table on each PE
-//   dtable@(v / R)[v % R] = scale * sum dout@p[t]     over all (p, t) with ids@p[t] = v, in the order of (p, t)
+//   dtable@(v / R)[v % R] = scale * sum dout@p[t]     over all (p, t) with ids@p[t] = v
 //
+// The sum's terms are taken in the order of (p, t), but added up in partial sums whose ends follow from the ids of the whole batch.
 // An id outside [0, vocab) is padding: a row of zeros, no gradient.
 #include "counting_sort.hpp"
 #include "token_common.hpp"
