@@ -88,9 +88,9 @@ __global__ __launch_bounds__(64) void combine_sum_kernel(T *__restrict__ out, co
     }
 }
 
-// The sum of one copy.  TOKENS tokens for each row's lanes, as wavefronts of one piece of two rows start too slowly to keep memory busy.
-// us for 8 x t rows of d bf16, one token / four: 6000 of 512 23.4 / 17.4, 6000 of 2048 86.7 / 61.6 (6.4 TB/s), 4096 of 7168 146 / 144, 600 of
-// 512 (4800 wavefronts of one) 4.9 / 4.4, 64 of 512 (512) 2.8 / 3.3; 8000 of 64 (8000) 7.4 / 6.4, 2100 of 64 (2104) 3.9 / 4.3.
+// The sum of one copy.  kTokens tokens for each row's lanes, as wavefronts of one piece of two rows start too slowly to keep memory busy.
+// us for 8 x t rows of d bf16, one token / four: 6000 of 512 23.1 / 17.4, 6000 of 2048 85 / 63 (6.2 TB/s), 4096 of 7168 148 / 147, 600 of
+// 512 (4800 wavefronts of one) 5.0 / 4.5, 64 of 512 (512) 2.5 / 3.0; 8000 of 64 (8000) 7.2 / 6.4, 2100 of 64 (2104) 4.1 / 4.3.
 constexpr uint64_t kManyPieces = 4096;
 constexpr unsigned kTokens = 4;
 

@@ -16,11 +16,13 @@ namespace {
 // them and shares the wavefront with others (2^lanes_log lanes a row).  Reads a row of the table and writes one: bound by memory, and
 // for short rows by the rate at which wavefronts start, so there one has TOKENS tokens (or TOKENS for each row's lanes).
 // Where a wavefront has whole tokens, their ids are scalar loads and their rows scalar addresses.
-// us for 8 x 4096 rows of 7168 bf16 (0.47 GB written, about a third of that read from memory: 113 us are 5.5 TB/s): one chunk a lane
+// us, bf16, of 100003 rows by a Zipf distribution.  8 x 4096 rows of 7168 (0.47 GB written, 0.16 GB of distinct rows: 113 us are 5.6 TB/s of
+// what is needed; 0.29 GB are read, as every XCD's L2 fetches a popular row for itself, which makes 6.7 of what is moved): one chunk a lane
 // 141, two 120, four (of 14) 130, seven 116; two, written through to memory 113.  8 x 64 rows: 4.4, written through 4.0.
-// Rows of up to four pieces of 64 chunks are one wavefront's, against two pieces each: 8 x 20000 rows of 1152 73 / 141, of 2048 118 / 150.
-// One / four tokens a wavefront: 8 x 5970 rows of 512 bf16 (47760 wavefronts of one) 22.2 / 10.8, 8 x 600 (4800) 4.2 / 3.5, 8 x 64 (512)
-// 2.3 / 2.7; 8 x 5970 rows of 64 (5976) 5.0 / 3.8, 8 x 2100 (2104) 3.3 / 3.4.  Two tokens for rows of 900: 14.6 / 15.1, not taken.
+// Rows of up to four pieces of 64 chunks are one wavefront's, against two pieces each: 8 x 20000 rows of 1152 92 / 137, of 2048 177 / 167;
+// of 16000 rows, which the Infinity Cache holds, 71 / 139 and 127 / 150.
+// One / four tokens a wavefront: 8 x 5970 rows of 512 (47760 wavefronts of one) 22.0 / 12.2, 8 x 600 (4800) 4.0 / 3.5, 8 x 64 (512)
+// 2.3 / 2.7; 8 x 5970 rows of 64 (5976) 5.0 / 3.9, 8 x 2100 (2104) 3.3 / 3.4.  Two tokens for rows of 900: 14.6 / 15.1, not taken.
 constexpr uint64_t kManyWaves = 4096;
 template <typename T, int V, int TOKENS, int MODE>
 __global__ __launch_bounds__(64) void embedding_kernel(T *__restrict__ out, const T *__restrict__ table, const int64_t *__restrict__ ids,
@@ -218,7 +220,7 @@ struct SumArgs {
     const Item *sorted;
     float *carry;
     uint64_t stride;
-    unsigned tokens, n, part, parts, vocab, rows, dim, pitch, pieces, sum_blocks, zero_rows;
+    unsigned tokens, n, part, parts, vocab, rows, dim, pitch, pieces, sum_blocks;
     float scale;
 };
 
@@ -239,7 +241,9 @@ __device__ __forceinline__ void zero_fill(T *p, uint64_t elems) {
     if (lane < elems - tail) p[tail + lane] = (T)0.0f;
 }
 
-// Loads of a wavefront's rows that are in flight together (four 335, eight 330, sixteen 327 us where the kernel below says 319).
+// Loads of a wavefront's rows that are in flight together.  us of the kernel below with eight / sixteen: 8 x 4096 tokens of 7168 bf16, 100003
+// rows, 307 to 320 / 306, 8 x 6081 of 1088 62.0 to 63.4 / 60.6, 8 x 500 of 8000, 1000 rows, 33 / 32, 608 of 515 fp32 13.2 / 13.0: the spread
+// between processes and little more, and sixteen take 100 registers, eight 68.  (Four: 335 where eight took 330.)
 constexpr unsigned kAhead = 8;
 
 template <typename T>
@@ -311,12 +315,14 @@ __device__ __forceinline__ unsigned items_below(const Item *sorted, unsigned n, 
     return low;
 }
 
-// Zeros for those of zero_rows (at most 64) rows that no token names.
+// Zeros for those of kZeroRows (at most 64) rows that no token names.
+constexpr unsigned kZeroRows = kLanes;
+
 template <typename T>
 __device__ __forceinline__ void embedding_zero_rows(T *dtable, const SumArgs &a, unsigned group) {
     const unsigned lane = threadIdx.x;
-    const uint64_t base = (uint64_t)group * a.zero_rows;
-    const unsigned rows = a.vocab - base < a.zero_rows ? (unsigned)(a.vocab - base) : a.zero_rows;
+    const uint64_t base = (uint64_t)group * kZeroRows;
+    const unsigned rows = a.vocab - base < kZeroRows ? (unsigned)(a.vocab - base) : kZeroRows;
     const unsigned begin = items_below(a.sorted, a.n, base);
     const uint64_t key = begin + lane < a.n ? a.sorted[begin + lane].key : a.vocab;
     uint64_t named = 0;
@@ -349,8 +355,9 @@ __device__ __forceinline__ void embedding_zero_rows(T *dtable, const SumArgs &a,
 }
 
 // The first sum_blocks blocks add up, the others fill with zeros: bound by memory.  8 x 4096 tokens of 7168 bf16, 100003 rows (0.47 GB read,
-// 1.43 written): 319 us are 6.0 TB/s; zeros as streaming stores 330, written through 330, zeros first 331, in turn with the sums 349;
-// zeros for 16 rows a wavefront instead of 64 334.
+// 1.43 written): 307 to 320 us by process are 6.0 to 6.2 TB/s; where this form took 319, zeros as streaming stores 330, written through 330,
+// zeros first 331, in turn with the sums 349.  Zeros for 64 / 16 rows a wavefront: there 307 to 320 / 328, 8 x 500 tokens of 8000 and 1000
+// rows, of which 16 wavefronts are few, 33 / 20.
 template <typename T>
 __global__ __launch_bounds__(64) void embedding_sum_kernel(T *dtable, const T *dout, SumArgs a) {
     if (blockIdx.x < a.sum_blocks) {
@@ -532,8 +539,7 @@ int embedding_grad_on_stream(API *dtable, const API *dout, const int64_t *ids, v
     a.part = space.part, a.parts = div_up(n, space.part);
     const uint64_t items = (uint64_t)a.parts * a.pieces;
     a.sum_blocks = (unsigned)(items < (1u << 22) ? items : 1u << 22);
-    a.zero_rows = kLanes;
-    launch_kernel(embedding_sum_kernel<T>, dim3(a.sum_blocks + div_up(vocab, a.zero_rows)), dim3(kLanes), 0, stream, tab, src, a);
+    launch_kernel(embedding_sum_kernel<T>, dim3(a.sum_blocks + div_up(vocab, kZeroRows)), dim3(kLanes), 0, stream, tab, src, a);
     if (a.parts > 1)
         launch_kernel(embedding_join_kernel<T>, dim3(a.pieces, a.parts < 65535 ? a.parts : 65535), dim3(kJoinWaves * kLanes), 0, stream,
                       tab, a);
