@@ -261,3 +261,28 @@ for t in (1, 100, 329, 600, 1206, 1207):
     for d in (1, 512, 1029, 4096):
         rt.embedding_grad("bfloat16", p[0], p[1], p[2], ws, t, 10003, d)
 """)
+
+
+def test_the_most_tokens_that_the_tables_take(recorded):  # noqa: F811
+    """2^31 - 1 copies over all PEs; one token more is refused."""
+    recorded("""
+from nvshmem_amd import Runtime
+from nvshmem_amd.host import NvshmemError
+rt = Runtime(npes=4, symmetric_size=16 << 30)
+tokens = (1 << 29) - 1
+expert, dest_pe, dest_row = rt.malloc(tokens * 4), rt.malloc(tokens * 4), rt.malloc(tokens * 8)
+counts, expected, expert_row = (rt.malloc(1025 * 8) for _ in range(3))
+ws = rt.malloc(rt.workspace_bytes("moe_place", tokens, 1, 1024))
+launches()
+for experts in (4, 1024):
+    rt.moe_place(dest_pe, dest_row, expected, expert_row, ws, expert, counts, tokens, 1, experts, 1 << 40)
+    names = [l[0] for l in launches()]
+    assert len(names) == 2 and "place_count" in names[0] and "place_kernel" in names[1], names
+    try:
+        rt.moe_place(dest_pe, dest_row, expected, expert_row, ws, expert, counts, tokens + 1, 1, experts, 1 << 40)
+    except NvshmemError as e:
+        assert "at most 2^31 - 1 in all" in str(e), str(e)
+    else:
+        raise AssertionError("not refused")
+    assert not launches()
+""")
