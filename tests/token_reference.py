@@ -144,3 +144,54 @@ def embedding_grad(dtable, dout, ids, vocab, scale):
     np.add.at(size, ids[ok], abs(scale) * np.abs(dout[ok].astype(np.float64)))
     np.add.at(n, ids[ok], 1)
     return flat.reshape(dtable.shape), size.reshape(dtable.shape), n.reshape(npes, rows)
+
+
+# ---- the same for batches that are too large to go through token by token ----
+
+def route_many(logits, topk, normalise, scale):
+    """route(), over whole arrays."""
+    npes, tokens, experts = logits.shape
+    ok, p = live(logits), softmax(logits)
+    x = np.where(ok, logits.astype(np.float64), -np.inf)
+    order = np.argsort(-x, axis=2, kind="stable")[..., :topk]
+    chosen = np.take_along_axis(ok, order, 2)
+    if normalise:
+        l = np.take_along_axis(x, order, 2)
+        with np.errstate(invalid="ignore"):
+            w = np.where(chosen, np.exp(np.where(l == l[..., :1], 0.0, l - l[..., :1])), 0.0)
+        w /= np.maximum(w.sum(2, keepdims=True), 1.0)
+    else:
+        w = np.where(chosen, np.take_along_axis(p, order, 2), 0.0)
+    expert = np.where(chosen, order, -1).astype(np.int32)
+    counts = np.stack([np.bincount(e[e >= 0], minlength=experts) for e in expert]).astype(np.int64)
+    c, n = counts.sum(0).astype(np.float64), ok.any(-1).sum()
+    balance = experts * c / (c.sum() * n) if n else np.zeros(experts)
+    return expert, scale * w, counts, float((balance * p.sum((0, 1))).sum()), balance
+
+
+def route_grad_many(logits, expert, dgate, balance, dloss, normalise, scale):
+    """route_grad(), over whole arrays."""
+    ok, p, experts = live(logits), softmax(logits), logits.shape[2]
+    at = np.maximum(expert, 0).astype(np.int64)
+    chosen = (expert >= 0) & np.take_along_axis(ok, at, 2)
+    g = np.where(chosen, scale * dgate.astype(np.float64), 0.0)
+
+    def spread(values):             # from a token's chosen ones to all of its experts, and those behind the last for none
+        out = np.zeros(logits.shape[:2] + (experts + 1,))
+        np.put_along_axis(out, np.where(chosen, at, experts), np.where(chosen, values, 0.0), 2)
+        return out[..., :experts]
+
+    q = np.zeros((1, 1, 1)) if balance is None else (dloss[:, None] * balance)[:, None, :]
+    extra = extra_size = 0.0
+    if normalise:
+        l = np.where(chosen, np.take_along_axis(logits, at, 2).astype(np.float64), -np.inf)
+        m = l.max(2, keepdims=True)
+        with np.errstate(invalid="ignore"):
+            w = np.where(chosen, np.exp(np.where(l == m, 0.0, l - m)), 0.0)
+        w /= np.maximum(w.sum(2, keepdims=True), 1.0)
+        extra = spread(w * (g - (w * g).sum(2, keepdims=True)))
+        extra_size = spread(w * (np.abs(g) + (w * np.abs(g)).sum(2, keepdims=True)))
+    else:
+        q = q + spread(g)
+    d = p * (q - (q * p).sum(2, keepdims=True)) + extra
+    return d, p * (np.abs(q) + (np.abs(q) * p).sum(2, keepdims=True)) + extra_size
