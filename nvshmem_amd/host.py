@@ -216,7 +216,7 @@ class Runtime:
     # -- rows of tokens: in front of and behind the token shuffle ------------------------------
     def workspace_bytes(self, op, *sizes):
         """Bytes per PE of a call's workspace: ("embedding_grad", tokens, vocab, dim), ("moe_route", tokens, experts) or
-        ("moe_place", tokens, topk, experts)."""
+        ("moe_place", tokens, topk, experts).  No size makes it fall, so that of the largest batch serves smaller ones."""
         return getattr(self.lib, "nvshmemx_amd_%s_workspace" % op)(*sizes)
 
     def _tokens(self, name, *args, stream=None):
