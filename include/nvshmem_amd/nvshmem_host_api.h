@@ -377,6 +377,16 @@ NVSHMEMI_REPT_FOR_ALL_REDUCE_TYPES_AND_OPS(NVSHMEMI_DECL_TYPED_REDUCE_HOST)
  *   outside [0, npes) x [0, recv_cap_rows) adds nothing.  Without gates it is the gradient of the dispatch as well.
  * <T>_moe_combine_grad: drecv@dest_pe[dest_row] = gate * dout[t] and dgate = <dout[t], that row of recv>, 0 for a copy that was
  *   skipped.  Rows of drecv that no copy names are left as they were; drecv may be recv.  No two copies may name one row.
+ *
+ * <T>_moe_experts: the experts between dispatch and combine, a gated feed-forward block each, on the rows that moe_place gave them:
+ *   for the rows x = rows[expert_row[i] .. expert_row[i + 1]) of the i-th of this PE's experts (experts / npes of them),
+ *   [gate | up] = x w_in[i]^T, h = gate * sigmoid(gate) * up, out = h w_out[i]^T, with w_in[i] of 2 hidden x dim (the rows of gate, then
+ *   those of up) and w_out[i] of dim x hidden elements.  `rows`, `out` (and `pre`) have recv_cap_rows rows; those that no expert has are
+ *   neither read nor written.  What expert_row holds beyond [0, recv_cap_rows] is cut off.  `pre`, 2 hidden elements a row, gets
+ *   [gate | up] for moe_experts_grad, or is NULL.  h is rounded to T on its way from one product to the next.  dim and hidden are at most
+ *   65536, experts at most 1024 and the same number on every PE.
+ * <T>_moe_experts_grad: drows, dw_in and dw_out from dout, rows, weights and moe_experts' pre.  [dgate | dup] and h are rounded to T in
+ *   between.  An expert without rows gets weights' gradients of zeros; rows of drows that no expert has are left as they were.
  */
 #define NVSHMEMI_AMD_DECL_TOKENS(NAME, TYPE)                                                                              \
     NVSHMEMI_HOST_ONLY int nvshmemx_amd_##NAME##_embedding_on_stream(                                                     \
@@ -396,7 +406,15 @@ NVSHMEMI_REPT_FOR_ALL_REDUCE_TYPES_AND_OPS(NVSHMEMI_DECL_TYPED_REDUCE_HOST)
         const int64_t *dest_row, size_t tokens, int topk, size_t dim, nvshmemx_stream_t stream);                          \
     NVSHMEMI_HOST_ONLY int nvshmemx_amd_##NAME##_moe_combine_grad_on_stream(                                              \
         TYPE *drecv, float *dgate, const TYPE *dout, const TYPE *recv, size_t recv_cap_rows, const float *gate,           \
-        const int32_t *dest_pe, const int64_t *dest_row, size_t tokens, int topk, size_t dim, nvshmemx_stream_t stream);
+        const int32_t *dest_pe, const int64_t *dest_row, size_t tokens, int topk, size_t dim, nvshmemx_stream_t stream); \
+    NVSHMEMI_HOST_ONLY int nvshmemx_amd_##NAME##_moe_experts_on_stream(                                                  \
+        TYPE *out, TYPE *pre, void *workspace, const TYPE *rows, const TYPE *w_in, const TYPE *w_out,                    \
+        const int64_t *expert_row, size_t recv_cap_rows, int experts, size_t dim, size_t hidden,                         \
+        nvshmemx_stream_t stream);                                                                                       \
+    NVSHMEMI_HOST_ONLY int nvshmemx_amd_##NAME##_moe_experts_grad_on_stream(                                             \
+        TYPE *drows, TYPE *dw_in, TYPE *dw_out, void *workspace, const TYPE *dout, const TYPE *rows, const TYPE *pre,    \
+        const TYPE *w_in, const TYPE *w_out, const int64_t *expert_row, size_t recv_cap_rows, int experts, size_t dim,   \
+        size_t hidden, nvshmemx_stream_t stream);
 NVSHMEMI_AMD_REPT_FOR_TOKEN_TYPES(NVSHMEMI_AMD_DECL_TOKENS)
 #undef NVSHMEMI_AMD_DECL_TOKENS
 NVSHMEMI_HOST_ONLY int nvshmemx_amd_moe_place_on_stream(int32_t *dest_pe, int64_t *dest_row, uint64_t *expected,
@@ -406,6 +424,8 @@ NVSHMEMI_HOST_ONLY int nvshmemx_amd_moe_place_on_stream(int32_t *dest_pe, int64_
 NVSHMEMI_HOST_ONLY size_t nvshmemx_amd_embedding_grad_workspace(size_t tokens, size_t vocab, size_t dim);
 NVSHMEMI_HOST_ONLY size_t nvshmemx_amd_moe_route_workspace(size_t tokens, int experts);
 NVSHMEMI_HOST_ONLY size_t nvshmemx_amd_moe_place_workspace(size_t tokens, int topk, int experts);
+NVSHMEMI_HOST_ONLY size_t nvshmemx_amd_moe_experts_workspace(size_t recv_cap_rows, int experts, size_t dim, size_t hidden);
+NVSHMEMI_HOST_ONLY size_t nvshmemx_amd_moe_experts_grad_workspace(size_t recv_cap_rows, int experts, size_t dim, size_t hidden);
 
 /*
  * Cooperative launch of a kernel that uses the device API (reference

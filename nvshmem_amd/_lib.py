@@ -118,12 +118,16 @@ def load():
             "nvshmemx_amd_%s_moe_route_grad_on_stream" % t: (i32, [vp] * 6 + [sz, i32, i32, i32, f32, vp]),
             "nvshmemx_amd_%s_moe_combine_sum_on_stream" % t: (i32, [vp, vp, sz, vp, vp, vp, sz, i32, sz, vp]),
             "nvshmemx_amd_%s_moe_combine_grad_on_stream" % t: (i32, [vp, vp, vp, vp, sz, vp, vp, vp, sz, i32, sz, vp]),
+            "nvshmemx_amd_%s_moe_experts_on_stream" % t: (i32, [vp] * 7 + [sz, i32, sz, sz, vp]),
+            "nvshmemx_amd_%s_moe_experts_grad_on_stream" % t: (i32, [vp] * 10 + [sz, i32, sz, sz, vp]),
         })
     sig.update({
         "nvshmemx_amd_moe_place_on_stream": (i32, [vp] * 7 + [sz, i32, i32, sz, vp]),
         "nvshmemx_amd_embedding_grad_workspace": (sz, [sz, sz, sz]),
         "nvshmemx_amd_moe_route_workspace": (sz, [sz, i32]),
         "nvshmemx_amd_moe_place_workspace": (sz, [sz, i32, i32]),
+        "nvshmemx_amd_moe_experts_workspace": (sz, [sz, i32, sz, sz]),
+        "nvshmemx_amd_moe_experts_grad_workspace": (sz, [sz, i32, sz, sz]),
     })
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -266,7 +270,8 @@ def declared_symbols(header_paths=None):
             names.update({"nvshmem_%s_%s_reduce" % (t, op), "nvshmemx_%s_%s_reduce_on_stream" % (t, op),
                           "nvshmem_%s_%s_reducescatter" % (t, op),
                           "nvshmemx_%s_%s_reducescatter_on_stream" % (t, op)})
-    for op in ("embedding", "embedding_grad", "moe_route", "moe_route_grad", "moe_combine_sum", "moe_combine_grad"):
+    for op in ("embedding", "embedding_grad", "moe_route", "moe_route_grad", "moe_combine_sum", "moe_combine_grad", "moe_experts",
+               "moe_experts_grad"):
         names.update("nvshmemx_amd_%s_%s_on_stream" % (t, op) for t in TOKEN_TYPES)
     perf = open(os.path.join(INCLUDE, "nvshmem_perftest.h")).read()
     perf_names = set(re.findall(r"\bint\s+(nvshmem_perftest_\w+)\s*\(", perf))

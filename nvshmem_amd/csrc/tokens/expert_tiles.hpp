@@ -1,0 +1,433 @@
+// The experts' products in tiles of the matrix cores: D[m, n] = sum over k of A(m, k) B(n, k) for one expert at a time.
+//
+//            A(m, k)            B(n, k)               D
+//   kIn      rows[m][k]         w_in[n][k], two n     pre, h = silu(gate) * up    one tile has 128 columns of gate and the same of up
+//   kOut     h[m][k]            w_out[n][k]           out
+//   kDh      dout[m][k]         w_out[k][n]           dh, and from it with pre: dpre and h
+//   kDx      dpre[m][k]         w_in[k][n]            drows
+//   kDwIn    dpre[k][m]         rows[k][n]            dw_in                       k runs over the expert's rows
+//   kDwOut   dout[k][m]         h[k][n]               dw_out
+//
+// A tile of D is BM x 256, a block of eight wavefronts has one, each wavefront BM/2 x 64 of it in its accumulators (fp32).  A and B
+// pass through LDS in steps of 128 bytes of k, two steps in turn: while one is multiplied the other is on its way.
+#pragma once
+
+#include "token_common.hpp"
+
+namespace nvshmem_amd {
+namespace tokens {
+
+enum ExpertProduct { kIn, kOut, kDh, kDx, kDwIn, kDwOut };
+
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
+typedef unsigned v2u __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+
+#define NVSHMEM_AMD_LDS __attribute__((address_space(3)))
+
+// What a lane holds of 16 rows for the matrix cores: 16 bytes of consecutive k of row lane % 16, the (lane / 16)-th such piece of 64
+// bytes.  D has a's row lane / 16 * 4 + i and b's row lane % 16 in element i.
+template <typename T>
+struct Mma;
+template <>
+struct Mma<__bf16> {
+    typedef __bf16 vec __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ v4f step(v4u a, v4u b, v4f c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
+    }
+};
+template <>
+struct Mma<_Float16> {
+    typedef _Float16 vec __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ v4f step(v4u a, v4u b, v4f c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
+    }
+};
+template <>
+struct Mma<float> {
+    static __device__ __forceinline__ v4f step(v4u a, v4u b, v4f c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // (k in another order than it lies in memory, the same for both)
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
+        return c;
+    }
+};
+
+// One call's operands, PE 0's copies.  Which of them a product reads and writes is in the table above.
+template <typename T>
+struct ExpertArgs {
+    const int64_t *expert_row;
+    const T *rows, *w_in, *w_out, *dout, *pre_in;
+    T *out, *pre, *h, *dpre, *drows, *dw_in, *dw_out;
+    uint64_t stride, cap;
+    unsigned experts;  // of a PE
+    unsigned dim, hidden;
+    unsigned more_than;  // experts of at most so many rows are another kernel's
+};
+
+// Expert e's rows, whatever the table holds: never outside [0, cap).
+__device__ __forceinline__ void expert_range(const int64_t *expert_row, unsigned e, uint64_t cap, uint64_t &first, uint64_t &rows) {
+    const int64_t a = expert_row[e], b = expert_row[e + 1];
+    const uint64_t lo = a < 0 ? 0 : (uint64_t)a < cap ? (uint64_t)a : cap, hi = b < 0 ? 0 : (uint64_t)b < cap ? (uint64_t)b : cap;
+    first = lo;
+    rows = hi > lo ? hi - lo : 0;
+}
+
+__device__ __forceinline__ uint64_t scalar64(uint64_t x) {
+    return (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)x);
+}
+
+// The tiles of a PE's experts in a row: expert by expert, `columns` tiles wide and as many high as its rows need.  The lanes of every
+// wavefront look at 64 experts at a time.
+struct TileList {
+    const int64_t *expert_row;
+    uint64_t cap;
+    unsigned experts, tile_rows, columns, more_than;
+
+    __device__ __forceinline__ uint64_t scan(unsigned base, uint64_t &own) const {
+        const unsigned lane = threadIdx.x % kLanes, e = base + lane;
+        uint64_t first = 0, rows = 0;
+        if (e < experts) expert_range(expert_row, e, cap, first, rows);
+        own = rows > more_than ? (rows + tile_rows - 1) / tile_rows * columns : 0;
+        uint64_t sum = own;
+#pragma unroll
+        for (int d = 1; d < kLanes; d *= 2) {
+            const uint64_t up = __shfl_up(sum, d);
+            if (lane >= (unsigned)d) sum += up;
+        }
+        return sum;
+    }
+    __device__ __forceinline__ uint64_t total() const {
+        uint64_t all = 0, own;
+        for (unsigned base = 0; base < experts; base += kLanes) all += __shfl(scan(base, own), kLanes - 1);
+        return scalar64(all);
+    }
+    // The expert of tile t < total(), which becomes the number among that expert's.
+    __device__ __forceinline__ unsigned find(uint64_t &t) const {
+        for (unsigned base = 0;; base += kLanes) {
+            uint64_t own;
+            const uint64_t sum = scan(base, own);
+            const uint64_t here = __ballot(t < sum);
+            if (here) {
+                const int lane = __builtin_ctzll(here);
+                t = scalar64(t - (__shfl(sum, lane) - __shfl(own, lane)));
+                return base + __builtin_amdgcn_readfirstlane(lane);
+            }
+            t = scalar64(t - __shfl(sum, kLanes - 1));
+        }
+    }
+};
+
+// Where tile number i of `high` x `wide` tiles lies: columns of four tiles are gone through from top to bottom, so that the 32 tiles
+// that an XCD works on at a time share 8 strips of A and 4 of B in its L2.
+__device__ __forceinline__ void tile_place(unsigned i, unsigned high, unsigned wide, unsigned &m, unsigned &n) {
+    const unsigned per = high * 4, strip = i / per, left = wide - strip * 4, width = left < 4 ? left : 4, rest = i - strip * per;
+    m = rest / width;
+    n = strip * 4 + rest % width;
+}
+
+constexpr unsigned kTileThreads = 512, kTileWaves = kTileThreads / kLanes;
+constexpr unsigned kTileN = 256;
+constexpr unsigned kStepBytes = 128;        // of k
+constexpr unsigned kNowhere = 0x80000000u;  // an offset behind every buffer: reads zeros
+
+// One operand's way into LDS: R rows of a step.
+//   KM false: k is contiguous in memory.  LDS holds R rows of 128 bytes, chunk c of row r (16 bytes) at place c ^ (r & 7): what 16 lanes
+//     read together, one chunk of 16 rows, then lies in 8 different groups of banks.
+//   KM true: k is the row in memory.  LDS holds the step's k one after the other, R elements each, whose blocks of 16 elements change
+//     places with k (block b at b ^ swap(k)) for the same reason; ds_read_b64_tr_b16 turns them over on the way to the registers.
+// A wavefront moves 1 KiB at a time, which lands in LDS as it goes over its lanes; so the lanes pick the chunks that belong there.
+template <typename T, unsigned R, bool KM, bool DMA>
+struct TileSide {
+    static constexpr unsigned N = 16 / sizeof(T), kMoves = R / 64, kBytes = R * kStepBytes, kStepK = kStepBytes / sizeof(T);
+    unsigned off[kMoves];   // from the step's base, kNowhere where nothing is to be read whatever k is
+    unsigned along[kMoves]; // KM: the step's k of this lane's chunk; else its first k
+    unsigned width[kMoves]; // KM: elements of the chunk that are inside; else N
+    v4u held[DMA ? 1 : kMoves];
+
+    static __device__ __forceinline__ unsigned swap(unsigned k) { return sizeof(T) == 2 ? k & 7 : k >> 2 & 3; }
+
+    // `extent`: rows (KM: columns) that exist from the tile's first on; ld in elements.  Tile row r is row place(r) of the operand.
+    template <typename PLACE>
+    __device__ __forceinline__ void begin(unsigned wave, unsigned lane, unsigned extent, unsigned ld, PLACE place) {
+#pragma unroll
+        for (unsigned j = 0; j < kMoves; ++j) {
+            const unsigned move = wave * kMoves + j;
+            if (!KM) {
+                const unsigned r = move * 8 + lane / 8, c = lane % 8 ^ (r & 7), at = place(r);
+                along[j] = c * N;
+                width[j] = N;
+                off[j] = at < extent ? at * ld * (unsigned)sizeof(T) + c * 16 : kNowhere;
+            } else {
+                constexpr unsigned kPer = R * sizeof(T) / 16, kBlock = sizeof(T);  // chunks of a k, chunks of 16 elements
+                const unsigned chunk = move * kLanes + lane, k = chunk / kPer, c = chunk % kPer;
+                const unsigned from = ((c / kBlock) ^ swap(k)) * kBlock + c % kBlock, col = from * N;
+                along[j] = k;
+                width[j] = col < extent ? (extent - col < N ? extent - col : N) : 0;
+                off[j] = col < extent ? k * ld * (unsigned)sizeof(T) + from * 16 : kNowhere;
+            }
+        }
+    }
+    // Starts the way of a step whose first k is at `base` (per move) and that has `left` k.
+    template <typename BASE>
+    __device__ __forceinline__ void fetch(NVSHMEM_AMD_LDS char *lds, unsigned wave, unsigned left, BASE base) {
+#pragma unroll
+        for (unsigned j = 0; j < kMoves; ++j) {
+            const char *p = (const char *)base(j);
+            if (DMA) {
+                const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, 0x7fffffff, 0x00020000);
+                const unsigned o = along[j] < left ? off[j] : kNowhere;
+                // Not the builtin: behind that, the compiler waits for all loads on their way to LDS in front of every read of it.
+                // The step's barrier waits for them instead.  (Four wait states: the buffer's words may come from v_readfirstlane.)
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                             :
+                             : "s"((unsigned)(uintptr_t)(lds + (wave * kMoves + j) * 1024)), "v"(o), "s"(rsrc)
+                             : "memory");
+            } else {
+                const unsigned n = off[j] == kNowhere || along[j] >= left ? 0 : KM ? width[j] : (left - along[j] < N ? left - along[j] : N);
+                held[j] = v4u{};
+                if (n == N) held[j] = __builtin_bit_cast(v4u, chunk_load((const T *)(p + off[j])));
+                else if (n) held[j] = __builtin_bit_cast(v4u, chunk_load_part((const T *)(p + off[j]), n));
+            }
+        }
+    }
+    __device__ __forceinline__ void land(NVSHMEM_AMD_LDS char *lds, unsigned wave, unsigned lane) {
+        if (DMA) return;
+#pragma unroll
+        for (unsigned j = 0; j < kMoves; ++j) *(NVSHMEM_AMD_LDS v4u *)(lds + (wave * kMoves + j) * 1024 + lane * 16) = held[j];
+    }
+    // Rows [16 block, 16 block + 16) of 64 bytes of k, the s-th of a step's two, as the matrix cores take them.
+    static __device__ __forceinline__ v4u read(NVSHMEM_AMD_LDS const char *lds, unsigned block, unsigned s, unsigned lane) {
+        const unsigned r = lane % 16, g = lane / 16;
+        if (!KM) return *(NVSHMEM_AMD_LDS const v4u *)(lds + (block * 16 + r) * kStepBytes + (((s * 4 + g) ^ (r & 7)) * 16));
+        if (sizeof(T) == 2) {
+            const unsigned k = s * 32 + g * 8 + r / 4;  // (k & 7 is r / 4, and r / 4 + 4 four k further)
+            const char NVSHMEM_AMD_LDS *p = lds + k * R * 2 + ((block ^ (r / 4)) * 32) + r % 4 * 8;
+            const char NVSHMEM_AMD_LDS *q = lds + (k + 4) * R * 2 + ((block ^ (r / 4 + 4)) * 32) + r % 4 * 8;
+            const v2u lo = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((NVSHMEM_AMD_LDS v4s *)p));
+            const v2u hi = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((NVSHMEM_AMD_LDS v4s *)q));
+            return v4u{lo[0], lo[1], hi[0], hi[1]};
+        }
+        v4u v;
+#pragma unroll
+        for (unsigned i = 0; i < 4; ++i)
+            v[i] = *(NVSHMEM_AMD_LDS const unsigned *)(lds + (s * 16 + g * 4 + i) * R * 4 + ((block ^ g) * 64) + r * 4);
+        return v;
+    }
+};
+
+// Four consecutive elements of a row, of which `n` exist.
+template <typename T>
+__device__ __forceinline__ void store_four(T *p, v4f v, unsigned n) {
+    typedef T four __attribute__((ext_vector_type(4)));
+    typedef four four_unaligned __attribute__((aligned(sizeof(T))));
+    const four y = __builtin_convertvector(v, four);
+    if (n >= 4) {
+        *(four_unaligned *)p = y;
+    } else {
+#pragma unroll
+        for (unsigned i = 0; i < 3; ++i)
+            if (i < n) p[i] = y[i];
+    }
+}
+template <typename T>
+__device__ __forceinline__ v4f load_four(const T *p, unsigned n) {
+    typedef T four __attribute__((ext_vector_type(4)));
+    typedef four four_unaligned __attribute__((aligned(sizeof(T))));
+    if (n >= 4) return __builtin_convertvector(*(const four_unaligned *)p, v4f);
+    v4f v = {};
+#pragma unroll
+    for (unsigned i = 0; i < 3; ++i)
+        if (i < n) v[i] = (float)p[i];
+    return v;
+}
+// 1 / (1 + exp(-x)); exp overflows to an infinity, whose reciprocal is 0.
+__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+
+template <int OP>
+constexpr bool a_by_k() { return OP == kDwIn || OP == kDwOut; }
+template <int OP>
+constexpr bool b_by_k() { return OP != kIn && OP != kOut; }
+
+template <typename T, int OP, unsigned BM, bool DMA>
+__global__ __launch_bounds__(kTileThreads, 2) void expert_tile_kernel(const ExpertArgs<T> args) {
+    typedef TileSide<T, BM, a_by_k<OP>(), DMA> A;
+    typedef TileSide<T, kTileN, b_by_k<OP>(), DMA> B;
+    constexpr unsigned kMi = BM / 32, kNi = 4, kStepK = A::kStepK;
+    constexpr bool kWeights = OP == kDwIn || OP == kDwOut;  // D is a weight's gradient: k runs over rows
+    __shared__ __attribute__((aligned(1024))) char lds_a[2][A::kBytes];
+    __shared__ __attribute__((aligned(1024))) char lds_b[2][B::kBytes];
+    const unsigned pe = blockIdx.z, wave = wave_of_block(), lane = threadIdx.x % kLanes;
+    const int64_t *expert_row = copy_of(args.expert_row, pe, args.stride);
+    const unsigned dim = args.dim, hidden = args.hidden;
+    const unsigned n_all = OP == kIn || OP == kDh || OP == kDwOut ? hidden : dim, n_tile = OP == kIn ? kTileN / 2 : kTileN;
+    const unsigned wide = (n_all + n_tile - 1) / n_tile;
+    const unsigned m_all = OP == kDwIn ? 2 * hidden : dim;  // of a weight's gradient
+    const unsigned lda = OP == kIn || OP == kDh || OP == kDwOut ? dim : OP == kOut ? hidden : 2 * hidden;
+    const unsigned ldb = OP == kIn || OP == kDx || OP == kDwIn ? dim : hidden;
+    const TileList list = {expert_row, args.cap, args.experts, BM, wide, args.more_than};
+    const unsigned high_w = (m_all + BM - 1) / BM;
+    const uint64_t total = kWeights ? (uint64_t)args.experts * high_w * wide : list.total();
+    // Consecutive tiles go to one XCD (a block runs on XCD blockIdx.x % 8).
+    const uint64_t chunk = (total + 7) / 8;
+    for (uint64_t i = blockIdx.x / 8; i < chunk; i += gridDim.x / 8) {
+        uint64_t t = blockIdx.x % 8 * chunk + i;
+        if (t >= total) return;
+        unsigned e;
+        if (kWeights) {
+            e = (unsigned)(t / (high_w * wide));
+            t -= (uint64_t)e * high_w * wide;
+        } else {
+            e = list.find(t);
+        }
+        uint64_t first, rows;
+        expert_range(expert_row, e, args.cap, first, rows);
+        first = scalar64(first), rows = scalar64(rows);
+        unsigned tm, tn;
+        if (kWeights) {
+            tile_place((unsigned)t, high_w, wide, tm, tn);
+        } else {
+            tile_place((unsigned)t, (unsigned)((rows + BM - 1) / BM), wide, tm, tn);
+        }
+        const uint64_t m0 = (uint64_t)tm * BM;
+        const unsigned n0 = tn * n_tile;
+        const uint64_t k_all = kWeights ? rows : OP == kOut ? hidden : OP == kDx ? 2 * hidden : dim;
+        const uint64_t m_left = (kWeights ? m_all : rows) - m0;
+        const unsigned m_here = m_left < BM ? (unsigned)m_left : BM, n_here = n_all - n0 < n_tile ? n_all - n0 : n_tile;
+        // the operands' corners
+        const T *a = OP == kIn ? args.rows : OP == kOut ? args.h : OP == kDh || OP == kDwOut ? args.dout : args.dpre;
+        a = copy_of(a, pe, args.stride) + first * lda + (kWeights ? m0 : m0 * lda);
+        const T *b = OP == kIn || OP == kDx ? args.w_in : OP == kOut || OP == kDh ? args.w_out : OP == kDwIn ? args.rows : args.h;
+        b = copy_of(b, pe, args.stride);
+        if (OP == kIn || OP == kDx) b += (uint64_t)e * 2 * hidden * dim;
+        if (OP == kOut || OP == kDh) b += (uint64_t)e * hidden * dim;
+        if (kWeights) b += first * ldb;
+        b += b_by_k<OP>() ? (uint64_t)n0 : (uint64_t)n0 * ldb;
+        const T *b_up = b + (uint64_t)hidden * dim;  // kIn: the same columns of up
+        A side_a;
+        B side_b;
+        side_a.begin(wave, lane, m_here, lda, [](unsigned r) { return r; });
+        // kIn: a wavefront's 64 columns are 32 of gate and the same 32 of up
+        side_b.begin(wave, lane, n_here, ldb, [](unsigned r) { return OP == kIn ? r / 64 * 32 + r % 32 : r; });
+        const auto fetch = [&](unsigned buffer, uint64_t k) {
+            const unsigned left = k_all - k < kStepK ? (unsigned)(k_all - k) : kStepK;
+            side_a.fetch((NVSHMEM_AMD_LDS char *)lds_a[buffer], wave, left, [&](unsigned) { return a + (a_by_k<OP>() ? k * lda : k); });
+            side_b.fetch((NVSHMEM_AMD_LDS char *)lds_b[buffer], wave, left, [&](unsigned j) {
+                const bool up = OP == kIn && (wave * B::kMoves + j) * 8 % 64 >= 32;
+                return (up ? b_up : b) + (b_by_k<OP>() ? k * ldb : k);
+            });
+        };
+        v4f acc[kMi][kNi] = {};
+        const unsigned wm = wave / 4, wn = wave % 4;
+        if (k_all) fetch(0, 0);
+        unsigned buffer = 0;
+        for (uint64_t k = 0; k < k_all; k += kStepK, buffer ^= 1) {
+            side_a.land((NVSHMEM_AMD_LDS char *)lds_a[buffer], wave, lane);
+            side_b.land((NVSHMEM_AMD_LDS char *)lds_b[buffer], wave, lane);
+            asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // (a barrier alone does not wait for what is on its way to LDS)
+            __syncthreads();
+            if (k + kStepK < k_all) fetch(buffer ^ 1, k + kStepK);
+#pragma unroll
+            for (unsigned s = 0; s < 2; ++s) {
+                v4u fa[kMi], fb[kNi];
+#pragma unroll
+                for (unsigned ni = 0; ni < kNi; ++ni) fb[ni] = B::read((NVSHMEM_AMD_LDS const char *)lds_b[buffer], wn * 4 + ni, s, lane);
+#pragma unroll
+                for (unsigned mi = 0; mi < kMi; ++mi) fa[mi] = A::read((NVSHMEM_AMD_LDS const char *)lds_a[buffer], wm * kMi + mi, s, lane);
+#pragma unroll
+                for (unsigned mi = 0; mi < kMi; ++mi)
+#pragma unroll
+                    for (unsigned ni = 0; ni < kNi; ++ni) acc[mi][ni] = Mma<T>::step(fb[ni], fa[mi], acc[mi][ni]);
+            }
+        }
+        __syncthreads();  // (the next tile's first step overwrites a buffer that others may still read)
+        // A lane has four consecutive columns of row lane % 16 of each 16 x 16 piece.
+        const unsigned r = lane % 16, g = lane / 16;
+#pragma unroll
+        for (unsigned mi = 0; mi < kMi; ++mi) {
+            const unsigned m = (wm * kMi + mi) * 16 + r;
+            if (m >= m_here) continue;
+            const uint64_t row = kWeights ? m0 + m : first + m0 + m;
+            if (OP == kIn) {
+#pragma unroll
+                for (unsigned ni = 0; ni < 2; ++ni) {
+                    const unsigned c = wn * 32 + ni * 16 + g * 4;
+                    if (c >= n_here) continue;
+                    const v4f gate = acc[mi][ni], up = acc[mi][ni + 2];
+                    v4f h;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) h[i] = gate[i] * sigmoid(gate[i]) * up[i];
+                    store_four(copy_of(args.h, pe, args.stride) + row * hidden + n0 + c, h, n_here - c);
+                    if (args.pre) {
+                        T *pre = copy_of(args.pre, pe, args.stride) + row * 2 * hidden + n0 + c;
+                        store_four(pre, gate, n_here - c);
+                        store_four(pre + hidden, up, n_here - c);
+                    }
+                }
+                continue;
+            }
+#pragma unroll
+            for (unsigned ni = 0; ni < kNi; ++ni) {
+                const unsigned c = wn * 64 + ni * 16 + g * 4;
+                if (c >= n_here) continue;
+                const unsigned n = n0 + c, there = n_here - c;
+                if (OP == kDh) {
+                    const T *pre = copy_of(args.pre_in, pe, args.stride) + row * 2 * hidden + n;
+                    const v4f gate = load_four(pre, there), up = load_four(pre + hidden, there), dh = acc[mi][ni];
+                    v4f dgate, dup, h;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float s = sigmoid(gate[i]), silu = gate[i] * s;
+                        h[i] = silu * up[i];
+                        dup[i] = dh[i] * silu;
+                        dgate[i] = dh[i] * up[i] * (s + silu * (1.0f - s));
+                    }
+                    T *dpre = copy_of(args.dpre, pe, args.stride) + row * 2 * hidden + n;
+                    store_four(dpre, dgate, there);
+                    store_four(dpre + hidden, dup, there);
+                    store_four(copy_of(args.h, pe, args.stride) + row * hidden + n, h, there);
+                } else if (OP == kOut || OP == kDx) {
+                    store_four(copy_of(OP == kOut ? args.out : args.drows, pe, args.stride) + row * dim + n, acc[mi][ni], there);
+                } else if (OP == kDwIn) {
+                    store_four(copy_of(args.dw_in, pe, args.stride) + ((uint64_t)e * 2 * hidden + row) * dim + n, acc[mi][ni], there);
+                } else {
+                    store_four(copy_of(args.dw_out, pe, args.stride) + ((uint64_t)e * dim + row) * hidden + n, acc[mi][ni], there);
+                }
+            }
+        }
+    }
+}
+
+// Blocks of a launch over the tiles of one PE: a multiple of the XCDs.  A block takes another tile where there are more.
+inline dim3 tile_grid(uint64_t tiles, int npes) {
+    const uint64_t most = (uint64_t)1 << 16;
+    return dim3((unsigned)((tiles < most ? tiles : most) + 7) / 8 * 8, 1, npes);
+}
+
+template <typename T, int OP, unsigned BM, bool DMA>
+inline void launch_expert_tiles(const ExpertArgs<T> &args, int npes, hipStream_t stream) {
+    const uint64_t n_all = OP == kIn || OP == kDh || OP == kDwOut ? args.hidden : args.dim;
+    const uint64_t wide = div_up(n_all, OP == kIn ? kTileN / 2 : kTileN);
+    const uint64_t m_all = OP == kDwIn ? 2 * (uint64_t)args.hidden : args.dim;
+    // (of `cap` rows in all, every expert has at most one tile that is not full)
+    const uint64_t high = OP == kDwIn || OP == kDwOut ? args.experts * (uint64_t)div_up(m_all, BM)
+                                                      : args.cap / BM + (args.experts < args.cap ? args.experts : args.cap);
+    if (high * wide) launch_kernel((expert_tile_kernel<T, OP, BM, DMA>), tile_grid(high * wide, npes), dim3(kTileThreads), 0, stream, args);
+}
+
+// Products of one PE's experts may be at most so wide and high; their offsets inside a tile stay under 2^31 bytes.
+constexpr size_t kMostFeatures = 65536;
+
+inline int check_expert_sizes(Runtime &rt, const char *what, int experts, size_t dim, size_t hidden) {
+    NVSHMEM_AMD_REFUSE(experts < 1 || experts > 1024, "%s: %d experts, outside [1, 1024]", what, experts);
+    NVSHMEM_AMD_REFUSE(experts % rt.npes, "%s: %d experts on %d PEs, which have to have the same number each", what, experts, rt.npes);
+    NVSHMEM_AMD_REFUSE(dim < 1 || dim > kMostFeatures, "%s: rows of %zu elements, outside [1, %zu]", what, dim, kMostFeatures);
+    NVSHMEM_AMD_REFUSE(hidden < 1 || hidden > kMostFeatures, "%s: %zu hidden elements, outside [1, %zu]", what, hidden, kMostFeatures);
+    return 0;
+}
+inline bool aligned16(const void *p) { return (uintptr_t)p % 16 == 0; }
+inline uint64_t align_up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
+
+}  // namespace tokens
+}  // namespace nvshmem_amd

@@ -215,8 +215,9 @@ class Runtime:
 
     # -- rows of tokens: in front of and behind the token shuffle ------------------------------
     def workspace_bytes(self, op, *sizes):
-        """Bytes per PE of a call's workspace: ("embedding_grad", tokens, vocab, dim), ("moe_route", tokens, experts) or
-        ("moe_place", tokens, topk, experts).  No size makes it fall, so that of the largest batch serves smaller ones."""
+        """Bytes per PE of a call's workspace: ("embedding_grad", tokens, vocab, dim), ("moe_route", tokens, experts),
+        ("moe_place", tokens, topk, experts), ("moe_experts" or "moe_experts_grad", recv_cap_rows, experts, dim, hidden).
+        No size makes it fall, so that of the largest batch serves smaller ones."""
         return getattr(self.lib, "nvshmemx_amd_%s_workspace" % op)(*sizes)
 
     def _tokens(self, name, *args, stream=None):
@@ -252,6 +253,16 @@ class Runtime:
                          stream=None):
         self._tokens("nvshmemx_amd_%s_moe_combine_grad_on_stream" % type_name, drecv, dgate, dout, recv, recv_cap_rows, gate,
                      dest_pe, dest_row, tokens, topk, dim, stream=stream)
+
+    def moe_experts(self, type_name, out, workspace, rows, w_in, w_out, expert_row, recv_cap_rows, experts, dim, hidden, pre=None,
+                    stream=None):
+        self._tokens("nvshmemx_amd_%s_moe_experts_on_stream" % type_name, out, pre, workspace, rows, w_in, w_out, expert_row,
+                     recv_cap_rows, experts, dim, hidden, stream=stream)
+
+    def moe_experts_grad(self, type_name, drows, dw_in, dw_out, workspace, dout, rows, pre, w_in, w_out, expert_row, recv_cap_rows,
+                         experts, dim, hidden, stream=None):
+        self._tokens("nvshmemx_amd_%s_moe_experts_grad_on_stream" % type_name, drows, dw_in, dw_out, workspace, dout, rows, pre,
+                     w_in, w_out, expert_row, recv_cap_rows, experts, dim, hidden, stream=stream)
 
     def read_timeout(self, pe):
         rec = (C.c_uint64 * 4)()
