@@ -387,6 +387,14 @@ NVSHMEMI_REPT_FOR_ALL_REDUCE_TYPES_AND_OPS(NVSHMEMI_DECL_TYPED_REDUCE_HOST)
  *   65536, experts at most 1024 and the same number on every PE.
  * <T>_moe_experts_grad: drows, dw_in and dw_out from dout, rows, weights and moe_experts' pre.  [dgate | dup] and h are rounded to T in
  *   between.  An expert without rows gets weights' gradients of zeros; rows of drows that no expert has are left as they were.
+ * <T>_moe_experts_w4: moe_experts with weights of 4 bits.  Element k of a row of w_in (of 2 hidden rows of dim) and w_out (dim rows of hidden)
+ *   is (q - 8) * scale[row][k / group], q in the low half of byte k / 2 of the row for even k, in the high half for odd ones; rows are
+ *   ceil(elements / 2) bytes and ceil(elements / group) scales of T long.  group is a multiple of 32.  The weights' values are taken as they
+ *   are, without rounding to T.  A row of `rows` with an infinity gives NaN.  The workspace is moe_experts'.
+ * <T>_dropout: out[e] = residual[e] + (keep(e) ? rows[e] / (1 - P) : 0) over the tokens * dim elements of a PE (residual NULL: zeros), with P
+ *   the probability p, 0 <= p < 1, in steps of 2^-16.  keep follows from seed[0], seed[1] (the PE's own copy, e.g. a run's seed and a step's
+ *   number, read when the kernel runs), the PE and e, by Philox4x32-10, and from nothing else: the gradient is the same call on dout without
+ *   a residual.  What is dropped may be an infinity or a NaN.  out may be residual, or rows where there is no residual.
  */
 #define NVSHMEMI_AMD_DECL_TOKENS(NAME, TYPE)                                                                              \
     NVSHMEMI_HOST_ONLY int nvshmemx_amd_##NAME##_embedding_on_stream(                                                     \
@@ -414,7 +422,14 @@ NVSHMEMI_REPT_FOR_ALL_REDUCE_TYPES_AND_OPS(NVSHMEMI_DECL_TYPED_REDUCE_HOST)
     NVSHMEMI_HOST_ONLY int nvshmemx_amd_##NAME##_moe_experts_grad_on_stream(                                             \
         TYPE *drows, TYPE *dw_in, TYPE *dw_out, void *workspace, const TYPE *dout, const TYPE *rows, const TYPE *pre,    \
         const TYPE *w_in, const TYPE *w_out, const int64_t *expert_row, size_t recv_cap_rows, int experts, size_t dim,   \
-        size_t hidden, nvshmemx_stream_t stream);
+        size_t hidden, nvshmemx_stream_t stream);                                                                        \
+    NVSHMEMI_HOST_ONLY int nvshmemx_amd_##NAME##_moe_experts_w4_on_stream(                                               \
+        TYPE *out, void *workspace, const TYPE *rows, const uint8_t *w_in, const TYPE *w_in_scale, const uint8_t *w_out, \
+        const TYPE *w_out_scale, const int64_t *expert_row, size_t recv_cap_rows, int experts, size_t dim, size_t hidden,\
+        int group, nvshmemx_stream_t stream);                                                                            \
+    NVSHMEMI_HOST_ONLY int nvshmemx_amd_##NAME##_dropout_on_stream(                                                      \
+        TYPE *out, const TYPE *rows, const TYPE *residual, const uint64_t *seed, size_t tokens, size_t dim, float p,     \
+        nvshmemx_stream_t stream);
 NVSHMEMI_AMD_REPT_FOR_TOKEN_TYPES(NVSHMEMI_AMD_DECL_TOKENS)
 #undef NVSHMEMI_AMD_DECL_TOKENS
 NVSHMEMI_HOST_ONLY int nvshmemx_amd_moe_place_on_stream(int32_t *dest_pe, int64_t *dest_row, uint64_t *expected,

@@ -120,6 +120,8 @@ def load():
             "nvshmemx_amd_%s_moe_combine_grad_on_stream" % t: (i32, [vp, vp, vp, vp, sz, vp, vp, vp, sz, i32, sz, vp]),
             "nvshmemx_amd_%s_moe_experts_on_stream" % t: (i32, [vp] * 7 + [sz, i32, sz, sz, vp]),
             "nvshmemx_amd_%s_moe_experts_grad_on_stream" % t: (i32, [vp] * 10 + [sz, i32, sz, sz, vp]),
+            "nvshmemx_amd_%s_moe_experts_w4_on_stream" % t: (i32, [vp] * 8 + [sz, i32, sz, sz, i32, vp]),
+            "nvshmemx_amd_%s_dropout_on_stream" % t: (i32, [vp] * 4 + [sz, sz, f32, vp]),
         })
     sig.update({
         "nvshmemx_amd_moe_place_on_stream": (i32, [vp] * 7 + [sz, i32, i32, sz, vp]),
@@ -271,7 +273,7 @@ def declared_symbols(header_paths=None):
                           "nvshmem_%s_%s_reducescatter" % (t, op),
                           "nvshmemx_%s_%s_reducescatter_on_stream" % (t, op)})
     for op in ("embedding", "embedding_grad", "moe_route", "moe_route_grad", "moe_combine_sum", "moe_combine_grad", "moe_experts",
-               "moe_experts_grad"):
+               "moe_experts_grad", "moe_experts_w4", "dropout"):
         names.update("nvshmemx_amd_%s_%s_on_stream" % (t, op) for t in TOKEN_TYPES)
     perf = open(os.path.join(INCLUDE, "nvshmem_perftest.h")).read()
     perf_names = set(re.findall(r"\bint\s+(nvshmem_perftest_\w+)\s*\(", perf))

@@ -29,7 +29,7 @@ HIP_FLAGS = [
 
 RUNTIME_SOURCES = ["mspace.cpp", "runtime.hip", "teams.cpp", "collectives.hip", "host_rma.hip",
                    "tokens/embedding.hip", "tokens/combine.hip", "tokens/router.hip",
-                   "tokens/experts.hip", "tokens/experts_grad.hip"]
+                   "tokens/experts.hip", "tokens/experts_grad.hip", "tokens/experts_w4.hip", "tokens/dropout.hip"]
 PERFTEST_SOURCES = ["perftest/rma_kernels.hip", "perftest/copy_depth.hip", "perftest/coll_kernels.hip",
                     "perftest/moe_shuffle.hip", "perftest/moe_rowsignal.hip", "perftest/moe_rowsignal_full.hip",
                     "perftest/api_matrix.hip",

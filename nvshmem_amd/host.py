@@ -216,7 +216,8 @@ class Runtime:
     # -- rows of tokens: in front of and behind the token shuffle ------------------------------
     def workspace_bytes(self, op, *sizes):
         """Bytes per PE of a call's workspace: ("embedding_grad", tokens, vocab, dim), ("moe_route", tokens, experts),
-        ("moe_place", tokens, topk, experts), ("moe_experts" or "moe_experts_grad", recv_cap_rows, experts, dim, hidden).
+        ("moe_place", tokens, topk, experts), ("moe_experts" - moe_experts_w4's as well - or "moe_experts_grad",
+        recv_cap_rows, experts, dim, hidden).
         No size makes it fall, so that of the largest batch serves smaller ones."""
         return getattr(self.lib, "nvshmemx_amd_%s_workspace" % op)(*sizes)
 
@@ -263,6 +264,14 @@ class Runtime:
                          experts, dim, hidden, stream=None):
         self._tokens("nvshmemx_amd_%s_moe_experts_grad_on_stream" % type_name, drows, dw_in, dw_out, workspace, dout, rows, pre,
                      w_in, w_out, expert_row, recv_cap_rows, experts, dim, hidden, stream=stream)
+
+    def moe_experts_w4(self, type_name, out, workspace, rows, w_in, w_in_scale, w_out, w_out_scale, expert_row, recv_cap_rows,
+                       experts, dim, hidden, group, stream=None):
+        self._tokens("nvshmemx_amd_%s_moe_experts_w4_on_stream" % type_name, out, workspace, rows, w_in, w_in_scale, w_out,
+                     w_out_scale, expert_row, recv_cap_rows, experts, dim, hidden, group, stream=stream)
+
+    def dropout(self, type_name, out, rows, seed, tokens, dim, p, residual=None, stream=None):
+        self._tokens("nvshmemx_amd_%s_dropout_on_stream" % type_name, out, rows, residual, seed, tokens, dim, p, stream=stream)
 
     def read_timeout(self, pe):
         rec = (C.c_uint64 * 4)()
