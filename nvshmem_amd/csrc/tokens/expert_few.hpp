@@ -21,47 +21,41 @@ struct PlainWeights {
     unsigned ld, k_all;
     unsigned row[4];   // this lane's of each group, from its base
 
-    v4u w[4][2];
-    __device__ __forceinline__ void load(unsigned k, unsigned lane, bool whole) {
+    template <int MT>
+    struct Stage {
+        v4u w[4][2], x[MT][2];
+    };
+    template <bool WHOLE, int MT>
+    __device__ __forceinline__ void load(Stage<MT> &s, const T *const (&x)[MT], unsigned k, unsigned lane) const {
         const unsigned g = lane / 16;
 #pragma unroll
-        for (unsigned ni = 0; ni < 4; ++ni)
+        for (unsigned h = 0; h < 2; ++h) {
+            const unsigned at = k + (h * 4 + g) * kN, n = at < k_all ? (k_all - at < kN ? k_all - at : kN) : 0;
 #pragma unroll
-            for (unsigned s = 0; s < 2; ++s) {
-                const unsigned at = k + (s * 4 + g) * kN;
-                const T *p = base[ni / 2] + (uint64_t)row[ni] * ld + at;
-                if (whole) w[ni][s] = __builtin_bit_cast(v4u, chunk_load_stream(p));
-                else w[ni][s] = __builtin_bit_cast(v4u, part(p, at));
+            for (unsigned ni = 0; ni < 4; ++ni) {
+                const T *p = base[ni / 2] + row[ni] * ld + at;
+                s.w[ni][h] = WHOLE ? __builtin_bit_cast(v4u, chunk_load_stream(p)) : chunk_load_front(p, n);
             }
-    }
-    __device__ __forceinline__ typename Chunk<T>::vec part(const T *p, unsigned at) const {
-        return chunk_load_part(p, at < k_all ? (k_all - at < kN ? k_all - at : kN) : 0);
+#pragma unroll
+            for (int mi = 0; mi < MT; ++mi) s.x[mi][h] = WHOLE ? __builtin_bit_cast(v4u, chunk_load(x[mi] + at)) : chunk_load_front(x[mi] + at, n);
+        }
     }
     template <int MT>
-    __device__ __forceinline__ void multiply(const T *const (&x)[MT], unsigned k, unsigned lane, bool whole, v4f (&acc)[MT][4]) const {
-        const unsigned g = lane / 16;
-        v4u a[MT][2];
+    __device__ __forceinline__ void multiply(const Stage<MT> &s, v4f (&acc)[MT][4]) const {
 #pragma unroll
-        for (int mi = 0; mi < MT; ++mi)
-#pragma unroll
-            for (unsigned s = 0; s < 2; ++s) {
-                const unsigned at = k + (s * 4 + g) * kN;
-                if (whole) a[mi][s] = __builtin_bit_cast(v4u, chunk_load(x[mi] + at));
-                else a[mi][s] = __builtin_bit_cast(v4u, part(x[mi] + at, at));
-            }
-#pragma unroll
-        for (unsigned s = 0; s < 2; ++s)
+        for (unsigned h = 0; h < 2; ++h)
 #pragma unroll
             for (int mi = 0; mi < MT; ++mi)
 #pragma unroll
-                for (unsigned ni = 0; ni < 4; ++ni) acc[mi][ni] = Mma<T>::step(a[mi][s], w[ni][s], acc[mi][ni]);
+                for (unsigned ni = 0; ni < 4; ++ni) acc[mi][ni] = Mma<T>::step(s.x[mi][h], s.w[ni][h], acc[mi][ni]);
     }
 };
 
-// One block has 64 rows of one expert's weights; its four wavefronts take steps of k in turn and their sums are added up in their order.
+// One block has 64 rows of one expert's weights; its four wavefronts take steps of k in turn, each with the loads of its next step on
+// their way while it multiplies, and their sums are added up in their order.
 // D = x w^T: element i of a lane is row lane / 16 * 4 + i of x, column lane % 16.
 template <typename W, typename T, int MT>
-__device__ __forceinline__ void few_rows_sum(W &weights, const T *x, unsigned ldx, unsigned rows, float (*part)[MT * 16][kFewColumns + 4]) {
+__device__ __forceinline__ void few_rows_sum(const W &weights, const T *x, unsigned ldx, unsigned rows, float (*part)[MT * 16][kFewColumns + 4]) {
     const unsigned wave = wave_of_block(), lane = threadIdx.x % kLanes;
     const T *from[MT];
 #pragma unroll
@@ -71,13 +65,18 @@ __device__ __forceinline__ void few_rows_sum(W &weights, const T *x, unsigned ld
     }
     v4f acc[MT][4] = {};
     const unsigned whole = weights.k_all / W::kStepK;
-    for (unsigned i = wave; i < whole; i += kFewWaves) {
-        weights.load(i * W::kStepK, lane, true);
-        weights.template multiply<MT>(from, i * W::kStepK, lane, true, acc);
+    typename W::template Stage<MT> even, odd;
+    if (wave < whole) weights.template load<true>(even, from, wave * W::kStepK, lane);
+    for (unsigned i = wave; i < whole; i += 2 * kFewWaves) {
+        if (i + kFewWaves < whole) weights.template load<true>(odd, from, (i + kFewWaves) * W::kStepK, lane);
+        weights.multiply(even, acc);
+        if (i + kFewWaves >= whole) break;
+        if (i + 2 * kFewWaves < whole) weights.template load<true>(even, from, (i + 2 * kFewWaves) * W::kStepK, lane);
+        weights.multiply(odd, acc);
     }
     if (weights.k_all % W::kStepK && wave == whole % kFewWaves) {
-        weights.load(whole * W::kStepK, lane, false);
-        weights.template multiply<MT>(from, whole * W::kStepK, lane, false, acc);
+        weights.template load<false>(even, from, whole * W::kStepK, lane);
+        weights.multiply(even, acc);
     }
 #pragma unroll
     for (int mi = 0; mi < MT; ++mi)

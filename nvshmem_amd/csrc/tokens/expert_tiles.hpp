@@ -54,6 +54,20 @@ struct Mma<float> {
     }
 };
 
+// The first n (at most N) elements at p, and zeros behind them.  All of a chunk is read: no operand ends less than
+// NVSHMEMI_AMD_INTERNAL_BYTES in front of its PE's slice, so that what lies behind it can be read, whatever it is.
+template <typename T>
+__device__ __forceinline__ v4u chunk_load_front(const T *p, unsigned n) {
+    const v4u v = __builtin_bit_cast(v4u, chunk_load(p));
+    v4u mask;
+#pragma unroll
+    for (unsigned i = 0; i < 4; ++i) {
+        const int bytes = (int)(n * sizeof(T)) - (int)i * 4;  // of this word
+        mask[i] = bytes >= 4 ? ~0u : bytes <= 0 ? 0u : (1u << bytes * 8) - 1;
+    }
+    return v & mask;
+}
+
 // One call's operands, PE 0's copies.  Which of them a product reads and writes is in the table above.
 template <typename T>
 struct ExpertArgs {
@@ -138,9 +152,9 @@ constexpr unsigned kNowhere = 0x80000000u;  // an offset behind every buffer: re
 //   KM true: k is the row in memory.  LDS holds the step's k one after the other, R elements each, whose blocks of 16 elements change
 //     places with k (block b at b ^ swap(k)) for the same reason; ds_read_b64_tr_b16 turns them over on the way to the registers.
 // A wavefront moves 1 KiB at a time, which lands in LDS as it goes over its lanes; so the lanes pick the chunks that belong there.
-template <typename T, unsigned R, bool KM, bool DMA>
+template <typename T, unsigned R, bool KM, bool DMA, unsigned WAVES = kTileWaves>
 struct TileSide {
-    static constexpr unsigned N = 16 / sizeof(T), kMoves = R / 64, kBytes = R * kStepBytes, kStepK = kStepBytes / sizeof(T);
+    static constexpr unsigned N = 16 / sizeof(T), kMoves = R / 8 / WAVES, kBytes = R * kStepBytes, kStepK = kStepBytes / sizeof(T);
     unsigned off[kMoves];   // from the step's base, kNowhere where nothing is to be read whatever k is
     unsigned along[kMoves]; // KM: the step's k of this lane's chunk; else its first k
     unsigned width[kMoves]; // KM: elements of the chunk that are inside; else N
@@ -186,9 +200,7 @@ struct TileSide {
                              : "memory");
             } else {
                 const unsigned n = off[j] == kNowhere || along[j] >= left ? 0 : KM ? width[j] : (left - along[j] < N ? left - along[j] : N);
-                held[j] = v4u{};
-                if (n == N) held[j] = __builtin_bit_cast(v4u, chunk_load((const T *)(p + off[j])));
-                else if (n) held[j] = __builtin_bit_cast(v4u, chunk_load_part((const T *)(p + off[j]), n));
+                held[j] = chunk_load_front((const T *)(p + (n ? off[j] : 0)), n);
             }
         }
     }

@@ -14,13 +14,15 @@ struct W4Args {
     ExpertArgs<T> e;
     const unsigned char *w_in, *w_out;
     const T *s_in, *s_out;
-    unsigned group;
+    unsigned group, per_group;  // per_group: 2^31 / (group / 32), rounded up: k / group is k / 32 times that, over 2^31 (k is at most 2^16)
 };
 
 // ---- experts of few rows ----
 
-// The two halves of a word that an element of x and a weight become for the matrix cores.  A weight is 16 + q, whose bits are those of
-// 16 with q in the mantissa; what that is too much, 24 times the sum of x, goes into the sums first as a product with -24.
+// What x and a weight become for the matrix cores.  Of 16-bit elements, a weight is 16 + q, whose bits are those of 16 with q in the
+// mantissa; what that is too much, 24 times the sum of x, goes into the sums first as a product with -24.  The sums are in fp32, so that
+// what they lose by it is far below what the result is rounded to.  An fp32 element is the sum of three bf16 ones, of 8 bits of its mantissa
+// each, and weights are q - 8: nothing of it is lost in front of the sum.
 template <typename T>
 struct Nibble;
 template <>
@@ -34,13 +36,23 @@ struct Nibble<_Float16> {
     typedef _Float16 type;
 };
 template <>
-struct Nibble<float> : Nibble<__bf16> {};  // an fp32 number is the sum of three bf16 ones, of 8 bits of its mantissa each
+struct Nibble<float> : Nibble<__bf16> {};
 
 // Eight weights, k in the order 0 4 1 5 2 6 3 7.
 template <typename T>
 __device__ __forceinline__ v4u eight_weights(unsigned q) {
     constexpr unsigned s = Nibble<T>::kShift, mask = 0x000F000Fu << s;
     v4u v;
+    if (sizeof(T) == 4) {
+        const unsigned even = q & 0x0F0F0F0Fu, odd = q >> 4 & 0x0F0F0F0Fu;
+#pragma unroll
+        for (unsigned j = 0; j < 4; ++j) {
+            const unsigned from = j % 2 ? odd : even;
+            const float a = (float)(from >> j / 2 * 8 & 255) - 8.0f, b = (float)(from >> (j / 2 * 8 + 16) & 255) - 8.0f;
+            v[j] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);  // (small whole numbers: bf16 is their upper half)
+        }
+        return v;
+    }
 #pragma unroll
     for (unsigned j = 0; j < 4; ++j) {
         const unsigned at = j * 4;
@@ -89,99 +101,206 @@ struct words<4> {
     typedef v4u type;
 };
 
-// A wavefront takes 64 rows and 32 * WORDS k at a time, all of one group: lane (r, g) has of each of four groups of 16 rows 4 * WORDS bytes,
-// 8 * WORDS consecutive k of row r.  WORDS is 4 where the group is a multiple of 128, else 2 or 1.
-template <typename T, unsigned WORDS>
-struct FourBitWeights {
-    static constexpr unsigned kStepK = 32 * WORDS, kParts = sizeof(T) == 4 ? 3 : 1;
-    typedef typename words<WORDS>::type raw;
-    typedef raw raw_unaligned __attribute__((aligned(1)));
-    typedef typename Nibble<T>::type M;
-    const unsigned char *base[2];
-    const T *scale[2];
-    unsigned row_bytes, row_scales, k_all, group;
-    unsigned row[4];
+// A block has 128 rows of one expert's weights, 32 a wavefront, and up to 32 rows of x.  It goes over k in chunks of 256: weights go to LDS as
+// they are, whole lines of memory (128 bytes of a row) at a time; x goes there in the order that the matrix cores take (fp32: as three
+// parts), and the rows' scales.  While a chunk is multiplied the next is on its way.
+// Within a chunk a step is 32 * WORDS k, all of one group: lane (r, g) has of each of two groups of 16 rows 4 * WORDS bytes, 8 * WORDS
+// consecutive k of row r.  WORDS is 4 where the group is a multiple of 128, else 2 or 1.
+constexpr unsigned kFewW4Columns = 128;
 
-    raw w[4];
-    float s[4];
-    __device__ __forceinline__ void load(unsigned k, unsigned lane, bool whole) {
-        const unsigned at = k + lane / 16 * 8 * WORDS;
+template <typename T, unsigned WORDS, bool DMA>
+struct FewFourBits {
+    typedef TileSide<unsigned char, kFewW4Columns, false, DMA, kFewWaves> Side;
+    static constexpr unsigned kChunk = 256, kParts = sizeof(T) == 4 ? 3 : 1, kStep = 32 * WORDS, kSteps = kChunk / kStep;
+    static constexpr unsigned kRowBytes = kChunk * 2;  // of x in LDS
+    typedef typename words<WORDS>::type raw;
+    typedef typename Nibble<T>::type M;
+    template <int MT>
+    struct Held {
+        static constexpr unsigned kPieces = MT * 16 * kChunk / 8 / kFewThreads;  // of eight elements of x, a thread's
+        v4u x[kPieces][8 / Chunk<T>::N];
+        T scale[kSteps / 2 ? kSteps / 2 : 1];  // two threads have a row's
+    };
+    Side side;
+    const unsigned char *w, *w_up;  // the block's first row
+    const T *scale;                 // this thread's row's
+    const T *x;
+    unsigned k_all, rows, per_group;
+
+    template <int MT>
+    __device__ __forceinline__ void fetch(Held<MT> &h, NVSHMEM_AMD_LDS char *lds_w, unsigned k, bool in) {
+        constexpr unsigned N = Chunk<T>::N, kPerRow = kChunk / 8;
+        const bool whole = k + kChunk <= k_all;
 #pragma unroll
-        for (unsigned ni = 0; ni < 4; ++ni) {
-            const unsigned char *p = base[ni / 2] + (uint64_t)row[ni] * row_bytes + at / 2;
-            if (whole) {
-                w[ni] = __builtin_nontemporal_load((const raw_unaligned *)p);
-            } else {
-                unsigned v[WORDS] = {};
-                const unsigned n = at < k_all ? (k_all - at + 1) / 2 : 0;
+        for (unsigned i = 0; i < Held<MT>::kPieces; ++i) {
+            const unsigned piece = i * kFewThreads + threadIdx.x, m = piece / kPerRow, at = k + piece % kPerRow * 8;
+            const T *p = x + (uint64_t)(m < rows ? m : rows - 1) * k_all + at;  // (the last row's products stand in for rows behind it)
 #pragma unroll
-                for (unsigned i = 0; i < 4 * WORDS; ++i)
-                    if (i < n) v[i / 4] |= (unsigned)p[i] << i % 4 * 8;
-                __builtin_memcpy(&w[ni], v, sizeof v);
-            }
-            s[ni] = (float)scale[ni / 2][(uint64_t)row[ni] * row_scales + k / group];
+            for (unsigned c = 0; c < 8 / N; ++c) h.x[i][c] = __builtin_bit_cast(v4u, chunk_load(p + c * N));
+            if (whole) continue;
+            const unsigned left = at < k_all ? k_all - at : 0;
+#pragma unroll
+            for (unsigned c = 0; c < 8 / N; ++c) h.x[i][c] = chunk_load_front(p + c * N, left > c * N ? left - c * N : 0);
         }
+#pragma unroll
+        for (unsigned j = 0; j < kSteps / 2; ++j) {
+            const unsigned at = k + (threadIdx.x / kFewW4Columns * (kSteps / 2) + j) * kStep;
+            h.scale[j] = scale[__umulhi((at < k_all ? at : k) / 16, per_group)];
+        }
+        const unsigned wave = wave_of_block(), left = (k_all - k + 1) / 2;
+        side.fetch(lds_w, wave, left < kStepBytes ? left : kStepBytes, [&](unsigned j) {
+            return (in && (wave * Side::kMoves + j) * 8 % 32 >= 16 ? w_up : w) + k / 2;
+        });
     }
     template <int MT>
-    __device__ __forceinline__ void multiply(const T *const (&x)[MT], unsigned k, unsigned lane, bool whole, v4f (&acc)[MT][4]) const {
-        const unsigned at = k + lane / 16 * 8 * WORDS;
+    __device__ __forceinline__ void land(const Held<MT> &h, NVSHMEM_AMD_LDS char *lds_x, NVSHMEM_AMD_LDS float *lds_s) const {
+        constexpr unsigned kPerRow = kChunk / 8;
+#pragma unroll
+        for (unsigned i = 0; i < Held<MT>::kPieces; ++i) {
+            const unsigned piece = i * kFewThreads + threadIdx.x, m = piece / kPerRow, c = piece % kPerRow;
+            v4u a[kParts];
+            if constexpr (sizeof(T) == 2) a[0] = reorder_eight(h.x[i][0]);
+            else split_eight(__builtin_bit_cast(v4f, h.x[i][0]), __builtin_bit_cast(v4f, h.x[i][1]), a);
+#pragma unroll
+            for (unsigned q = 0; q < kParts; ++q)
+                *(NVSHMEM_AMD_LDS v4u *)(lds_x + (q * MT * 16 + m) * kRowBytes + (c ^ (m & 7)) * 16) = a[q];
+        }
+#pragma unroll
+        for (unsigned j = 0; j < kSteps / 2; ++j)
+            lds_s[(threadIdx.x / kFewW4Columns * (kSteps / 2) + j) * kFewW4Columns + threadIdx.x % kFewW4Columns] = (float)h.scale[j];
+    }
+    // D = w x^T: element i of a lane is row lane / 16 * 4 + i of the weights' 16, column lane % 16: a row of x.
+    template <int MT>
+    __device__ __forceinline__ void multiply(unsigned j, NVSHMEM_AMD_LDS const char *lds_w, NVSHMEM_AMD_LDS const char *lds_x,
+                                             NVSHMEM_AMD_LDS const float *lds_s, unsigned wave, unsigned lane, v4f (&acc)[MT][2]) const {
+        const unsigned r = lane % 16, g = lane / 16, c = Nibble<T>::kMinus24;
         v4u a[MT][WORDS][kParts];
         v4f sum[MT] = {};
-        const unsigned c = Nibble<T>::kMinus24;
 #pragma unroll
         for (int mi = 0; mi < MT; ++mi)
 #pragma unroll
-            for (unsigned j = 0; j < WORDS; ++j) {
-                const T *p = x[mi] + at + j * 8;
-                const unsigned from = at + j * 8, n = whole ? 8 : from < k_all ? (k_all - from < 8 ? k_all - from : 8) : 0;
-                if constexpr (sizeof(T) == 2) {
-                    a[mi][j][0] = reorder_eight(__builtin_bit_cast(v4u, whole ? chunk_load(p) : chunk_load_part(p, n)));
-                } else {
-                    const v4f lo = whole ? chunk_load(p) : chunk_load_part(p, n < 4 ? n : 4);
-                    const v4f hi = whole ? chunk_load(p + 4) : chunk_load_part(p + 4, n < 4 ? 0 : n - 4);
-                    split_eight(lo, hi, a[mi][j]);
+            for (unsigned i = 0; i < WORDS; ++i)
+#pragma unroll
+                for (unsigned q = 0; q < kParts; ++q) {
+                    const unsigned chunk = (j * 4 + g) * WORDS + i;
+                    a[mi][i][q] = *(NVSHMEM_AMD_LDS const v4u *)(lds_x + ((q * MT + mi) * 16 + r) * kRowBytes + (chunk ^ (r & 7)) * 16);
+                    if (sizeof(T) == 2) sum[mi] = Mma<M>::step(v4u{c, c, c, c}, a[mi][i][q], sum[mi]);
                 }
 #pragma unroll
-                for (unsigned q = 0; q < kParts; ++q) sum[mi] = Mma<M>::step(a[mi][j][q], v4u{c, c, c, c}, sum[mi]);
-            }
-#pragma unroll
-        for (unsigned ni = 0; ni < 4; ++ni) {
+        for (unsigned ni = 0; ni < 2; ++ni) {
+            const unsigned byte = (j * 4 + g) * 4 * WORDS, row = wave * 32 + ni * 16;
+            const raw held = *(NVSHMEM_AMD_LDS const raw *)(lds_w + (row + r) * kStepBytes + ((byte / 16) ^ (r & 7)) * 16 + byte % 16);
             v4f d[MT];
 #pragma unroll
             for (int mi = 0; mi < MT; ++mi) d[mi] = sum[mi];
 #pragma unroll
-            for (unsigned j = 0; j < WORDS; ++j) {
+            for (unsigned i = 0; i < WORDS; ++i) {
                 unsigned word;
-                if constexpr (WORDS == 1) word = w[ni];
-                else word = w[ni][j];
+                if constexpr (WORDS == 1) word = held;
+                else word = held[i];
                 const v4u b = eight_weights<T>(word);
 #pragma unroll
                 for (int mi = 0; mi < MT; ++mi)
 #pragma unroll
-                    for (unsigned q = 0; q < kParts; ++q) d[mi] = Mma<M>::step(a[mi][j][q], b, d[mi]);
+                    for (unsigned q = 0; q < kParts; ++q) d[mi] = Mma<M>::step(b, a[mi][i][q], d[mi]);
             }
+            const v4f s = *(NVSHMEM_AMD_LDS const v4f *)(lds_s + j * kFewW4Columns + row + g * 4);
 #pragma unroll
             for (int mi = 0; mi < MT; ++mi)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[mi][ni][i] = __builtin_fmaf(s[ni], d[mi][i], acc[mi][ni][i]);
+                for (int i = 0; i < 4; ++i) acc[mi][ni][i] = __builtin_fmaf(s[i], d[mi][i], acc[mi][ni][i]);
+        }
+    }
+    template <int MT>
+    __device__ __forceinline__ void sum(char *lds_w, char *lds_x, float *lds_s, bool in, v4f (&acc)[MT][2]) {
+        constexpr unsigned kXBytes = kParts * MT * 16 * kRowBytes, kScales = kSteps * kFewW4Columns;
+        const unsigned wave = wave_of_block(), lane = threadIdx.x % kLanes;
+        Held<MT> next;
+        fetch(next, (NVSHMEM_AMD_LDS char *)lds_w, 0, in);
+        unsigned buffer = 0;
+        for (unsigned k = 0; k < k_all; k += kChunk, buffer ^= 1) {
+            NVSHMEM_AMD_LDS char *lw = (NVSHMEM_AMD_LDS char *)lds_w + buffer * Side::kBytes;
+            NVSHMEM_AMD_LDS char *lx = (NVSHMEM_AMD_LDS char *)lds_x + buffer * kXBytes;
+            NVSHMEM_AMD_LDS float *ls = (NVSHMEM_AMD_LDS float *)lds_s + buffer * kScales;
+            side.land(lw, wave, lane);
+            land(next, lx, ls);
+            asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+            __syncthreads();  // (one a chunk: a buffer is written again two chunks later)
+            if (k + kChunk < k_all) fetch(next, (NVSHMEM_AMD_LDS char *)lds_w + (buffer ^ 1) * Side::kBytes, k + kChunk, in);
+#pragma unroll
+            for (unsigned j = 0; j < kSteps; ++j) {
+                multiply<MT>(j, lw, lx, ls, wave, lane, acc);
+                __builtin_amdgcn_sched_barrier(0);  // (the compiler would gather all steps' reads, in registers for all)
+            }
         }
     }
 };
 
-template <typename T, int OP, unsigned WORDS>
-__global__ __launch_bounds__(kFewThreads) void expert_few_w4_kernel(const W4Args<T> args) {
-    typedef FourBitWeights<T, WORDS> W;
-    few_rows_block<W, T, OP>(args.e, [&](W &w, unsigned pe, unsigned e, unsigned n0) {
-        const ExpertArgs<T> &a = args.e;
-        const unsigned n_all = OP == kIn ? a.hidden : a.dim, k_all = OP == kIn ? a.dim : a.hidden;
-        const uint64_t before = (uint64_t)e * (OP == kIn ? 2 * n_all : n_all) + n0;
-        w.k_all = k_all, w.group = args.group, w.row_bytes = (k_all + 1) / 2, w.row_scales = (k_all + args.group - 1) / args.group;
-        w.base[0] = copy_of(OP == kIn ? args.w_in : args.w_out, pe, a.stride) + before * w.row_bytes;
-        w.scale[0] = copy_of(OP == kIn ? args.s_in : args.s_out, pe, a.stride) + before * w.row_scales;
-        w.base[1] = OP == kIn ? w.base[0] + (uint64_t)n_all * w.row_bytes : w.base[0];
-        w.scale[1] = OP == kIn ? w.scale[0] + (uint64_t)n_all * w.row_scales : w.scale[0];
-        for (unsigned ni = 0; ni < 4; ++ni) w.row[ni] = few_rows_row<OP>(ni, threadIdx.x % kLanes, n_all - n0);
-    });
+template <typename T, int OP, int MT>
+__device__ __forceinline__ void few_w4_store(const ExpertArgs<T> &args, const v4f (&acc)[MT][2], unsigned pe, uint64_t first, unsigned rows,
+                                             unsigned n0) {
+    const unsigned wave = wave_of_block(), lane = threadIdx.x % kLanes, g = lane / 16;
+    const unsigned n_all = OP == kIn ? args.hidden : args.dim;
+#pragma unroll
+    for (int mi = 0; mi < MT; ++mi) {
+        const unsigned m = mi * 16 + lane % 16;
+        if (m >= rows) continue;
+        const uint64_t row = first + m;
+#pragma unroll
+        for (unsigned ni = 0; ni < (OP == kIn ? 1 : 2); ++ni) {
+            const unsigned n = n0 + wave * (OP == kIn ? 16 : 32) + ni * 16 + g * 4;
+            if (n >= n_all) continue;
+            if (OP == kIn) {
+                v4f h;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) h[i] = acc[mi][0][i] * sigmoid(acc[mi][0][i]) * acc[mi][1][i];
+                store_four(copy_of(args.h, pe, args.stride) + row * n_all + n, h, n_all - n);
+            } else {
+                store_four(copy_of(args.out, pe, args.stride) + row * n_all + n, acc[mi][ni], n_all - n);
+            }
+        }
+    }
+}
+
+// An expert of up to `more_than` rows has a block for each 32 of them, which reads the weights again.
+template <typename T, int OP, unsigned WORDS, bool DMA>
+__global__ __launch_bounds__(kFewThreads, sizeof(T) == 4 ? 1 : 2) void expert_few_w4_kernel(const W4Args<T> args4) {
+    typedef FewFourBits<T, WORDS, DMA> W;
+    constexpr unsigned kMost = sizeof(T) == 4 ? 16 : 32;  // rows of x at a time
+    __shared__ __attribute__((aligned(1024))) char lds_w[2 * W::Side::kBytes];
+    __shared__ __attribute__((aligned(16))) char lds_x[2 * W::kParts * kMost * W::kRowBytes];
+    __shared__ __attribute__((aligned(16))) float lds_s[2 * W::kSteps * kFewW4Columns];
+    const ExpertArgs<T> &args = args4.e;
+    const unsigned pe = blockIdx.z, lane = threadIdx.x % kLanes, part = blockIdx.y / args.experts, e = blockIdx.y % args.experts;
+    const unsigned n0 = blockIdx.x * (OP == kIn ? kFewW4Columns / 2 : kFewW4Columns);
+    uint64_t first, rows;
+    expert_range(copy_of(args.expert_row, pe, args.stride), e, args.cap, first, rows);
+    if (rows <= part * kMost || rows > args.more_than) return;
+    first = scalar64(first + part * kMost);
+    const unsigned mine = rows - part * kMost < kMost ? (unsigned)(rows - part * kMost) : kMost;
+    const unsigned n_all = OP == kIn ? args.hidden : args.dim, k_all = OP == kIn ? args.dim : args.hidden;
+    const unsigned row_bytes = (k_all + 1) / 2, n_here = n_all - n0;
+    const uint64_t before = (uint64_t)e * (OP == kIn ? 2 : 1) * n_all + n0;
+    // Row r of the block's weights, from its first: kIn's wavefronts have 16 of gate and the same 16 of up.
+    const auto place = [](unsigned r) { return OP == kIn ? r / 32 * 16 + r % 16 : r; };
+    W w;
+    w.side.begin(wave_of_block(), lane, n_here, row_bytes, place);
+    w.w = copy_of(OP == kIn ? args4.w_in : args4.w_out, pe, args.stride) + before * row_bytes;
+    w.w_up = w.w + (uint64_t)n_all * row_bytes;
+    const unsigned r = threadIdx.x % kFewW4Columns, at = place(r) < n_here ? place(r) : n_here - 1;
+    w.scale = copy_of(OP == kIn ? args4.s_in : args4.s_out, pe, args.stride) +
+              (before + (OP == kIn && r % 32 >= 16 ? n_all : 0) + at) * ((k_all + args4.group - 1) / args4.group);
+    w.x = copy_of(OP == kIn ? args.rows : (const T *)args.h, pe, args.stride) + first * k_all;
+    w.k_all = k_all, w.rows = mine, w.per_group = args4.per_group;
+    if (kMost == 16 || mine <= 16) {
+        v4f acc[1][2] = {};
+        w.template sum<1>(lds_w, lds_x, lds_s, OP == kIn, acc);
+        few_w4_store<T, OP, 1>(args, acc, pe, first, mine, n0);
+    } else if constexpr (kMost > 16) {
+        v4f acc[2][2] = {};
+        w.template sum<2>(lds_w, lds_x, lds_s, OP == kIn, acc);
+        few_w4_store<T, OP, 2>(args, acc, pe, first, mine, n0);
+    }
 }
 
 // ---- experts of more rows: tiles ----
@@ -202,17 +321,8 @@ struct FourBitSide {
     __device__ __forceinline__ void fetch(uint64_t k) {
         const unsigned at = (unsigned)k + threadIdx.x % 2 * kHalfK;
         const unsigned char *p = row + at / 2;
-        const unsigned n = at < k_all ? (k_all - at + 1) / 2 : 0;
-        if (n >= kHalfK / 2) {
-            held = *(const raw_unaligned *)p;
-        } else {
-            unsigned v[kWords] = {};
-#pragma unroll
-            for (unsigned i = 0; i < 4 * kWords; ++i)
-                if (i < n) v[i / 4] |= (unsigned)p[i] << i % 4 * 8;
-            __builtin_memcpy(&held, v, sizeof v);
-        }
-        held_scale = n ? (float)scale[at / group] : 0.0f;
+        held = *(const raw_unaligned *)p;  // (behind the row's end: what lies there, times zeros of A)
+        held_scale = (float)scale[(at < k_all ? at : (unsigned)k) / group];
     }
     __device__ __forceinline__ void land(NVSHMEM_AMD_LDS char *lds, float *scales) const {
         const unsigned r = threadIdx.x / 2, half = threadIdx.x % 2;
@@ -343,13 +453,24 @@ __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_w4_kernel(const W
     }
 }
 
+// Experts of more rows are the tiles'.
+constexpr unsigned kW4FewRows = 64;
+
+template <typename T, int OP, bool DMA>
+void launch_few_w4(const W4Args<T> &args, int npes, hipStream_t stream) {
+    const uint64_t rows = args.e.cap < kW4FewRows ? args.e.cap : kW4FewRows;
+    const dim3 grid(div_up(OP == kIn ? args.e.hidden : args.e.dim, OP == kIn ? kFewW4Columns / 2 : kFewW4Columns),
+                    args.e.experts * div_up(rows, sizeof(T) == 4 ? 16 : 32), npes);
+    if (args.group % 128 == 0) launch_kernel((expert_few_w4_kernel<T, OP, 4, DMA>), grid, dim3(kFewThreads), 0, stream, args);
+    else if (args.group % 64 == 0) launch_kernel((expert_few_w4_kernel<T, OP, 2, DMA>), grid, dim3(kFewThreads), 0, stream, args);
+    else launch_kernel((expert_few_w4_kernel<T, OP, 1, DMA>), grid, dim3(kFewThreads), 0, stream, args);
+}
 template <typename T, int OP>
 void launch_w4(const W4Args<T> &args, bool whole, int npes, hipStream_t stream) {
-    const dim3 few = few_rows_grid<OP>(args.e, npes);
-    if (args.group % 128 == 0) launch_kernel((expert_few_w4_kernel<T, OP, 4>), few, dim3(kFewThreads), 0, stream, args);
-    else if (args.group % 64 == 0) launch_kernel((expert_few_w4_kernel<T, OP, 2>), few, dim3(kFewThreads), 0, stream, args);
-    else launch_kernel((expert_few_w4_kernel<T, OP, 1>), few, dim3(kFewThreads), 0, stream, args);
-    if (args.e.cap <= kFewRows) return;
+    const unsigned row_bytes = ((OP == kIn ? args.e.dim : args.e.hidden) + 1) / 2;
+    if (row_bytes % 16 == 0 && aligned16(OP == kIn ? args.w_in : args.w_out)) launch_few_w4<T, OP, true>(args, npes, stream);
+    else launch_few_w4<T, OP, false>(args, npes, stream);
+    if (args.e.cap <= kW4FewRows) return;
     const uint64_t wide = div_up(OP == kIn ? args.e.hidden : args.e.dim, OP == kIn ? kTileN / 2 : kTileN);
     const uint64_t tiles = (args.e.cap / kW4TileRows + (args.e.experts < args.e.cap ? args.e.experts : args.e.cap)) * wide;
     if (whole) launch_kernel((expert_tile_w4_kernel<T, OP, true>), tile_grid(tiles, npes), dim3(kTileThreads), 0, stream, args);
@@ -383,8 +504,9 @@ int experts_w4_on_stream(API *out, void *workspace, const API *rows, const uint8
     if (!ops.ok()) return NVSHMEMX_ERROR_INVALID_VALUE;
     if (cap == 0) return 0;
     args.group = (unsigned)group;
+    args.per_group = (unsigned)((((uint64_t)1 << 31) + group / 32 - 1) / (group / 32));
     a.stride = rt.heap_size, a.cap = cap, a.experts = (unsigned)mine, a.dim = (unsigned)dim, a.hidden = (unsigned)hidden;
-    a.more_than = kFewRows;
+    a.more_than = kW4FewRows;
     const bool whole = dim * sizeof(T) % 16 == 0 && hidden * sizeof(T) % 16 == 0 && aligned16(a.rows);
     launch_w4<T, kIn>(args, whole, rt.npes, stream);
     launch_w4<T, kOut>(args, whole, rt.npes, stream);
