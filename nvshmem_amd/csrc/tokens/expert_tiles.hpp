@@ -8,7 +8,7 @@
 //   kDwIn    dpre[k][m]         rows[k][n]            dw_in                       k runs over the expert's rows
 //   kDwOut   dout[k][m]         h[k][n]               dw_out
 //
-// A tile of D is BM x 256, a block of eight wavefronts has one, each wavefront BM/2 x 64 of it in its accumulators (fp32).  A and B
+// A tile of D is BM x BN, a block of eight wavefronts has one, each wavefront BM/2 x BN/4 of it in its accumulators (fp32).  A and B
 // pass through LDS in steps of 128 bytes of k, two steps in turn: while one is multiplied the other is on its way.
 #pragma once
 
@@ -75,7 +75,7 @@ struct ExpertArgs {
     const T *rows, *w_in, *w_out, *dout, *pre_in;
     T *out, *pre, *h, *dpre, *drows, *dw_in, *dw_out;
     uint64_t stride, cap;
-    unsigned experts;  // of a PE
+    unsigned experts, npes;  // experts of a PE
     unsigned dim, hidden;
     unsigned more_than;  // experts of at most so many rows are another kernel's
 };
@@ -92,46 +92,63 @@ __device__ __forceinline__ uint64_t scalar64(uint64_t x) {
     return (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)x);
 }
 
-// The tiles of a PE's experts in a row: expert by expert, `columns` tiles wide and as many high as its rows need.  The lanes of every
-// wavefront look at 64 experts at a time.
-struct TileList {
-    const int64_t *expert_row;
-    uint64_t cap;
-    unsigned experts, tile_rows, columns, more_than;
+constexpr unsigned kTileThreads = 512, kTileWaves = kTileThreads / kLanes;
+constexpr unsigned kMostExperts = 1024;
 
-    __device__ __forceinline__ uint64_t scan(unsigned base, uint64_t &own) const {
-        const unsigned lane = threadIdx.x % kLanes, e = base + lane;
-        uint64_t first = 0, rows = 0;
-        if (e < experts) expert_range(expert_row, e, cap, first, rows);
-        own = rows > more_than ? (rows + tile_rows - 1) / tile_rows * columns : 0;
-        uint64_t sum = own;
+// The tiles of all PEs' experts in a row: expert by expert, `columns` tiles wide and as many high as its rows need.  first[e] is where
+// those of expert e (the e-th of all) begin.
+struct TileList {
+    unsigned first[kMostExperts + 1];
+    unsigned wave_sum[kTileWaves];
+
+    // By a whole block; two experts a thread.
+    __device__ __forceinline__ void make(const int64_t *expert_row, uint64_t stride, uint64_t cap, unsigned per_pe, unsigned npes, unsigned tile_rows,
+                                         unsigned columns, unsigned more_than) {
+        const unsigned wave = wave_of_block(), lane = threadIdx.x % kLanes, all = per_pe * npes;
+        unsigned own[2], sum = 0;
+#pragma unroll
+        for (unsigned i = 0; i < 2; ++i) {
+            const unsigned e = threadIdx.x * 2 + i;
+            uint64_t at = 0, rows = 0;
+            if (e < all) expert_range(copy_of(expert_row, e / per_pe, stride), e % per_pe, cap, at, rows);
+            own[i] = rows > more_than ? (unsigned)((rows + tile_rows - 1) / tile_rows) * columns : 0;
+            sum += own[i];
+        }
+        unsigned before = sum;
 #pragma unroll
         for (int d = 1; d < kLanes; d *= 2) {
-            const uint64_t up = __shfl_up(sum, d);
-            if (lane >= (unsigned)d) sum += up;
+            const unsigned up = __shfl_up(before, d);
+            if (lane >= (unsigned)d) before += up;
         }
-        return sum;
+        if (lane == kLanes - 1) wave_sum[wave] = before;
+        __syncthreads();
+        for (unsigned w = 0; w < wave; ++w) before += wave_sum[w];
+        before -= sum;
+        first[threadIdx.x * 2] = before;
+        first[threadIdx.x * 2 + 1] = before + own[0];
+        if (threadIdx.x == kTileThreads - 1) first[kMostExperts] = before + sum;
+        __syncthreads();
     }
-    __device__ __forceinline__ uint64_t total() const {
-        uint64_t all = 0, own;
-        for (unsigned base = 0; base < experts; base += kLanes) all += __shfl(scan(base, own), kLanes - 1);
-        return scalar64(all);
-    }
+    __device__ __forceinline__ unsigned total() const { return __builtin_amdgcn_readfirstlane(first[kMostExperts]); }
     // The expert of tile t < total(), which becomes the number among that expert's.
-    __device__ __forceinline__ unsigned find(uint64_t &t) const {
-        for (unsigned base = 0;; base += kLanes) {
-            uint64_t own;
-            const uint64_t sum = scan(base, own);
-            const uint64_t here = __ballot(t < sum);
-            if (here) {
-                const int lane = __builtin_ctzll(here);
-                t = scalar64(t - (__shfl(sum, lane) - __shfl(own, lane)));
-                return base + __builtin_amdgcn_readfirstlane(lane);
-            }
-            t = scalar64(t - __shfl(sum, kLanes - 1));
-        }
+    __device__ __forceinline__ unsigned find(unsigned &t) const {
+        unsigned lo = 0;  // first[lo] <= t < first[lo + 2 * step]
+#pragma unroll
+        for (unsigned step = kMostExperts / 2; step; step /= 2)
+            if (first[lo + step] <= t) lo += step;
+        lo = __builtin_amdgcn_readfirstlane(lo);
+        t = __builtin_amdgcn_readfirstlane(t - first[lo]);
+        return lo;
     }
 };
+
+// The tiles of a launch go to its blocks in turn, groups of up to 32 consecutive ones to an XCD (a block runs on XCD blockIdx.x % 8, which
+// has 32 compute units): what such a group shares is read into one L2.  Block `b` of `blocks` has tile number i, and so on.
+__device__ __forceinline__ unsigned tile_of_block(unsigned i, unsigned total) {
+    const unsigned slots = gridDim.x / 8, even = (total + 7) / 8, group = even < slots ? even : slots;
+    const unsigned slot = blockIdx.x / 8;
+    return slot < group ? (i * 8 + blockIdx.x % 8) * group + slot : ~0u;
+}
 
 // Where tile number i of `high` x `wide` tiles lies: columns of four tiles are gone through from top to bottom, so that the 32 tiles
 // that an XCD works on at a time share 8 strips of A and 4 of B in its L2.
@@ -141,8 +158,6 @@ __device__ __forceinline__ void tile_place(unsigned i, unsigned high, unsigned w
     n = strip * 4 + rest % width;
 }
 
-constexpr unsigned kTileThreads = 512, kTileWaves = kTileThreads / kLanes;
-constexpr unsigned kTileN = 256;
 constexpr unsigned kStepBytes = 128;        // of k
 constexpr unsigned kNowhere = 0x80000000u;  // an offset behind every buffer: reads zeros
 
@@ -262,47 +277,44 @@ constexpr bool a_by_k() { return OP == kDwIn || OP == kDwOut; }
 template <int OP>
 constexpr bool b_by_k() { return OP != kIn && OP != kOut; }
 
-template <typename T, int OP, unsigned BM, bool DMA>
+template <typename T, int OP, unsigned BM, unsigned BN, bool DMA>
 __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_kernel(const ExpertArgs<T> args) {
     typedef TileSide<T, BM, a_by_k<OP>(), DMA> A;
-    typedef TileSide<T, kTileN, b_by_k<OP>(), DMA> B;
-    constexpr unsigned kMi = BM / 32, kNi = 4, kStepK = A::kStepK;
+    typedef TileSide<T, BN, b_by_k<OP>(), DMA> B;
+    constexpr unsigned kMi = BM / 32, kNi = BN / 64, kStepK = A::kStepK;
     constexpr bool kWeights = OP == kDwIn || OP == kDwOut;  // D is a weight's gradient: k runs over rows
     __shared__ __attribute__((aligned(1024))) char lds_a[2][A::kBytes];
     __shared__ __attribute__((aligned(1024))) char lds_b[2][B::kBytes];
-    const unsigned pe = blockIdx.z, wave = wave_of_block(), lane = threadIdx.x % kLanes;
-    const int64_t *expert_row = copy_of(args.expert_row, pe, args.stride);
+    __shared__ TileList list;
+    const unsigned wave = wave_of_block(), lane = threadIdx.x % kLanes;
     const unsigned dim = args.dim, hidden = args.hidden;
-    const unsigned n_all = OP == kIn || OP == kDh || OP == kDwOut ? hidden : dim, n_tile = OP == kIn ? kTileN / 2 : kTileN;
+    const unsigned n_all = OP == kIn || OP == kDh || OP == kDwOut ? hidden : dim, n_tile = OP == kIn ? BN / 2 : BN;
     const unsigned wide = (n_all + n_tile - 1) / n_tile;
     const unsigned m_all = OP == kDwIn ? 2 * hidden : dim;  // of a weight's gradient
     const unsigned lda = OP == kIn || OP == kDh || OP == kDwOut ? dim : OP == kOut ? hidden : 2 * hidden;
     const unsigned ldb = OP == kIn || OP == kDx || OP == kDwIn ? dim : hidden;
-    const TileList list = {expert_row, args.cap, args.experts, BM, wide, args.more_than};
     const unsigned high_w = (m_all + BM - 1) / BM;
-    const uint64_t total = kWeights ? (uint64_t)args.experts * high_w * wide : list.total();
-    // Consecutive tiles go to one XCD (a block runs on XCD blockIdx.x % 8).
-    const uint64_t chunk = (total + 7) / 8;
-    for (uint64_t i = blockIdx.x / 8; i < chunk; i += gridDim.x / 8) {
-        uint64_t t = blockIdx.x % 8 * chunk + i;
+    if (!kWeights) list.make(args.expert_row, args.stride, args.cap, args.experts, args.npes, BM, wide, args.more_than);
+    const unsigned total = kWeights ? args.experts * args.npes * high_w * wide : list.total();
+    for (unsigned i = 0;; ++i) {
+        unsigned t = tile_of_block(i, total);
         if (t >= total) return;
         unsigned e;
         if (kWeights) {
-            e = (unsigned)(t / (high_w * wide));
-            t -= (uint64_t)e * high_w * wide;
+            e = t / (high_w * wide);
+            t -= e * high_w * wide;
         } else {
             e = list.find(t);
         }
+        const unsigned pe = e / args.experts;
+        e -= pe * args.experts;
         uint64_t first, rows;
-        expert_range(expert_row, e, args.cap, first, rows);
+        expert_range(copy_of(args.expert_row, pe, args.stride), e, args.cap, first, rows);
         first = scalar64(first), rows = scalar64(rows);
         unsigned tm, tn;
-        if (kWeights) {
-            tile_place((unsigned)t, high_w, wide, tm, tn);
-        } else {
-            tile_place((unsigned)t, (unsigned)((rows + BM - 1) / BM), wide, tm, tn);
-        }
+        tile_place(t, kWeights ? high_w : (unsigned)((rows + BM - 1) / BM), wide, tm, tn);
         const uint64_t m0 = (uint64_t)tm * BM;
+        if (!kWeights && m0 >= rows) continue;  // (a table whose ranges overlap many times over may count past 2^32)
         const unsigned n0 = tn * n_tile;
         const uint64_t k_all = kWeights ? rows : OP == kOut ? hidden : OP == kDx ? 2 * hidden : dim;
         const uint64_t m_left = (kWeights ? m_all : rows) - m0;
@@ -320,13 +332,13 @@ __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_kernel(const Expe
         A side_a;
         B side_b;
         side_a.begin(wave, lane, m_here, lda, [](unsigned r) { return r; });
-        // kIn: a wavefront's 64 columns are 32 of gate and the same 32 of up
-        side_b.begin(wave, lane, n_here, ldb, [](unsigned r) { return OP == kIn ? r / 64 * 32 + r % 32 : r; });
+        // kIn: the first half of a wavefront's columns are gate's, the second half the same of up
+        side_b.begin(wave, lane, n_here, ldb, [](unsigned r) { return OP == kIn ? r / (BN / 4) * (BN / 8) + r % (BN / 8) : r; });
         const auto fetch = [&](unsigned buffer, uint64_t k) {
             const unsigned left = k_all - k < kStepK ? (unsigned)(k_all - k) : kStepK;
             side_a.fetch((NVSHMEM_AMD_LDS char *)lds_a[buffer], wave, left, [&](unsigned) { return a + (a_by_k<OP>() ? k * lda : k); });
             side_b.fetch((NVSHMEM_AMD_LDS char *)lds_b[buffer], wave, left, [&](unsigned j) {
-                const bool up = OP == kIn && (wave * B::kMoves + j) * 8 % 64 >= 32;
+                const bool up = OP == kIn && (wave * B::kMoves + j) * 8 % (BN / 4) >= BN / 8;
                 return (up ? b_up : b) + (b_by_k<OP>() ? k * ldb : k);
             });
         };
@@ -344,7 +356,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_kernel(const Expe
             for (unsigned s = 0; s < 2; ++s) {
                 v4u fa[kMi], fb[kNi];
 #pragma unroll
-                for (unsigned ni = 0; ni < kNi; ++ni) fb[ni] = B::read((NVSHMEM_AMD_LDS const char *)lds_b[buffer], wn * 4 + ni, s, lane);
+                for (unsigned ni = 0; ni < kNi; ++ni) fb[ni] = B::read((NVSHMEM_AMD_LDS const char *)lds_b[buffer], wn * kNi + ni, s, lane);
 #pragma unroll
                 for (unsigned mi = 0; mi < kMi; ++mi) fa[mi] = A::read((NVSHMEM_AMD_LDS const char *)lds_a[buffer], wm * kMi + mi, s, lane);
 #pragma unroll
@@ -363,10 +375,10 @@ __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_kernel(const Expe
             const uint64_t row = kWeights ? m0 + m : first + m0 + m;
             if (OP == kIn) {
 #pragma unroll
-                for (unsigned ni = 0; ni < 2; ++ni) {
-                    const unsigned c = wn * 32 + ni * 16 + g * 4;
+                for (unsigned ni = 0; ni < kNi / 2; ++ni) {
+                    const unsigned c = wn * (BN / 8) + ni * 16 + g * 4;
                     if (c >= n_here) continue;
-                    const v4f gate = acc[mi][ni], up = acc[mi][ni + 2];
+                    const v4f gate = acc[mi][ni], up = acc[mi][ni + kNi / 2];
                     v4f h;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) h[i] = gate[i] * sigmoid(gate[i]) * up[i];
@@ -381,7 +393,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_kernel(const Expe
             }
 #pragma unroll
             for (unsigned ni = 0; ni < kNi; ++ni) {
-                const unsigned c = wn * 64 + ni * 16 + g * 4;
+                const unsigned c = wn * (BN / 4) + ni * 16 + g * 4;
                 if (c >= n_here) continue;
                 const unsigned n = n0 + c, there = n_here - c;
                 if (OP == kDh) {
@@ -411,28 +423,44 @@ __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_kernel(const Expe
     }
 }
 
-// Blocks of a launch over the tiles of one PE: a multiple of the XCDs.  A block takes another tile where there are more.
-inline dim3 tile_grid(uint64_t tiles, int npes) {
-    const uint64_t most = (uint64_t)1 << 16;
-    return dim3((unsigned)((tiles < most ? tiles : most) + 7) / 8 * 8, 1, npes);
+// One block a compute unit takes tiles as long as there are any; of the smaller ones, two have room.
+inline unsigned tile_blocks(uint64_t tiles, unsigned blocks_per_cu) {
+    const uint64_t most = 256 * blocks_per_cu;
+    return (unsigned)((tiles < most ? tiles : most) + 7) / 8 * 8;
 }
 
-template <typename T, int OP, unsigned BM, bool DMA>
-inline void launch_expert_tiles(const ExpertArgs<T> &args, int npes, hipStream_t stream) {
+// Tiles of a product, if each expert had as many rows as any could at most on average.
+template <typename T, int OP>
+inline uint64_t tiles_of(const ExpertArgs<T> &args, uint64_t bm, uint64_t bn) {
     const uint64_t n_all = OP == kIn || OP == kDh || OP == kDwOut ? args.hidden : args.dim;
-    const uint64_t wide = div_up(n_all, OP == kIn ? kTileN / 2 : kTileN);
-    const uint64_t m_all = OP == kDwIn ? 2 * (uint64_t)args.hidden : args.dim;
+    const uint64_t m_all = OP == kDwIn ? 2 * (uint64_t)args.hidden : OP == kDwOut ? args.dim : (args.cap + args.experts - 1) / args.experts;
+    return (uint64_t)args.experts * args.npes * ((m_all + bm - 1) / bm) * ((n_all * (OP == kIn ? 2 : 1) + bn - 1) / bn);
+}
+
+template <typename T, int OP, unsigned BM, unsigned BN, bool DMA>
+inline void launch_tiles_as(const ExpertArgs<T> &args, hipStream_t stream) {
     // (of `cap` rows in all, every expert has at most one tile that is not full)
-    const uint64_t high = OP == kDwIn || OP == kDwOut ? args.experts * (uint64_t)div_up(m_all, BM)
+    const uint64_t n_all = OP == kIn || OP == kDh || OP == kDwOut ? args.hidden : args.dim, wide = div_up(n_all, OP == kIn ? BN / 2 : BN);
+    const uint64_t high = OP == kDwIn || OP == kDwOut ? args.experts * (uint64_t)div_up(OP == kDwIn ? 2 * (uint64_t)args.hidden : args.dim, BM)
                                                       : args.cap / BM + (args.experts < args.cap ? args.experts : args.cap);
-    if (high * wide) launch_kernel((expert_tile_kernel<T, OP, BM, DMA>), tile_grid(high * wide, npes), dim3(kTileThreads), 0, stream, args);
+    const uint64_t tiles = high * wide * args.npes;
+    if (tiles) launch_kernel((expert_tile_kernel<T, OP, BM, BN, DMA>), dim3(tile_blocks(tiles, BM == 128 && BN == 128 ? 2 : 1)), dim3(kTileThreads), 0, stream, args);
+}
+template <typename T, int OP, bool DMA>
+inline void launch_expert_tiles(const ExpertArgs<T> &args, hipStream_t stream) {
+    // The time of a shape: as often as its tiles fill the compute units, times what one takes.
+    const auto cost = [&](uint64_t bm, uint64_t bn, uint64_t weight) { return (tiles_of<T, OP>(args, bm, bn) + 255) / 256 * bm * bn * weight; };
+    const uint64_t large = cost(256, 256, 8), medium = cost(128, 256, 9), small = cost(128, 128, 12);
+    if (large <= medium && large <= small) launch_tiles_as<T, OP, 256, 256, DMA>(args, stream);
+    else if (medium <= small) launch_tiles_as<T, OP, 128, 256, DMA>(args, stream);
+    else launch_tiles_as<T, OP, 128, 128, DMA>(args, stream);
 }
 
 // Products of one PE's experts may be at most so wide and high; their offsets inside a tile stay under 2^31 bytes.
 constexpr size_t kMostFeatures = 65536;
 
 inline int check_expert_sizes(Runtime &rt, const char *what, int experts, size_t dim, size_t hidden) {
-    NVSHMEM_AMD_REFUSE(experts < 1 || experts > 1024, "%s: %d experts, outside [1, 1024]", what, experts);
+    NVSHMEM_AMD_REFUSE(experts < 1 || experts > (int)kMostExperts, "%s: %d experts, outside [1, %u]", what, experts, kMostExperts);
     NVSHMEM_AMD_REFUSE(experts % rt.npes, "%s: %d experts on %d PEs, which have to have the same number each", what, experts, rt.npes);
     NVSHMEM_AMD_REFUSE(dim < 1 || dim > kMostFeatures, "%s: rows of %zu elements, outside [1, %zu]", what, dim, kMostFeatures);
     NVSHMEM_AMD_REFUSE(hidden < 1 || hidden > kMostFeatures, "%s: %zu hidden elements, outside [1, %zu]", what, hidden, kMostFeatures);

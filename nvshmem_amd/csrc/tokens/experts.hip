@@ -15,8 +15,8 @@ template <typename T, int OP>
 void launch_experts(const ExpertArgs<T> &args, bool whole, int npes, hipStream_t stream) {
     launch_kernel((expert_few_kernel<T, OP>), few_rows_grid<OP>(args, npes), dim3(kFewThreads), 0, stream, args);
     if (args.cap <= kFewRows) return;
-    if (whole) launch_expert_tiles<T, OP, 256, true>(args, npes, stream);
-    else launch_expert_tiles<T, OP, 256, false>(args, npes, stream);
+    if (whole) launch_expert_tiles<T, OP, true>(args, stream);
+    else launch_expert_tiles<T, OP, false>(args, stream);
 }
 
 template <typename API>
@@ -41,7 +41,7 @@ int experts_on_stream(API *out, API *pre, void *workspace, const API *rows, cons
     args.h = (T *)ops.out("workspace", (char *)workspace, cap * hidden * sizeof(T), 64);
     if (!ops.ok()) return NVSHMEMX_ERROR_INVALID_VALUE;
     if (cap == 0) return 0;
-    args.stride = rt.heap_size, args.cap = cap, args.experts = (unsigned)mine, args.dim = (unsigned)dim, args.hidden = (unsigned)hidden;
+    args.stride = rt.heap_size, args.cap = cap, args.experts = (unsigned)mine, args.npes = (unsigned)rt.npes, args.dim = (unsigned)dim, args.hidden = (unsigned)hidden;
     // (the slices' stride is a multiple of 2 MiB, so that every PE's copies are aligned like PE 0's)
     const bool whole = dim * sizeof(T) % 16 == 0 && hidden * sizeof(T) % 16 == 0 && aligned16(args.rows) && aligned16(args.w_in) &&
                        aligned16(args.w_out);

@@ -41,19 +41,19 @@ int experts_grad_on_stream(API *drows, API *dw_in, API *dw_out, void *workspace,
     char *ws = ops.out("workspace", (char *)workspace, cap ? h_at + cap * hidden * sizeof(T) : 0, 64);
     if (!ops.ok()) return NVSHMEMX_ERROR_INVALID_VALUE;
     args.dpre = (T *)ws, args.h = (T *)(ws + h_at);
-    args.stride = rt.heap_size, args.cap = cap, args.experts = (unsigned)mine, args.dim = (unsigned)dim, args.hidden = (unsigned)hidden;
+    args.stride = rt.heap_size, args.cap = cap, args.experts = (unsigned)mine, args.npes = (unsigned)rt.npes, args.dim = (unsigned)dim, args.hidden = (unsigned)hidden;
     const bool whole = dim * sizeof(T) % 16 == 0 && hidden * sizeof(T) % 16 == 0 && aligned16(args.rows) && aligned16(args.w_in) &&
                        aligned16(args.w_out) && aligned16(args.dout);
     if (whole) {
-        launch_expert_tiles<T, kDh, 256, true>(args, rt.npes, stream);
-        launch_expert_tiles<T, kDx, 256, true>(args, rt.npes, stream);
-        launch_expert_tiles<T, kDwIn, 256, true>(args, rt.npes, stream);
-        launch_expert_tiles<T, kDwOut, 256, true>(args, rt.npes, stream);
+        launch_expert_tiles<T, kDh, true>(args, stream);
+        launch_expert_tiles<T, kDx, true>(args, stream);
+        launch_expert_tiles<T, kDwIn, true>(args, stream);
+        launch_expert_tiles<T, kDwOut, true>(args, stream);
     } else {
-        launch_expert_tiles<T, kDh, 256, false>(args, rt.npes, stream);
-        launch_expert_tiles<T, kDx, 256, false>(args, rt.npes, stream);
-        launch_expert_tiles<T, kDwIn, 256, false>(args, rt.npes, stream);
-        launch_expert_tiles<T, kDwOut, 256, false>(args, rt.npes, stream);
+        launch_expert_tiles<T, kDh, false>(args, stream);
+        launch_expert_tiles<T, kDx, false>(args, stream);
+        launch_expert_tiles<T, kDwIn, false>(args, stream);
+        launch_expert_tiles<T, kDwOut, false>(args, stream);
     }
     return launched("moe_experts_grad");
 }

@@ -309,7 +309,7 @@ __global__ __launch_bounds__(kFewThreads, sizeof(T) == 4 ? 1 : 2) void expert_fe
 // reads them.  Their scales go beside them, one for each half of each row.
 template <typename T>
 struct FourBitSide {
-    static constexpr unsigned kStepK = kStepBytes / sizeof(T), kHalfK = kStepK / 2, kWords = kHalfK / 8;
+    static constexpr unsigned kTileN = 256, kStepK = kStepBytes / sizeof(T), kHalfK = kStepK / 2, kWords = kHalfK / 8;
     typedef typename words<kWords>::type raw;
     typedef raw raw_unaligned __attribute__((aligned(1)));
     const unsigned char *row;  // this thread's; where it has none, a row that exists
@@ -340,7 +340,7 @@ struct FourBitSide {
     }
 };
 
-constexpr unsigned kW4TileRows = 128;
+constexpr unsigned kW4TileRows = 128, kTileN = 256;
 
 template <typename T, int OP, bool DMA>
 __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_w4_kernel(const W4Args<T> args4) {
@@ -353,22 +353,25 @@ __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_w4_kernel(const W
     __shared__ __attribute__((aligned(1024))) char lds_b[2][B::kBytes];
     __shared__ __attribute__((aligned(16))) float lds_s[2][2 * kTileN];
     const ExpertArgs<T> &args = args4.e;
-    const unsigned pe = blockIdx.z, wave = wave_of_block(), lane = threadIdx.x % kLanes;
-    const int64_t *expert_row = copy_of(args.expert_row, pe, args.stride);
+    __shared__ TileList list;
+    const unsigned wave = wave_of_block(), lane = threadIdx.x % kLanes;
     const unsigned n_all = OP == kIn ? args.hidden : args.dim, k_all = OP == kIn ? args.dim : args.hidden;
     const unsigned n_tile = OP == kIn ? kTileN / 2 : kTileN, wide = (n_all + n_tile - 1) / n_tile;
-    const TileList list = {expert_row, args.cap, args.experts, BM, wide, args.more_than};
-    const uint64_t total = list.total(), chunk = (total + 7) / 8;
-    for (uint64_t i = blockIdx.x / 8; i < chunk; i += gridDim.x / 8) {
-        uint64_t t = blockIdx.x % 8 * chunk + i;
+    list.make(args.expert_row, args.stride, args.cap, args.experts, args.npes, BM, wide, args.more_than);
+    const unsigned total = list.total();
+    for (unsigned i = 0;; ++i) {
+        unsigned t = tile_of_block(i, total);
         if (t >= total) return;
-        const unsigned e = list.find(t);
+        unsigned e = list.find(t);
+        const unsigned pe = e / args.experts;
+        e -= pe * args.experts;
         uint64_t first, rows;
-        expert_range(expert_row, e, args.cap, first, rows);
+        expert_range(copy_of(args.expert_row, pe, args.stride), e, args.cap, first, rows);
         first = scalar64(first), rows = scalar64(rows);
         unsigned tm, tn;
-        tile_place((unsigned)t, (unsigned)((rows + BM - 1) / BM), wide, tm, tn);
+        tile_place(t, (unsigned)((rows + BM - 1) / BM), wide, tm, tn);
         const uint64_t m0 = (uint64_t)tm * BM;
+        if (m0 >= rows) continue;  // (a table whose ranges overlap many times over may count past 2^32)
         const unsigned n0 = tn * n_tile, m_here = rows - m0 < BM ? (unsigned)(rows - m0) : BM;
         const unsigned n_here = n_all - n0 < n_tile ? n_all - n0 : n_tile;
         const T *a = copy_of(OP == kIn ? args.rows : (const T *)args.h, pe, args.stride) + (first + m0) * k_all;
@@ -472,9 +475,9 @@ void launch_w4(const W4Args<T> &args, bool whole, int npes, hipStream_t stream) 
     else launch_few_w4<T, OP, false>(args, npes, stream);
     if (args.e.cap <= kW4FewRows) return;
     const uint64_t wide = div_up(OP == kIn ? args.e.hidden : args.e.dim, OP == kIn ? kTileN / 2 : kTileN);
-    const uint64_t tiles = (args.e.cap / kW4TileRows + (args.e.experts < args.e.cap ? args.e.experts : args.e.cap)) * wide;
-    if (whole) launch_kernel((expert_tile_w4_kernel<T, OP, true>), tile_grid(tiles, npes), dim3(kTileThreads), 0, stream, args);
-    else launch_kernel((expert_tile_w4_kernel<T, OP, false>), tile_grid(tiles, npes), dim3(kTileThreads), 0, stream, args);
+    const uint64_t tiles = (args.e.cap / kW4TileRows + (args.e.experts < args.e.cap ? args.e.experts : args.e.cap)) * wide * npes;
+    if (whole) launch_kernel((expert_tile_w4_kernel<T, OP, true>), dim3(tile_blocks(tiles, 1)), dim3(kTileThreads), 0, stream, args);
+    else launch_kernel((expert_tile_w4_kernel<T, OP, false>), dim3(tile_blocks(tiles, 1)), dim3(kTileThreads), 0, stream, args);
 }
 
 template <typename API>
@@ -505,7 +508,7 @@ int experts_w4_on_stream(API *out, void *workspace, const API *rows, const uint8
     if (cap == 0) return 0;
     args.group = (unsigned)group;
     args.per_group = (unsigned)((((uint64_t)1 << 31) + group / 32 - 1) / (group / 32));
-    a.stride = rt.heap_size, a.cap = cap, a.experts = (unsigned)mine, a.dim = (unsigned)dim, a.hidden = (unsigned)hidden;
+    a.stride = rt.heap_size, a.cap = cap, a.experts = (unsigned)mine, a.npes = (unsigned)rt.npes, a.dim = (unsigned)dim, a.hidden = (unsigned)hidden;
     a.more_than = kW4FewRows;
     const bool whole = dim * sizeof(T) % 16 == 0 && hidden * sizeof(T) % 16 == 0 && aligned16(a.rows);
     launch_w4<T, kIn>(args, whole, rt.npes, stream);
