@@ -277,14 +277,82 @@ constexpr bool a_by_k() { return OP == kDwIn || OP == kDwOut; }
 template <int OP>
 constexpr bool b_by_k() { return OP != kIn && OP != kOut; }
 
+// The multiplication of a tile, once its first two steps are on their way (start()).  A wavefront goes through a step in groups of one
+// piece of A with all of its pieces of B, kAhead groups after it read the piece, so that reads of LDS and products overlap.  All of a
+// step's pieces are in registers kAhead groups before its end: there the block meets, the step after the next takes the step's place in
+// LDS, and what is read from there on is of the next step.  us for 131072 rows of 64 experts (7168 x 2048 bf16, kIn / kOut) with the reads left to
+// the compiler, which waits for each pair of them: 6473 / 3637.
+template <typename T, typename A, typename B, unsigned kMi, unsigned kNi>
+struct TileProduct {
+    static constexpr unsigned kGroups = 2 * kMi, kAhead = kMi < 4 ? 1 : 2;
+    static constexpr int kMoves = A::kMoves + B::kMoves;
+    NVSHMEM_AMD_LDS char *lds_a, *lds_b;  // two steps of each
+    unsigned wave, lane;
+
+    // fetch(buffer, step): starts the step's way; land(buffer): ends it where it leads through registers.
+    template <bool DMA, typename FETCH, typename LAND>
+    __device__ __forceinline__ void start(unsigned steps, FETCH fetch, LAND land) const {
+        if (steps == 0) return;
+        fetch(0, 0);
+        land(0);
+        if (steps > 1) fetch(1, 1);
+    }
+    template <bool DMA, typename FETCH, typename LAND>
+    __device__ __forceinline__ void run(unsigned steps, FETCH fetch, LAND land, v4f (&acc)[kMi][kNi]) const {
+        if (steps == 0) return;
+        if (DMA && steps > 1) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kMoves) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+        __syncthreads();
+        const unsigned wm = wave / 4, wn = wave % 4;
+        v4u fa[2 * kAhead], fb[2][kNi];
+        const auto read_a = [&](unsigned buffer, unsigned g) {
+            fa[g % (2 * kAhead)] = A::read(lds_a + buffer * A::kBytes, wm * kMi + g % kMi, g / kMi, lane);
+        };
+        const auto read_b = [&](unsigned buffer, unsigned s, unsigned ni) { fb[s][ni] = B::read(lds_b + buffer * B::kBytes, wn * kNi + ni, s, lane); };
+#pragma unroll
+        for (unsigned ni = 0; ni < kNi; ++ni) read_b(0, 0, ni);
+#pragma unroll
+        for (unsigned g = 0; g < kAhead; ++g) read_a(0, g);
+        for (unsigned step = 0; step < steps; ++step) {
+            const unsigned buffer = step & 1;
+#pragma unroll
+            for (unsigned g = 0; g < kGroups; ++g) {
+                if (g == kGroups - kAhead) {
+                    land(buffer ^ 1);
+                    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // (a barrier alone does not wait for what is on its way to LDS)
+                    __syncthreads();
+                    if (step + 2 < steps) fetch(buffer, step + 2);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                // (behind the last step: what LDS happens to hold, unused)
+                const unsigned from = g < kGroups - kAhead ? buffer : buffer ^ 1;
+                read_a(from, (g + kAhead) % kGroups);
+                // the other half step's pieces of B, spread over the groups in front of it
+                if (g < kMi) {
+#pragma unroll
+                    for (unsigned ni = 0; ni < kNi; ++ni)
+                        if (kMi - kAhead <= g && ni * kAhead / kNi == g - (kMi - kAhead)) read_b(buffer, 1, ni);
+                } else if (g >= kGroups - kAhead) {
+#pragma unroll
+                    for (unsigned ni = 0; ni < kNi; ++ni)
+                        if (ni * kAhead / kNi == g - (kGroups - kAhead)) read_b(buffer ^ 1, 0, ni);
+                }
+#pragma unroll
+                for (unsigned ni = 0; ni < kNi; ++ni) acc[g % kMi][ni] = Mma<T>::step(fb[g / kMi][ni], fa[g % (2 * kAhead)], acc[g % kMi][ni]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    }
+};
+
 template <typename T, int OP, unsigned BM, unsigned BN, bool DMA>
 __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_kernel(const ExpertArgs<T> args) {
     typedef TileSide<T, BM, a_by_k<OP>(), DMA> A;
     typedef TileSide<T, BN, b_by_k<OP>(), DMA> B;
     constexpr unsigned kMi = BM / 32, kNi = BN / 64, kStepK = A::kStepK;
     constexpr bool kWeights = OP == kDwIn || OP == kDwOut;  // D is a weight's gradient: k runs over rows
-    __shared__ __attribute__((aligned(1024))) char lds_a[2][A::kBytes];
-    __shared__ __attribute__((aligned(1024))) char lds_b[2][B::kBytes];
+    __shared__ __attribute__((aligned(1024))) char lds_a[2 * A::kBytes];
+    __shared__ __attribute__((aligned(1024))) char lds_b[2 * B::kBytes];
     __shared__ TileList list;
     const unsigned wave = wave_of_block(), lane = threadIdx.x % kLanes;
     const unsigned dim = args.dim, hidden = args.hidden;
@@ -296,6 +364,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_kernel(const Expe
     const unsigned high_w = (m_all + BM - 1) / BM;
     if (!kWeights) list.make(args.expert_row, args.stride, args.cap, args.experts, args.npes, BM, wide, args.more_than);
     const unsigned total = kWeights ? args.experts * args.npes * high_w * wide : list.total();
+    const TileProduct<T, A, B, kMi, kNi> product = {(NVSHMEM_AMD_LDS char *)lds_a, (NVSHMEM_AMD_LDS char *)lds_b, wave, lane};
+    A side_a;
+    B side_b;
     for (unsigned i = 0;; ++i) {
         unsigned t = tile_of_block(i, total);
         if (t >= total) return;
@@ -329,43 +400,26 @@ __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_kernel(const Expe
         if (kWeights) b += first * ldb;
         b += b_by_k<OP>() ? (uint64_t)n0 : (uint64_t)n0 * ldb;
         const T *b_up = b + (uint64_t)hidden * dim;  // kIn: the same columns of up
-        A side_a;
-        B side_b;
         side_a.begin(wave, lane, m_here, lda, [](unsigned r) { return r; });
         // kIn: the first half of a wavefront's columns are gate's, the second half the same of up
         side_b.begin(wave, lane, n_here, ldb, [](unsigned r) { return OP == kIn ? r / (BN / 4) * (BN / 8) + r % (BN / 8) : r; });
-        const auto fetch = [&](unsigned buffer, uint64_t k) {
+        const auto fetch = [&](unsigned buffer, unsigned step) {
+            const uint64_t k = (uint64_t)step * kStepK;
             const unsigned left = k_all - k < kStepK ? (unsigned)(k_all - k) : kStepK;
-            side_a.fetch((NVSHMEM_AMD_LDS char *)lds_a[buffer], wave, left, [&](unsigned) { return a + (a_by_k<OP>() ? k * lda : k); });
-            side_b.fetch((NVSHMEM_AMD_LDS char *)lds_b[buffer], wave, left, [&](unsigned j) {
+            side_a.fetch((NVSHMEM_AMD_LDS char *)lds_a + buffer * A::kBytes, wave, left, [&](unsigned) { return a + (a_by_k<OP>() ? k * lda : k); });
+            side_b.fetch((NVSHMEM_AMD_LDS char *)lds_b + buffer * B::kBytes, wave, left, [&](unsigned j) {
                 const bool up = OP == kIn && (wave * B::kMoves + j) * 8 % (BN / 4) >= BN / 8;
                 return (up ? b_up : b) + (b_by_k<OP>() ? k * ldb : k);
             });
         };
+        const auto land = [&](unsigned buffer) {
+            side_a.land((NVSHMEM_AMD_LDS char *)lds_a + buffer * A::kBytes, wave, lane);
+            side_b.land((NVSHMEM_AMD_LDS char *)lds_b + buffer * B::kBytes, wave, lane);
+        };
         v4f acc[kMi][kNi] = {};
-        const unsigned wm = wave / 4, wn = wave % 4;
-        if (k_all) fetch(0, 0);
-        unsigned buffer = 0;
-        for (uint64_t k = 0; k < k_all; k += kStepK, buffer ^= 1) {
-            side_a.land((NVSHMEM_AMD_LDS char *)lds_a[buffer], wave, lane);
-            side_b.land((NVSHMEM_AMD_LDS char *)lds_b[buffer], wave, lane);
-            asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // (a barrier alone does not wait for what is on its way to LDS)
-            __syncthreads();
-            if (k + kStepK < k_all) fetch(buffer ^ 1, k + kStepK);
-#pragma unroll
-            for (unsigned s = 0; s < 2; ++s) {
-                v4u fa[kMi], fb[kNi];
-#pragma unroll
-                for (unsigned ni = 0; ni < kNi; ++ni) fb[ni] = B::read((NVSHMEM_AMD_LDS const char *)lds_b[buffer], wn * kNi + ni, s, lane);
-#pragma unroll
-                for (unsigned mi = 0; mi < kMi; ++mi) fa[mi] = A::read((NVSHMEM_AMD_LDS const char *)lds_a[buffer], wm * kMi + mi, s, lane);
-#pragma unroll
-                for (unsigned mi = 0; mi < kMi; ++mi)
-#pragma unroll
-                    for (unsigned ni = 0; ni < kNi; ++ni) acc[mi][ni] = Mma<T>::step(fb[ni], fa[mi], acc[mi][ni]);
-            }
-        }
-        __syncthreads();  // (the next tile's first step overwrites a buffer that others may still read)
+        const unsigned wm = wave / 4, wn = wave % 4, steps = (unsigned)((k_all + kStepK - 1) / kStepK);
+        product.template start<DMA>(steps, fetch, land);
+        product.template run<DMA>(steps, fetch, land, acc);
         // A lane has four consecutive columns of row lane % 16 of each 16 x 16 piece.
         const unsigned r = lane % 16, g = lane / 16;
 #pragma unroll
@@ -444,16 +498,22 @@ inline void launch_tiles_as(const ExpertArgs<T> &args, hipStream_t stream) {
     const uint64_t high = OP == kDwIn || OP == kDwOut ? args.experts * (uint64_t)div_up(OP == kDwIn ? 2 * (uint64_t)args.hidden : args.dim, BM)
                                                       : args.cap / BM + (args.experts < args.cap ? args.experts : args.cap);
     const uint64_t tiles = high * wide * args.npes;
-    if (tiles) launch_kernel((expert_tile_kernel<T, OP, BM, BN, DMA>), dim3(tile_blocks(tiles, BM == 128 && BN == 128 ? 2 : 1)), dim3(kTileThreads), 0, stream, args);
+    if (tiles) launch_kernel((expert_tile_kernel<T, OP, BM, BN, DMA>), dim3(tile_blocks(tiles, BN == 128 ? BM == 64 ? 3 : 2 : 1)), dim3(kTileThreads), 0, stream, args);
 }
+// Large tiles read the least and overlap the best within a tile, small ones waste less on experts of few rows and let one block of a compute
+// unit multiply while another stores.  What an expert may have on average, `rows`, is all that the host knows of the rows.
+// us of the forward pass, 256 x 256 / 128 x 128 / 64 x 128: bf16, 64 experts of 2048 x 1408 with 48 rows each 329 / 284 / 294, 100: 343 / 330 / 352, 300: 504 /
+// 519 / 612, 600: 754 / 821 / 1045; 32 of 7168 x 2048 with 48: 741 / 661 / 606, 300: 1148 / 1159 / 1479, 600: 1776 / 1971 / 2592.  fp32, 16 experts of 2048 x
+// 1408 with 48 rows 901 / 435 / 283, 180: 831 / 672 / 572, 600: 1648 / 1494 / 1401.  Tiles of 128 x 256 and 64 x 256 were not ahead of these anywhere.
 template <typename T, int OP, bool DMA>
 inline void launch_expert_tiles(const ExpertArgs<T> &args, hipStream_t stream) {
-    // The time of a shape: as often as its tiles fill the compute units, times what one takes.
-    const auto cost = [&](uint64_t bm, uint64_t bn, uint64_t weight) { return (tiles_of<T, OP>(args, bm, bn) + 255) / 256 * bm * bn * weight; };
-    const uint64_t large = cost(256, 256, 8), medium = cost(128, 256, 9), small = cost(128, 128, 12);
-    if (large <= medium && large <= small) launch_tiles_as<T, OP, 256, 256, DMA>(args, stream);
-    else if (medium <= small) launch_tiles_as<T, OP, 128, 256, DMA>(args, stream);
-    else launch_tiles_as<T, OP, 128, 128, DMA>(args, stream);
+    constexpr bool kWeights = OP == kDwIn || OP == kDwOut;
+    const uint64_t rows = (args.cap + args.experts - 1) / args.experts;
+    if constexpr (DMA && sizeof(T) == 2)
+        if (rows > 448 && tiles_of<T, OP>(args, 256, 256) >= 256) return launch_tiles_as<T, OP, 256, 256, DMA>(args, stream);
+    if constexpr (!kWeights)
+        if (sizeof(T) == 4 || rows <= 80 || tiles_of<T, OP>(args, 128, 128) < 256) return launch_tiles_as<T, OP, 64, 128, DMA>(args, stream);
+    launch_tiles_as<T, OP, 128, 128, DMA>(args, stream);
 }
 
 // Products of one PE's experts may be at most so wide and high; their offsets inside a tile stay under 2^31 bytes.
