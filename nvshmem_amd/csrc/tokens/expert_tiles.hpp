@@ -175,7 +175,7 @@ struct TileSide {
     unsigned width[kMoves]; // KM: elements of the chunk that are inside; else N
     v4u held[DMA ? 1 : kMoves];
 
-    static __device__ __forceinline__ unsigned swap(unsigned k) { return sizeof(T) == 2 ? k & 7 : k >> 2 & 3; }
+    static __device__ __forceinline__ unsigned swap(unsigned k) { return sizeof(T) == 2 ? (k & 3) | (k >> 1 & 4) : k >> 2 & 3; }
 
     // `extent`: rows (KM: columns) that exist from the tile's first on; ld in elements.  Tile row r is row place(r) of the operand.
     template <typename PLACE>
@@ -229,9 +229,9 @@ struct TileSide {
         const unsigned r = lane % 16, g = lane / 16;
         if (!KM) return *(NVSHMEM_AMD_LDS const v4u *)(lds + (block * 16 + r) * kStepBytes + (((s * 4 + g) ^ (r & 7)) * 16));
         if (sizeof(T) == 2) {
-            const unsigned k = s * 32 + g * 8 + r / 4;  // (k & 7 is r / 4, and r / 4 + 4 four k further)
-            const char NVSHMEM_AMD_LDS *p = lds + k * R * 2 + ((block ^ (r / 4)) * 32) + r % 4 * 8;
-            const char NVSHMEM_AMD_LDS *q = lds + (k + 4) * R * 2 + ((block ^ (r / 4 + 4)) * 32) + r % 4 * 8;
+            // (what a wavefront reads at once, k of g * 8 + 0..3 and four k further, is spread over all eight places of a block among eight)
+            const unsigned k = s * 32 + g * 8 + r / 4;
+            const char NVSHMEM_AMD_LDS *p = lds + k * R * 2 + ((block ^ (r / 4 | (g & 1) * 4)) * 32) + r % 4 * 8, *q = p + 4 * R * 2;
             const v2u lo = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((NVSHMEM_AMD_LDS v4s *)p));
             const v2u hi = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((NVSHMEM_AMD_LDS v4s *)q));
             return v4u{lo[0], lo[1], hi[0], hi[1]};
