@@ -258,6 +258,26 @@ __device__ __forceinline__ void store_four(T *p, v4f v, unsigned n) {
             if (i < n) p[i] = y[i];
     }
 }
+// Columns [c, c + 32) of a row, of which a lane has c + 4 (lane / 16) + i in lo and 16 further in hi; `n` of them exist.  Of 16-bit elements,
+// rows of 16 lanes exchange halves first, so that each lane stores eight consecutive ones: half as many stores of twice the length.
+template <typename T>
+__device__ __forceinline__ void store_32(T *row, unsigned c, v4f lo, v4f hi, unsigned n, unsigned lane) {
+    const unsigned g = lane / 16;
+    if constexpr (sizeof(T) == 4) {
+        if (c + g * 4 < n) store_four(row + c + g * 4, lo, n - c - g * 4);
+        if (c + 16 + g * 4 < n) store_four(row + c + 16 + g * 4, hi, n - c - 16 - g * 4);
+    } else {
+        typedef T four __attribute__((ext_vector_type(4)));
+        const v2u a = __builtin_bit_cast(v2u, __builtin_convertvector(lo, four)), b = __builtin_bit_cast(v2u, __builtin_convertvector(hi, four));
+        // (the second and fourth row of the first operand change places with the first and third of the second)
+        const auto x = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false), y = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+        const unsigned at = c + (g & 1) * 16 + (g >> 1) * 8;
+        if (at >= n) return;
+        const typename Chunk<T>::vec v = __builtin_bit_cast(typename Chunk<T>::vec, v4u{x[0], y[0], x[1], y[1]});
+        if (n - at >= 8) *(typename Chunk<T>::vec_unaligned *)(row + at) = v;
+        else chunk_store_part(row + at, v, n - at);
+    }
+}
 template <typename T>
 __device__ __forceinline__ v4f load_four(const T *p, unsigned n) {
     typedef T four __attribute__((ext_vector_type(4)));
@@ -428,49 +448,57 @@ __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_kernel(const Expe
             if (m >= m_here) continue;
             const uint64_t row = kWeights ? m0 + m : first + m0 + m;
             if (OP == kIn) {
+                v4f h[kNi / 2];
 #pragma unroll
                 for (unsigned ni = 0; ni < kNi / 2; ++ni) {
-                    const unsigned c = wn * (BN / 8) + ni * 16 + g * 4;
-                    if (c >= n_here) continue;
                     const v4f gate = acc[mi][ni], up = acc[mi][ni + kNi / 2];
-                    v4f h;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) h[i] = gate[i] * sigmoid(gate[i]) * up[i];
-                    store_four(copy_of(args.h, pe, args.stride) + row * hidden + n0 + c, h, n_here - c);
+                    for (int i = 0; i < 4; ++i) h[ni][i] = gate[i] * sigmoid(gate[i]) * up[i];
+                }
+                const unsigned c = wn * (BN / 8);
+                T *to = copy_of(args.h, pe, args.stride) + row * hidden + n0, *pre = copy_of(args.pre, pe, args.stride) + row * 2 * hidden + n0;
+                if constexpr (kNi == 4) {
+                    store_32(to, c, h[0], h[1], n_here, lane);
                     if (args.pre) {
-                        T *pre = copy_of(args.pre, pe, args.stride) + row * 2 * hidden + n0 + c;
-                        store_four(pre, gate, n_here - c);
-                        store_four(pre + hidden, up, n_here - c);
+                        store_32(pre, c, acc[mi][0], acc[mi][1], n_here, lane);
+                        store_32(pre + hidden, c, acc[mi][2], acc[mi][3], n_here, lane);
+                    }
+                } else if (c + g * 4 < n_here) {
+                    store_four(to + c + g * 4, h[0], n_here - c - g * 4);
+                    if (args.pre) {
+                        store_four(pre + c + g * 4, acc[mi][0], n_here - c - g * 4);
+                        store_four(pre + hidden + c + g * 4, acc[mi][1], n_here - c - g * 4);
                     }
                 }
                 continue;
             }
 #pragma unroll
-            for (unsigned ni = 0; ni < kNi; ++ni) {
-                const unsigned c = wn * (BN / 4) + ni * 16 + g * 4;
-                if (c >= n_here) continue;
-                const unsigned n = n0 + c, there = n_here - c;
+            for (unsigned ni = 0; ni < kNi; ni += 2) {
+                const unsigned c = wn * (BN / 4) + ni * 16;
                 if (OP == kDh) {
-                    const T *pre = copy_of(args.pre_in, pe, args.stride) + row * 2 * hidden + n;
-                    const v4f gate = load_four(pre, there), up = load_four(pre + hidden, there), dh = acc[mi][ni];
-                    v4f dgate, dup, h;
+                    const T *pre = copy_of(args.pre_in, pe, args.stride) + row * 2 * hidden + n0;
+                    v4f dgate[2], dup[2], h[2];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float s = sigmoid(gate[i]), silu = gate[i] * s;
-                        h[i] = silu * up[i];
-                        dup[i] = dh[i] * silu;
-                        dgate[i] = dh[i] * up[i] * (s + silu * (1.0f - s));
+                    for (unsigned half = 0; half < 2; ++half) {
+                        const unsigned at = c + half * 16 + g * 4, there = at < n_here ? n_here - at : 0;
+                        const v4f gate = load_four(pre + at, there), up = load_four(pre + hidden + at, there), dh = acc[mi][ni + half];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float s = sigmoid(gate[i]), silu = gate[i] * s;
+                            h[half][i] = silu * up[i];
+                            dup[half][i] = dh[i] * silu;
+                            dgate[half][i] = dh[i] * up[i] * (s + silu * (1.0f - s));
+                        }
                     }
-                    T *dpre = copy_of(args.dpre, pe, args.stride) + row * 2 * hidden + n;
-                    store_four(dpre, dgate, there);
-                    store_four(dpre + hidden, dup, there);
-                    store_four(copy_of(args.h, pe, args.stride) + row * hidden + n, h, there);
-                } else if (OP == kOut || OP == kDx) {
-                    store_four(copy_of(OP == kOut ? args.out : args.drows, pe, args.stride) + row * dim + n, acc[mi][ni], there);
-                } else if (OP == kDwIn) {
-                    store_four(copy_of(args.dw_in, pe, args.stride) + ((uint64_t)e * 2 * hidden + row) * dim + n, acc[mi][ni], there);
+                    T *dpre = copy_of(args.dpre, pe, args.stride) + row * 2 * hidden + n0;
+                    store_32(dpre, c, dgate[0], dgate[1], n_here, lane);
+                    store_32(dpre + hidden, c, dup[0], dup[1], n_here, lane);
+                    store_32(copy_of(args.h, pe, args.stride) + row * hidden + n0, c, h[0], h[1], n_here, lane);
                 } else {
-                    store_four(copy_of(args.dw_out, pe, args.stride) + ((uint64_t)e * dim + row) * hidden + n, acc[mi][ni], there);
+                    T *to = OP == kDwIn ? copy_of(args.dw_in, pe, args.stride) + ((uint64_t)e * 2 * hidden + row) * dim
+                          : OP == kDwOut ? copy_of(args.dw_out, pe, args.stride) + ((uint64_t)e * dim + row) * hidden
+                                         : copy_of(OP == kOut ? args.out : args.drows, pe, args.stride) + row * dim;
+                    store_32(to + n0, c, acc[mi][ni], acc[mi][ni + 1], n_here, lane);
                 }
             }
         }
