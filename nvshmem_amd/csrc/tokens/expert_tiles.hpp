@@ -114,6 +114,11 @@ struct TileList {
             own[i] = rows > more_than ? (unsigned)((rows + tile_rows - 1) / tile_rows) * columns : 0;
             sum += own[i];
         }
+        if (!__syncthreads_or(sum)) {  // as in a step of single tokens: none of this kernel's experts has rows
+            if (threadIdx.x == 0) first[kMostExperts] = 0;
+            __syncthreads();
+            return;
+        }
         unsigned before = sum;
 #pragma unroll
         for (int d = 1; d < kLanes; d *= 2) {

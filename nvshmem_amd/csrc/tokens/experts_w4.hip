@@ -106,18 +106,18 @@ struct words<4> {
 // parts), and the rows' scales.  While a chunk is multiplied the next is on its way.
 // Within a chunk a step is 32 * WORDS k, all of one group: lane (r, g) has of each of two groups of 16 rows 4 * WORDS bytes, 8 * WORDS
 // consecutive k of row r.  WORDS is 4 where the group is a multiple of 128, else 2 or 1.
-constexpr unsigned kFewW4Columns = 128;
+constexpr unsigned kFewW4Columns = 128, kFewW4Waves = 4, kFewW4Threads = kFewW4Waves * kLanes;
 
 template <typename T, unsigned WORDS, bool DMA>
 struct FewFourBits {
-    typedef TileSide<unsigned char, kFewW4Columns, false, DMA, kFewWaves> Side;
+    typedef TileSide<unsigned char, kFewW4Columns, false, DMA, kFewW4Waves> Side;
     static constexpr unsigned kChunk = 256, kParts = sizeof(T) == 4 ? 3 : 1, kStep = 32 * WORDS, kSteps = kChunk / kStep;
     static constexpr unsigned kRowBytes = kChunk * 2;  // of x in LDS
     typedef typename words<WORDS>::type raw;
     typedef typename Nibble<T>::type M;
     template <int MT>
     struct Held {
-        static constexpr unsigned kPieces = MT * 16 * kChunk / 8 / kFewThreads;  // of eight elements of x, a thread's
+        static constexpr unsigned kPieces = MT * 16 * kChunk / 8 / kFewW4Threads;  // of eight elements of x, a thread's
         v4u x[kPieces][8 / Chunk<T>::N];
         T scale[kSteps / 2 ? kSteps / 2 : 1];  // two threads have a row's
     };
@@ -133,7 +133,7 @@ struct FewFourBits {
         const bool whole = k + kChunk <= k_all;
 #pragma unroll
         for (unsigned i = 0; i < Held<MT>::kPieces; ++i) {
-            const unsigned piece = i * kFewThreads + threadIdx.x, m = piece / kPerRow, at = k + piece % kPerRow * 8;
+            const unsigned piece = i * kFewW4Threads + threadIdx.x, m = piece / kPerRow, at = k + piece % kPerRow * 8;
             const T *p = x + (uint64_t)(m < rows ? m : rows - 1) * k_all + at;  // (the last row's products stand in for rows behind it)
 #pragma unroll
             for (unsigned c = 0; c < 8 / N; ++c) h.x[i][c] = __builtin_bit_cast(v4u, chunk_load(p + c * N));
@@ -157,7 +157,7 @@ struct FewFourBits {
         constexpr unsigned kPerRow = kChunk / 8;
 #pragma unroll
         for (unsigned i = 0; i < Held<MT>::kPieces; ++i) {
-            const unsigned piece = i * kFewThreads + threadIdx.x, m = piece / kPerRow, c = piece % kPerRow;
+            const unsigned piece = i * kFewW4Threads + threadIdx.x, m = piece / kPerRow, c = piece % kPerRow;
             v4u a[kParts];
             if constexpr (sizeof(T) == 2) a[0] = reorder_eight(h.x[i][0]);
             else split_eight(__builtin_bit_cast(v4f, h.x[i][0]), __builtin_bit_cast(v4f, h.x[i][1]), a);
@@ -264,7 +264,7 @@ __device__ __forceinline__ void few_w4_store(const ExpertArgs<T> &args, const v4
 
 // An expert of up to `more_than` rows has a block for each 32 of them, which reads the weights again.
 template <typename T, int OP, unsigned WORDS, bool DMA>
-__global__ __launch_bounds__(kFewThreads, sizeof(T) == 4 ? 1 : 2) void expert_few_w4_kernel(const W4Args<T> args4) {
+__global__ __launch_bounds__(kFewW4Threads, sizeof(T) == 4 ? 1 : 2) void expert_few_w4_kernel(const W4Args<T> args4) {
     typedef FewFourBits<T, WORDS, DMA> W;
     constexpr unsigned kMost = sizeof(T) == 4 ? 16 : 32;  // rows of x at a time
     __shared__ __attribute__((aligned(1024))) char lds_w[2 * W::Side::kBytes];
@@ -464,9 +464,9 @@ void launch_few_w4(const W4Args<T> &args, int npes, hipStream_t stream) {
     const uint64_t rows = args.e.cap < kW4FewRows ? args.e.cap : kW4FewRows;
     const dim3 grid(div_up(OP == kIn ? args.e.hidden : args.e.dim, OP == kIn ? kFewW4Columns / 2 : kFewW4Columns),
                     args.e.experts * div_up(rows, sizeof(T) == 4 ? 16 : 32), npes);
-    if (args.group % 128 == 0) launch_kernel((expert_few_w4_kernel<T, OP, 4, DMA>), grid, dim3(kFewThreads), 0, stream, args);
-    else if (args.group % 64 == 0) launch_kernel((expert_few_w4_kernel<T, OP, 2, DMA>), grid, dim3(kFewThreads), 0, stream, args);
-    else launch_kernel((expert_few_w4_kernel<T, OP, 1, DMA>), grid, dim3(kFewThreads), 0, stream, args);
+    if (args.group % 128 == 0) launch_kernel((expert_few_w4_kernel<T, OP, 4, DMA>), grid, dim3(kFewW4Threads), 0, stream, args);
+    else if (args.group % 64 == 0) launch_kernel((expert_few_w4_kernel<T, OP, 2, DMA>), grid, dim3(kFewW4Threads), 0, stream, args);
+    else launch_kernel((expert_few_w4_kernel<T, OP, 1, DMA>), grid, dim3(kFewW4Threads), 0, stream, args);
 }
 template <typename T, int OP>
 void launch_w4(const W4Args<T> &args, bool whole, int npes, hipStream_t stream) {
