@@ -19,21 +19,23 @@ struct W4Args {
 
 // ---- experts of few rows ----
 
-// What x and a weight become for the matrix cores.  Of 16-bit elements, a weight is 16 + q, whose bits are those of 16 with q in the
-// mantissa; what that is too much, 24 times the sum of x, goes into the sums first as a product with -24.  The sums are in fp32, so that
-// what they lose by it is far below what the result is rounded to.  An fp32 element is the sum of three bf16 ones, of 8 bits of its mantissa
-// each, and weights are q - 8: nothing of it is lost in front of the sum.
+// What x and a weight become for the matrix cores.  Of 16-bit elements a weight is a power of two plus q, whose bits are those of the power
+// with q in the mantissa: one operation for two weights.  What that is too much, times the sum of x, goes into the sums first as a product
+// with too_much().  The sums are in fp32, so that what they lose by it is far below what the result is rounded to.  An fp32 element is the
+// sum of three bf16 ones, of 8 bits of its mantissa each, and weights are q - 8: nothing of it is lost in front of the sum.
 template <typename T>
 struct Nibble;
 template <>
 struct Nibble<__bf16> {
-    static constexpr unsigned kSixteen = 0x41804180u, kMinus24 = 0xC1C0C1C0u, kShift = 3;
     typedef __bf16 type;
+    // 128 + q, and 136 to take back
+    static __device__ __forceinline__ v4u too_much() { return v4u{0xC308C308u, 0xC308C308u, 0xC308C308u, 0xC308C308u}; }
 };
 template <>
 struct Nibble<_Float16> {
-    static constexpr unsigned kSixteen = 0x4C004C00u, kMinus24 = 0xCE00CE00u, kShift = 6;
     typedef _Float16 type;
+    // 1024 + q where q is the lowest four bits of a half, 64 + q where it is the next four: 1032 and 72 to take back
+    static __device__ __forceinline__ v4u too_much() { return v4u{0xE408E408u, 0xD480D480u, 0xE408E408u, 0xD480D480u}; }
 };
 template <>
 struct Nibble<float> : Nibble<__bf16> {};
@@ -41,7 +43,6 @@ struct Nibble<float> : Nibble<__bf16> {};
 // Eight weights, k in the order 0 4 1 5 2 6 3 7.
 template <typename T>
 __device__ __forceinline__ v4u eight_weights(unsigned q) {
-    constexpr unsigned s = Nibble<T>::kShift, mask = 0x000F000Fu << s;
     v4u v;
     if (sizeof(T) == 4) {
         const unsigned even = q & 0x0F0F0F0Fu, odd = q >> 4 & 0x0F0F0F0Fu;
@@ -53,11 +54,15 @@ __device__ __forceinline__ v4u eight_weights(unsigned q) {
         }
         return v;
     }
-#pragma unroll
-    for (unsigned j = 0; j < 4; ++j) {
-        const unsigned at = j * 4;
-        v[j] = ((at <= s ? q << (s - at) : q >> (at - s)) & mask) | Nibble<T>::kSixteen;
+    // (constants that the compiler does not see through stay in registers, where an "and" and an "or" are one instruction)
+    unsigned low = 0x000F000Fu, next = 0x00F000F0u, base = sizeof(T) == 4 ? 0 : __is_same(T, _Float16) ? 0x64006400u : 0x43004300u, base_next = 0x54005400u;
+    asm("" : "+v"(base), "+v"(base_next));
+    if (__is_same(T, _Float16)) {
+        const unsigned upper = q >> 8;
+        return v4u{(q & low) | base, (q & next) | base_next, (upper & low) | base, (upper & next) | base_next};
     }
+#pragma unroll
+    for (unsigned j = 0; j < 4; ++j) v[j] = (q >> j * 4 & low) | base;
     return v;
 }
 // Eight elements of x in that order.
@@ -173,7 +178,7 @@ struct FewFourBits {
     template <int MT>
     __device__ __forceinline__ void multiply(unsigned j, NVSHMEM_AMD_LDS const char *lds_w, NVSHMEM_AMD_LDS const char *lds_x,
                                              NVSHMEM_AMD_LDS const float *lds_s, unsigned wave, unsigned lane, v4f (&acc)[MT][2]) const {
-        const unsigned r = lane % 16, g = lane / 16, c = Nibble<T>::kMinus24;
+        const unsigned r = lane % 16, g = lane / 16;
         v4u a[MT][WORDS][kParts];
         v4f sum[MT] = {};
 #pragma unroll
@@ -184,7 +189,7 @@ struct FewFourBits {
                 for (unsigned q = 0; q < kParts; ++q) {
                     const unsigned chunk = (j * 4 + g) * WORDS + i;
                     a[mi][i][q] = *(NVSHMEM_AMD_LDS const v4u *)(lds_x + ((q * MT + mi) * 16 + r) * kRowBytes + (chunk ^ (r & 7)) * 16);
-                    if (sizeof(T) == 2) sum[mi] = Mma<M>::step(v4u{c, c, c, c}, a[mi][i][q], sum[mi]);
+                    if (sizeof(T) == 2) sum[mi] = Mma<M>::step(Nibble<T>::too_much(), a[mi][i][q], sum[mi]);
                 }
 #pragma unroll
         for (unsigned ni = 0; ni < 2; ++ni) {
@@ -305,16 +310,18 @@ __global__ __launch_bounds__(kFewW4Threads, sizeof(T) == 4 ? 1 : 2) void expert_
 
 // ---- experts of more rows: tiles ----
 
-// B's way into LDS: 256 rows of packed weights, half a step's k of a row for each thread, as q - 8 in T (exact) where TileSide<T, 256, false>
+constexpr unsigned kTileN = 256;
+
+// B's way into LDS: 256 rows of packed weights, half a step's k of a row for each thread, as (q - 8) / 16 in T (exact) where TileSide<T, 256, false>
 // reads them.  Their scales go beside them, one for each half of each row.
 template <typename T>
 struct FourBitSide {
-    static constexpr unsigned kTileN = 256, kStepK = kStepBytes / sizeof(T), kHalfK = kStepK / 2, kWords = kHalfK / 8;
+    static constexpr unsigned kStepK = kStepBytes / sizeof(T), kHalfK = kStepK / 2, kWords = kHalfK / 8;
     typedef typename words<kWords>::type raw;
     typedef raw raw_unaligned __attribute__((aligned(1)));
     const unsigned char *row;  // this thread's; where it has none, a row that exists
     const T *scale;
-    unsigned k_all, group;
+    unsigned k_all, per_group;
     raw held;
     float held_scale;
 
@@ -322,9 +329,9 @@ struct FourBitSide {
         const unsigned at = (unsigned)k + threadIdx.x % 2 * kHalfK;
         const unsigned char *p = row + at / 2;
         held = *(const raw_unaligned *)p;  // (behind the row's end: what lies there, times zeros of A)
-        held_scale = (float)scale[(at < k_all ? at : (unsigned)k) / group];
+        held_scale = (float)scale[__umulhi((at < k_all ? at : (unsigned)k) / 16, per_group)];
     }
-    __device__ __forceinline__ void land(NVSHMEM_AMD_LDS char *lds, float *scales) const {
+    __device__ __forceinline__ void land(NVSHMEM_AMD_LDS char *lds, NVSHMEM_AMD_LDS float *scales) const {
         const unsigned r = threadIdx.x / 2, half = threadIdx.x % 2;
         scales[half * kTileN + r] = held_scale;
 #pragma unroll
@@ -332,28 +339,28 @@ struct FourBitSide {
             typename Chunk<T>::vec v;
 #pragma unroll
             for (unsigned i = 0; i < (unsigned)Chunk<T>::N; ++i) {
-                const unsigned at = j * Chunk<T>::N + i;
-                v[i] = (T)((float)(held[at / 8] >> at % 8 * 4 & 15) - 8.0f);
+                // (the instruction takes four bits with a sign and gives a sixteenth of them: q - 8 with its highest bit turned over)
+                const unsigned at = j * Chunk<T>::N + i, word = held[at / 8] ^ 0x88888888u;
+                v[i] = (T)__builtin_amdgcn_cvt_off_f32_i4((int)((at % 2 ? word >> 4 : word) >> at % 8 / 2 * 8));
             }
             *(NVSHMEM_AMD_LDS v4u *)(lds + r * kStepBytes + (((half * 4 + j) ^ (r & 7)) * 16)) = __builtin_bit_cast(v4u, v);
         }
     }
 };
 
-constexpr unsigned kW4TileRows = 128, kTileN = 256;
-
-template <typename T, int OP, bool DMA>
+// HALVES: the halves of a step may be of two groups.
+template <typename T, int OP, unsigned BM, bool HALVES, bool DMA>
 __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_w4_kernel(const W4Args<T> args4) {
-    constexpr unsigned BM = kW4TileRows, kMi = BM / 32, kNi = 4;
+    constexpr unsigned kMi = BM / 32, kNi = 4;
     typedef TileSide<T, BM, false, DMA> A;
     typedef TileSide<T, kTileN, false, true> B;  // (its layout in LDS)
     typedef FourBitSide<T> Q;
     constexpr unsigned kStepK = A::kStepK;
-    __shared__ __attribute__((aligned(1024))) char lds_a[2][A::kBytes];
-    __shared__ __attribute__((aligned(1024))) char lds_b[2][B::kBytes];
-    __shared__ __attribute__((aligned(16))) float lds_s[2][2 * kTileN];
-    const ExpertArgs<T> &args = args4.e;
+    __shared__ __attribute__((aligned(1024))) char lds_a[2 * A::kBytes];
+    __shared__ __attribute__((aligned(1024))) char lds_b[2 * B::kBytes];
+    __shared__ __attribute__((aligned(16))) float lds_s[2 * 2 * kTileN];
     __shared__ TileList list;
+    const ExpertArgs<T> &args = args4.e;
     const unsigned wave = wave_of_block(), lane = threadIdx.x % kLanes;
     const unsigned n_all = OP == kIn ? args.hidden : args.dim, k_all = OP == kIn ? args.dim : args.hidden;
     const unsigned n_tile = OP == kIn ? kTileN / 2 : kTileN, wide = (n_all + n_tile - 1) / n_tile;
@@ -381,76 +388,73 @@ __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_w4_kernel(const W
         {
             const unsigned r = threadIdx.x / 2, at = OP == kIn ? r / 64 * 32 + r % 32 : r;
             const uint64_t n = (uint64_t)e * (OP == kIn ? 2 : 1) * n_all + (OP == kIn && r % 64 >= 32 ? n_all : 0) + n0 + (at < n_here ? at : n_here - 1);
-            side_b.k_all = k_all, side_b.group = args4.group;
+            side_b.k_all = k_all, side_b.per_group = args4.per_group;
             side_b.row = copy_of(OP == kIn ? args4.w_in : args4.w_out, pe, args.stride) + n * ((k_all + 1) / 2);
             side_b.scale = copy_of(OP == kIn ? args4.s_in : args4.s_out, pe, args.stride) + n * ((k_all + args4.group - 1) / args4.group);
         }
         const auto fetch = [&](unsigned buffer, unsigned k) {
             const unsigned left = k_all - k < kStepK ? k_all - k : kStepK;
-            side_a.fetch((NVSHMEM_AMD_LDS char *)lds_a[buffer], wave, left, [&](unsigned) { return a + k; });
             side_b.fetch(k);
+            side_a.fetch((NVSHMEM_AMD_LDS char *)lds_a + buffer * A::kBytes, wave, left, [&](unsigned) { return a + k; });
         };
         v4f acc[kMi][kNi] = {};
         const unsigned wm = wave / 4, wn = wave % 4;
         fetch(0, 0);
         unsigned buffer = 0;
-        const bool halves = args4.group % kStepK != 0;  // (then the halves of a step may be of two groups)
         for (unsigned k = 0; k < k_all; k += kStepK, buffer ^= 1) {
-            side_a.land((NVSHMEM_AMD_LDS char *)lds_a[buffer], wave, lane);
-            side_b.land((NVSHMEM_AMD_LDS char *)lds_b[buffer], lds_s[buffer]);
+            NVSHMEM_AMD_LDS char *la = (NVSHMEM_AMD_LDS char *)lds_a + buffer * A::kBytes, *lb = (NVSHMEM_AMD_LDS char *)lds_b + buffer * B::kBytes;
+            NVSHMEM_AMD_LDS float *ls = (NVSHMEM_AMD_LDS float *)lds_s + buffer * 2 * kTileN;
+            side_a.land(la, wave, lane);
+            side_b.land(lb, ls);
             asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
             __syncthreads();
             if (k + kStepK < k_all) fetch(buffer ^ 1, k + kStepK);
-            v4u fa[2][kMi], fb[2][kNi];
-#pragma unroll
-            for (unsigned s = 0; s < 2; ++s) {
-#pragma unroll
-                for (unsigned ni = 0; ni < kNi; ++ni) fb[s][ni] = B::read((NVSHMEM_AMD_LDS const char *)lds_b[buffer], wn * 4 + ni, s, lane);
-#pragma unroll
-                for (unsigned mi = 0; mi < kMi; ++mi) fa[s][mi] = A::read((NVSHMEM_AMD_LDS const char *)lds_a[buffer], wm * kMi + mi, s, lane);
-            }
+            v4u fb[2][kNi], fa[2][2];
+            v4f s[HALVES ? 2 : 1][kNi];
 #pragma unroll
             for (unsigned ni = 0; ni < kNi; ++ni) {
-                const float *s = &lds_s[buffer][wn * 64 + ni * 16 + lane / 16 * 4];
-                const v4f s0 = *(const v4f *)s, s1 = *(const v4f *)(s + kTileN);
+                fb[0][ni] = B::read(lb, wn * 4 + ni, 0, lane), fb[1][ni] = B::read(lb, wn * 4 + ni, 1, lane);
+                s[0][ni] = *(NVSHMEM_AMD_LDS const v4f *)(ls + wn * 64 + ni * 16 + lane / 16 * 4);
+                if (HALVES) s[HALVES][ni] = *(NVSHMEM_AMD_LDS const v4f *)(ls + kTileN + wn * 64 + ni * 16 + lane / 16 * 4);
+            }
+            fa[0][0] = A::read(la, wm * kMi, 0, lane), fa[0][1] = A::read(la, wm * kMi, 1, lane);
 #pragma unroll
-                for (unsigned mi = 0; mi < kMi; ++mi) {
-                    v4f d = Mma<T>::step(fb[0][ni], fa[0][mi], v4f{});
-                    if (halves) {
+            for (unsigned mi = 0; mi < kMi; ++mi) {
+                if (mi + 1 < kMi) fa[(mi + 1) % 2][0] = A::read(la, wm * kMi + mi + 1, 0, lane), fa[(mi + 1) % 2][1] = A::read(la, wm * kMi + mi + 1, 1, lane);
+                v4f d[2][kNi];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) acc[mi][ni][j] = __builtin_fmaf(s0[j], d[j], acc[mi][ni][j]);
-                        d = v4f{};
+                for (unsigned ni = 0; ni < kNi; ++ni) d[0][ni] = Mma<T>::step(fb[0][ni], fa[mi % 2][0], v4f{});
+#pragma unroll
+                for (unsigned ni = 0; ni < kNi; ++ni) d[1][ni] = Mma<T>::step(fb[1][ni], fa[mi % 2][1], HALVES ? v4f{} : d[0][ni]);
+#pragma unroll
+                for (unsigned ni = 0; ni < kNi; ++ni)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (HALVES) acc[mi][ni][j] = __builtin_fmaf(s[0][ni][j], d[0][ni][j], acc[mi][ni][j]);
+                        acc[mi][ni][j] = __builtin_fmaf(s[HALVES][ni][j], d[1][ni][j], acc[mi][ni][j]);
                     }
-                    d = Mma<T>::step(fb[1][ni], fa[1][mi], d);
-                    const v4f scale = halves ? s1 : s0;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[mi][ni][j] = __builtin_fmaf(scale[j], d[j], acc[mi][ni][j]);
-                }
             }
         }
         __syncthreads();
-        const unsigned r = lane % 16, g = lane / 16;
+        const unsigned r = lane % 16;
 #pragma unroll
         for (unsigned mi = 0; mi < kMi; ++mi) {
             const unsigned m = (wm * kMi + mi) * 16 + r;
             if (m >= m_here) continue;
             const uint64_t row = first + m0 + m;
+            v4f v[kNi];
+#pragma unroll
+            for (unsigned ni = 0; ni < kNi; ++ni) v[ni] = acc[mi][ni] * 16.0f;  // (weights were sixteenths)
             if (OP == kIn) {
 #pragma unroll
-                for (unsigned ni = 0; ni < 2; ++ni) {
-                    const unsigned c = wn * 32 + ni * 16 + g * 4;
-                    if (c >= n_here) continue;
-                    v4f h;
+                for (unsigned ni = 0; ni < 2; ++ni)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) h[j] = acc[mi][ni][j] * sigmoid(acc[mi][ni][j]) * acc[mi][ni + 2][j];
-                    store_four(copy_of(args.h, pe, args.stride) + row * args.hidden + n0 + c, h, n_here - c);
-                }
+                    for (int j = 0; j < 4; ++j) v[ni][j] = v[ni][j] * sigmoid(v[ni][j]) * v[ni + 2][j];
+                store_32(copy_of(args.h, pe, args.stride) + row * args.hidden + n0, wn * 32, v[0], v[1], n_here, lane);
             } else {
 #pragma unroll
-                for (unsigned ni = 0; ni < kNi; ++ni) {
-                    const unsigned c = wn * 64 + ni * 16 + g * 4;
-                    if (c < n_here) store_four(copy_of(args.out, pe, args.stride) + row * args.dim + n0 + c, acc[mi][ni], n_here - c);
-                }
+                for (unsigned ni = 0; ni < kNi; ni += 2)
+                    store_32(copy_of(args.out, pe, args.stride) + row * args.dim + n0, wn * 64 + ni * 16, v[ni], v[ni + 1], n_here, lane);
             }
         }
     }
@@ -458,6 +462,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_w4_kernel(const W
 
 // Experts of more rows are the tiles'.
 constexpr unsigned kW4FewRows = 64;
+// ... and those of 256 rows where experts have more than this on average at most: weights are made ready half as often.
+constexpr unsigned kW4LargeRows = 256;
 
 template <typename T, int OP, bool DMA>
 void launch_few_w4(const W4Args<T> &args, int npes, hipStream_t stream) {
@@ -468,16 +474,27 @@ void launch_few_w4(const W4Args<T> &args, int npes, hipStream_t stream) {
     else if (args.group % 64 == 0) launch_kernel((expert_few_w4_kernel<T, OP, 2, DMA>), grid, dim3(kFewW4Threads), 0, stream, args);
     else launch_kernel((expert_few_w4_kernel<T, OP, 1, DMA>), grid, dim3(kFewW4Threads), 0, stream, args);
 }
+template <typename T, int OP, unsigned BM, bool HALVES, bool DMA>
+void launch_tiles_w4_as(const W4Args<T> &args, int npes, hipStream_t stream) {
+    const uint64_t wide = div_up(OP == kIn ? args.e.hidden : args.e.dim, OP == kIn ? kTileN / 2 : kTileN);
+    const uint64_t tiles = (args.e.cap / BM + (args.e.experts < args.e.cap ? args.e.experts : args.e.cap)) * wide * npes;
+    launch_kernel((expert_tile_w4_kernel<T, OP, BM, HALVES, DMA>), dim3(tile_blocks(tiles, 1)), dim3(kTileThreads), 0, stream, args);
+}
+template <typename T, int OP, bool HALVES>
+void launch_tiles_w4(const W4Args<T> &args, bool whole, int npes, hipStream_t stream) {
+    const uint64_t rows = (args.e.cap + args.e.experts - 1) / args.e.experts;
+    if (!whole) launch_tiles_w4_as<T, OP, 128, HALVES, false>(args, npes, stream);
+    else if (sizeof(T) == 2 && rows > kW4LargeRows) launch_tiles_w4_as<T, OP, 256, HALVES, true>(args, npes, stream);
+    else launch_tiles_w4_as<T, OP, 128, HALVES, true>(args, npes, stream);
+}
 template <typename T, int OP>
 void launch_w4(const W4Args<T> &args, bool whole, int npes, hipStream_t stream) {
     const unsigned row_bytes = ((OP == kIn ? args.e.dim : args.e.hidden) + 1) / 2;
     if (row_bytes % 16 == 0 && aligned16(OP == kIn ? args.w_in : args.w_out)) launch_few_w4<T, OP, true>(args, npes, stream);
     else launch_few_w4<T, OP, false>(args, npes, stream);
     if (args.e.cap <= kW4FewRows) return;
-    const uint64_t wide = div_up(OP == kIn ? args.e.hidden : args.e.dim, OP == kIn ? kTileN / 2 : kTileN);
-    const uint64_t tiles = (args.e.cap / kW4TileRows + (args.e.experts < args.e.cap ? args.e.experts : args.e.cap)) * wide * npes;
-    if (whole) launch_kernel((expert_tile_w4_kernel<T, OP, true>), dim3(tile_blocks(tiles, 1)), dim3(kTileThreads), 0, stream, args);
-    else launch_kernel((expert_tile_w4_kernel<T, OP, false>), dim3(tile_blocks(tiles, 1)), dim3(kTileThreads), 0, stream, args);
+    if (sizeof(T) == 2 && args.group % 64) launch_tiles_w4<T, OP, true>(args, whole, npes, stream);
+    else launch_tiles_w4<T, OP, false>(args, whole, npes, stream);
 }
 
 template <typename API>
