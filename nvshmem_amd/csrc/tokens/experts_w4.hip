@@ -421,18 +421,22 @@ __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_w4_kernel(const W
 #pragma unroll
             for (unsigned mi = 0; mi < kMi; ++mi) {
                 if (mi + 1 < kMi) fa[(mi + 1) % 2][0] = A::read(la, wm * kMi + mi + 1, 0, lane), fa[(mi + 1) % 2][1] = A::read(la, wm * kMi + mi + 1, 1, lane);
-                v4f d[2][kNi];
 #pragma unroll
-                for (unsigned ni = 0; ni < kNi; ++ni) d[0][ni] = Mma<T>::step(fb[0][ni], fa[mi % 2][0], v4f{});
+                for (unsigned n = 0; n < kNi; n += 2) {
+                    v4f d[2][2];
 #pragma unroll
-                for (unsigned ni = 0; ni < kNi; ++ni) d[1][ni] = Mma<T>::step(fb[1][ni], fa[mi % 2][1], HALVES ? v4f{} : d[0][ni]);
+                    for (unsigned ni = 0; ni < 2; ++ni) d[0][ni] = Mma<T>::step(fb[0][n + ni], fa[mi % 2][0], v4f{});
 #pragma unroll
-                for (unsigned ni = 0; ni < kNi; ++ni)
+                    for (unsigned ni = 0; ni < 2; ++ni) d[1][ni] = Mma<T>::step(fb[1][n + ni], fa[mi % 2][1], HALVES ? v4f{} : d[0][ni]);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (HALVES) acc[mi][ni][j] = __builtin_fmaf(s[0][ni][j], d[0][ni][j], acc[mi][ni][j]);
-                        acc[mi][ni][j] = __builtin_fmaf(s[HALVES][ni][j], d[1][ni][j], acc[mi][ni][j]);
-                    }
+                    for (unsigned ni = 0; ni < 2; ++ni)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if (HALVES) acc[mi][n + ni][j] = __builtin_fmaf(s[0][n + ni][j], d[0][ni][j], acc[mi][n + ni][j]);
+                            acc[mi][n + ni][j] = __builtin_fmaf(s[HALVES][n + ni][j], d[1][ni][j], acc[mi][n + ni][j]);
+                        }
+                }
+                if (BM == 256) __builtin_amdgcn_sched_barrier(0);  // (or products of several rows wait for their sums in registers that are not there)
             }
         }
         __syncthreads();
