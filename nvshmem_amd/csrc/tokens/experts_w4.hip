@@ -106,23 +106,32 @@ struct words<4> {
     typedef v4u type;
 };
 
-// A block has 128 rows of one expert's weights, 32 a wavefront, and up to 32 rows of x.  It goes over k in chunks of 256: weights go to LDS as
+// A block has 32 rows of one expert's weights for each of its wavefronts, and up to 32 rows of x.  It goes over k in chunks of 256: weights go to LDS as
 // they are, whole lines of memory (128 bytes of a row) at a time; x goes there in the order that the matrix cores take (fp32: as three
 // parts), and the rows' scales.  While a chunk is multiplied the next is on its way.
 // Within a chunk a step is 32 * WORDS k, all of one group: lane (r, g) has of each of two groups of 16 rows 4 * WORDS bytes, 8 * WORDS
 // consecutive k of row r.  WORDS is 4 where the group is a multiple of 128, else 2 or 1.
-constexpr unsigned kFewW4Columns = 128, kFewW4Waves = 4, kFewW4Threads = kFewW4Waves * kLanes;
+
+
+// Wavefronts of a block.  A few small blocks to a compute unit wait for memory apart from each other; only of fp32 elements, whose three
+// parts fill LDS, eight wavefronts share one x.
+template <typename T>
+constexpr unsigned few_w4_waves() {
+    return sizeof(T) == 4 ? 8 : 4;
+}
 
 template <typename T, unsigned WORDS, bool DMA>
 struct FewFourBits {
-    typedef TileSide<unsigned char, kFewW4Columns, false, DMA, kFewW4Waves> Side;
+    static constexpr unsigned kWaves = few_w4_waves<T>(), kThreads = kWaves * kLanes, kColumns = kWaves * 32;
+    static constexpr bool kTwo = sizeof(T) == 4;  // x and scales of two chunks in LDS
+    typedef TileSide<unsigned char, kColumns, false, DMA, kWaves> Side;
     static constexpr unsigned kChunk = 256, kParts = sizeof(T) == 4 ? 3 : 1, kStep = 32 * WORDS, kSteps = kChunk / kStep;
     static constexpr unsigned kRowBytes = kChunk * 2;  // of x in LDS
     typedef typename words<WORDS>::type raw;
     typedef typename Nibble<T>::type M;
     template <int MT>
     struct Held {
-        static constexpr unsigned kPieces = MT * 16 * kChunk / 8 / kFewW4Threads;  // of eight elements of x, a thread's
+        static constexpr unsigned kPieces = MT * 16 * kChunk / 8 / kThreads;  // of eight elements of x, a thread's
         v4u x[kPieces][8 / Chunk<T>::N];
         T scale[kSteps / 2 ? kSteps / 2 : 1];  // two threads have a row's
     };
@@ -138,7 +147,7 @@ struct FewFourBits {
         const bool whole = k + kChunk <= k_all;
 #pragma unroll
         for (unsigned i = 0; i < Held<MT>::kPieces; ++i) {
-            const unsigned piece = i * kFewW4Threads + threadIdx.x, m = piece / kPerRow, at = k + piece % kPerRow * 8;
+            const unsigned piece = i * kThreads + threadIdx.x, m = piece / kPerRow, at = k + piece % kPerRow * 8;
             const T *p = x + (uint64_t)(m < rows ? m : rows - 1) * k_all + at;  // (the last row's products stand in for rows behind it)
 #pragma unroll
             for (unsigned c = 0; c < 8 / N; ++c) h.x[i][c] = __builtin_bit_cast(v4u, chunk_load(p + c * N));
@@ -149,7 +158,7 @@ struct FewFourBits {
         }
 #pragma unroll
         for (unsigned j = 0; j < kSteps / 2; ++j) {
-            const unsigned at = k + (threadIdx.x / kFewW4Columns * (kSteps / 2) + j) * kStep;
+            const unsigned at = k + (threadIdx.x / kColumns * (kSteps / 2) + j) * kStep;
             h.scale[j] = scale[__umulhi((at < k_all ? at : k) / 16, per_group)];
         }
         const unsigned wave = wave_of_block(), left = (k_all - k + 1) / 2;
@@ -162,7 +171,7 @@ struct FewFourBits {
         constexpr unsigned kPerRow = kChunk / 8;
 #pragma unroll
         for (unsigned i = 0; i < Held<MT>::kPieces; ++i) {
-            const unsigned piece = i * kFewW4Threads + threadIdx.x, m = piece / kPerRow, c = piece % kPerRow;
+            const unsigned piece = i * kThreads + threadIdx.x, m = piece / kPerRow, c = piece % kPerRow;
             v4u a[kParts];
             if constexpr (sizeof(T) == 2) a[0] = reorder_eight(h.x[i][0]);
             else split_eight(__builtin_bit_cast(v4f, h.x[i][0]), __builtin_bit_cast(v4f, h.x[i][1]), a);
@@ -172,7 +181,7 @@ struct FewFourBits {
         }
 #pragma unroll
         for (unsigned j = 0; j < kSteps / 2; ++j)
-            lds_s[(threadIdx.x / kFewW4Columns * (kSteps / 2) + j) * kFewW4Columns + threadIdx.x % kFewW4Columns] = (float)h.scale[j];
+            lds_s[(threadIdx.x / kColumns * (kSteps / 2) + j) * kColumns + threadIdx.x % kColumns] = (float)h.scale[j];
     }
     // D = w x^T: element i of a lane is row lane / 16 * 4 + i of the weights' 16, column lane % 16: a row of x.
     template <int MT>
@@ -209,7 +218,7 @@ struct FewFourBits {
 #pragma unroll
                     for (unsigned q = 0; q < kParts; ++q) d[mi] = Mma<M>::step(b, a[mi][i][q], d[mi]);
             }
-            const v4f s = *(NVSHMEM_AMD_LDS const v4f *)(lds_s + j * kFewW4Columns + row + g * 4);
+            const v4f s = *(NVSHMEM_AMD_LDS const v4f *)(lds_s + j * kColumns + row + g * 4);
 #pragma unroll
             for (int mi = 0; mi < MT; ++mi)
 #pragma unroll
@@ -218,19 +227,20 @@ struct FewFourBits {
     }
     template <int MT>
     __device__ __forceinline__ void sum(char *lds_w, char *lds_x, float *lds_s, bool in, v4f (&acc)[MT][2]) {
-        constexpr unsigned kXBytes = kParts * MT * 16 * kRowBytes, kScales = kSteps * kFewW4Columns;
+        constexpr unsigned kXBytes = kParts * MT * 16 * kRowBytes, kScales = kSteps * kColumns;
         const unsigned wave = wave_of_block(), lane = threadIdx.x % kLanes;
         Held<MT> next;
         fetch(next, (NVSHMEM_AMD_LDS char *)lds_w, 0, in);
         unsigned buffer = 0;
         for (unsigned k = 0; k < k_all; k += kChunk, buffer ^= 1) {
             NVSHMEM_AMD_LDS char *lw = (NVSHMEM_AMD_LDS char *)lds_w + buffer * Side::kBytes;
-            NVSHMEM_AMD_LDS char *lx = (NVSHMEM_AMD_LDS char *)lds_x + buffer * kXBytes;
-            NVSHMEM_AMD_LDS float *ls = (NVSHMEM_AMD_LDS float *)lds_s + buffer * kScales;
+            NVSHMEM_AMD_LDS char *lx = (NVSHMEM_AMD_LDS char *)lds_x + (kTwo ? buffer : 0) * kXBytes;
+            NVSHMEM_AMD_LDS float *ls = (NVSHMEM_AMD_LDS float *)lds_s + (kTwo ? buffer : 0) * kScales;
+            if (!kTwo && k) __syncthreads();  // (all have multiplied the last chunk)
             side.land(lw, wave, lane);
             land(next, lx, ls);
             asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-            __syncthreads();  // (one a chunk: a buffer is written again two chunks later)
+            __syncthreads();
             if (k + kChunk < k_all) fetch(next, (NVSHMEM_AMD_LDS char *)lds_w + (buffer ^ 1) * Side::kBytes, k + kChunk, in);
 #pragma unroll
             for (unsigned j = 0; j < kSteps; ++j) {
@@ -269,15 +279,15 @@ __device__ __forceinline__ void few_w4_store(const ExpertArgs<T> &args, const v4
 
 // An expert of up to `more_than` rows has a block for each 32 of them, which reads the weights again.
 template <typename T, int OP, unsigned WORDS, bool DMA>
-__global__ __launch_bounds__(kFewW4Threads, sizeof(T) == 4 ? 1 : 2) void expert_few_w4_kernel(const W4Args<T> args4) {
+__global__ __launch_bounds__(few_w4_waves<T>() * kLanes, sizeof(T) == 4 ? 2 : 3) void expert_few_w4_kernel(const W4Args<T> args4) {
     typedef FewFourBits<T, WORDS, DMA> W;
     constexpr unsigned kMost = sizeof(T) == 4 ? 16 : 32;  // rows of x at a time
     __shared__ __attribute__((aligned(1024))) char lds_w[2 * W::Side::kBytes];
-    __shared__ __attribute__((aligned(16))) char lds_x[2 * W::kParts * kMost * W::kRowBytes];
-    __shared__ __attribute__((aligned(16))) float lds_s[2 * W::kSteps * kFewW4Columns];
+    __shared__ __attribute__((aligned(16))) char lds_x[(W::kTwo ? 2 : 1) * W::kParts * kMost * W::kRowBytes];
+    __shared__ __attribute__((aligned(16))) float lds_s[(W::kTwo ? 2 : 1) * W::kSteps * W::kColumns];
     const ExpertArgs<T> &args = args4.e;
     const unsigned pe = blockIdx.z, lane = threadIdx.x % kLanes, part = blockIdx.y / args.experts, e = blockIdx.y % args.experts;
-    const unsigned n0 = blockIdx.x * (OP == kIn ? kFewW4Columns / 2 : kFewW4Columns);
+    const unsigned n0 = blockIdx.x * (OP == kIn ? W::kColumns / 2 : W::kColumns);
     uint64_t first, rows;
     expert_range(copy_of(args.expert_row, pe, args.stride), e, args.cap, first, rows);
     if (rows <= part * kMost || rows > args.more_than) return;
@@ -292,7 +302,7 @@ __global__ __launch_bounds__(kFewW4Threads, sizeof(T) == 4 ? 1 : 2) void expert_
     w.side.begin(wave_of_block(), lane, n_here, row_bytes, place);
     w.w = copy_of(OP == kIn ? args4.w_in : args4.w_out, pe, args.stride) + before * row_bytes;
     w.w_up = w.w + (uint64_t)n_all * row_bytes;
-    const unsigned r = threadIdx.x % kFewW4Columns, at = place(r) < n_here ? place(r) : n_here - 1;
+    const unsigned r = threadIdx.x % W::kColumns, at = place(r) < n_here ? place(r) : n_here - 1;
     w.scale = copy_of(OP == kIn ? args4.s_in : args4.s_out, pe, args.stride) +
               (before + (OP == kIn && r % 32 >= 16 ? n_all : 0) + at) * ((k_all + args4.group - 1) / args4.group);
     w.x = copy_of(OP == kIn ? args.rows : (const T *)args.h, pe, args.stride) + first * k_all;
@@ -472,11 +482,12 @@ constexpr unsigned kW4LargeRows = 256;
 template <typename T, int OP, bool DMA>
 void launch_few_w4(const W4Args<T> &args, int npes, hipStream_t stream) {
     const uint64_t rows = args.e.cap < kW4FewRows ? args.e.cap : kW4FewRows;
-    const dim3 grid(div_up(OP == kIn ? args.e.hidden : args.e.dim, OP == kIn ? kFewW4Columns / 2 : kFewW4Columns),
+    constexpr unsigned threads = few_w4_waves<T>() * kLanes, columns = few_w4_waves<T>() * 32;
+    const dim3 grid(div_up(OP == kIn ? args.e.hidden : args.e.dim, OP == kIn ? columns / 2 : columns),
                     args.e.experts * div_up(rows, sizeof(T) == 4 ? 16 : 32), npes);
-    if (args.group % 128 == 0) launch_kernel((expert_few_w4_kernel<T, OP, 4, DMA>), grid, dim3(kFewW4Threads), 0, stream, args);
-    else if (args.group % 64 == 0) launch_kernel((expert_few_w4_kernel<T, OP, 2, DMA>), grid, dim3(kFewW4Threads), 0, stream, args);
-    else launch_kernel((expert_few_w4_kernel<T, OP, 1, DMA>), grid, dim3(kFewW4Threads), 0, stream, args);
+    if (args.group % 128 == 0) launch_kernel((expert_few_w4_kernel<T, OP, 4, DMA>), grid, dim3(threads), 0, stream, args);
+    else if (args.group % 64 == 0) launch_kernel((expert_few_w4_kernel<T, OP, 2, DMA>), grid, dim3(threads), 0, stream, args);
+    else launch_kernel((expert_few_w4_kernel<T, OP, 1, DMA>), grid, dim3(threads), 0, stream, args);
 }
 template <typename T, int OP, unsigned BM, bool HALVES, bool DMA>
 void launch_tiles_w4_as(const W4Args<T> &args, int npes, hipStream_t stream) {
