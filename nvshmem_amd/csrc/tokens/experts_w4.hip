@@ -332,25 +332,29 @@ struct FourBitSide {
     const unsigned char *row;  // this thread's; where it has none, a row that exists
     const T *scale;
     unsigned k_all, per_group;
-    raw held;
-    float held_scale;
+    struct Held {
+        raw q;
+        T scale;
+    };
 
-    __device__ __forceinline__ void fetch(uint64_t k) {
-        const unsigned at = (unsigned)k + threadIdx.x % 2 * kHalfK;
+    __device__ __forceinline__ Held fetch(unsigned k) const {
+        Held h;
+        const unsigned at = k + threadIdx.x % 2 * kHalfK;
         const unsigned char *p = row + at / 2;
-        held = *(const raw_unaligned *)p;  // (behind the row's end: what lies there, times zeros of A)
-        held_scale = (float)scale[__umulhi((at < k_all ? at : (unsigned)k) / 16, per_group)];
+        h.scale = scale[__umulhi((at < k_all ? at : k) / 16, per_group)];
+        h.q = *(const raw_unaligned *)p;  // (behind the row's end: what lies there, times zeros of A)
+        return h;
     }
-    __device__ __forceinline__ void land(NVSHMEM_AMD_LDS char *lds, NVSHMEM_AMD_LDS float *scales) const {
+    __device__ __forceinline__ void land(const Held &h, NVSHMEM_AMD_LDS char *lds, NVSHMEM_AMD_LDS float *scales) const {
         const unsigned r = threadIdx.x / 2, half = threadIdx.x % 2;
-        scales[half * kTileN + r] = held_scale;
+        scales[half * kTileN + r] = (float)h.scale;
 #pragma unroll
         for (unsigned j = 0; j < 4; ++j) {
             typename Chunk<T>::vec v;
 #pragma unroll
             for (unsigned i = 0; i < (unsigned)Chunk<T>::N; ++i) {
                 // (the instruction takes four bits with a sign and gives a sixteenth of them: q - 8 with its highest bit turned over)
-                const unsigned at = j * Chunk<T>::N + i, word = held[at / 8] ^ 0x88888888u;
+                const unsigned at = j * Chunk<T>::N + i, word = h.q[at / 8] ^ 0x88888888u;
                 v[i] = (T)__builtin_amdgcn_cvt_off_f32_i4((int)((at % 2 ? word >> 4 : word) >> at % 8 / 2 * 8));
             }
             *(NVSHMEM_AMD_LDS v4u *)(lds + r * kStepBytes + (((half * 4 + j) ^ (r & 7)) * 16)) = __builtin_bit_cast(v4u, v);
@@ -366,6 +370,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_w4_kernel(const W
     typedef TileSide<T, kTileN, false, true> B;  // (its layout in LDS)
     typedef FourBitSide<T> Q;
     constexpr unsigned kStepK = A::kStepK;
+    constexpr bool kAhead = BM == 128 && DMA;
     __shared__ __attribute__((aligned(1024))) char lds_a[2 * A::kBytes];
     __shared__ __attribute__((aligned(1024))) char lds_b[2 * B::kBytes];
     __shared__ __attribute__((aligned(16))) float lds_s[2 * 2 * kTileN];
@@ -402,23 +407,33 @@ __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_w4_kernel(const W
             side_b.row = copy_of(OP == kIn ? args4.w_in : args4.w_out, pe, args.stride) + n * ((k_all + 1) / 2);
             side_b.scale = copy_of(OP == kIn ? args4.s_in : args4.s_out, pe, args.stride) + n * ((k_all + args4.group - 1) / args4.group);
         }
-        const auto fetch = [&](unsigned buffer, unsigned k) {
+        const auto fetch_a = [&](unsigned buffer, unsigned k) {
             const unsigned left = k_all - k < kStepK ? k_all - k : kStepK;
-            side_b.fetch(k);
             side_a.fetch((NVSHMEM_AMD_LDS char *)lds_a + buffer * A::kBytes, wave, left, [&](unsigned) { return a + k; });
         };
         v4f acc[kMi][kNi] = {};
         const unsigned wm = wave / 4, wn = wave % 4;
-        fetch(0, 0);
+        typename Q::Held held = side_b.fetch(0), next = {};
+        fetch_a(0, 0);
+        // (tiles of 128 rows, of which there are few: weights are fetched two steps ahead)
+        if (kAhead && kStepK < k_all) next = side_b.fetch(kStepK);
         unsigned buffer = 0;
         for (unsigned k = 0; k < k_all; k += kStepK, buffer ^= 1) {
             NVSHMEM_AMD_LDS char *la = (NVSHMEM_AMD_LDS char *)lds_a + buffer * A::kBytes, *lb = (NVSHMEM_AMD_LDS char *)lds_b + buffer * B::kBytes;
             NVSHMEM_AMD_LDS float *ls = (NVSHMEM_AMD_LDS float *)lds_s + buffer * 2 * kTileN;
             side_a.land(la, wave, lane);
-            side_b.land(lb, ls);
-            asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+            side_b.land(held, lb, ls);
+            // what of A is on its way to LDS was asked for in front of the weights two steps ahead, whose last load may go on
+            if (kAhead && k + kStepK < k_all) asm volatile("s_waitcnt vmcnt(1)" : : : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
             __syncthreads();
-            if (k + kStepK < k_all) fetch(buffer ^ 1, k + kStepK);
+            if (k + kStepK < k_all) {
+                fetch_a(buffer ^ 1, k + kStepK);
+                if (!kAhead) held = side_b.fetch(k + kStepK);
+                else held = next;
+                if (kAhead && k + 2 * kStepK < k_all) next = side_b.fetch(k + 2 * kStepK);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             v4u fb[2][kNi], fa[2][2];
             v4f s[HALVES ? 2 : 1][kNi];
 #pragma unroll
