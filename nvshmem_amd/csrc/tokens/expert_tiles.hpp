@@ -8,8 +8,9 @@
 //   kDwIn    dpre[k][m]         rows[k][n]            dw_in                       k runs over the expert's rows
 //   kDwOut   dout[k][m]         h[k][n]               dw_out
 //
-// A tile of D is BM x BN, a block of eight wavefronts has one, each wavefront BM/2 x BN/4 of it in its accumulators (fp32).  A and B
-// pass through LDS in steps of 128 bytes of k, two steps in turn: while one is multiplied the other is on its way.
+// A tile of D is BM x BN, a block has one: eight wavefronts in two rows of four (four in one of 32 rows), each with BM/2 x BN/4 of it in
+// its accumulators (fp32).  A and B
+// pass through LDS in steps of 128 bytes of k, two or three in turn: while one is multiplied the others are on their way.
 #pragma once
 
 #include "token_common.hpp"
@@ -101,14 +102,16 @@ struct TileList {
     unsigned first[kMostExperts + 1];
     unsigned wave_sum[kTileWaves];
 
-    // By a whole block; two experts a thread.
+    // By a whole block of WAVES wavefronts; two experts a thread, or four.
+    template <unsigned WAVES = kTileWaves>
     __device__ __forceinline__ void make(const int64_t *expert_row, uint64_t stride, uint64_t cap, unsigned per_pe, unsigned npes, unsigned tile_rows,
                                          unsigned columns, unsigned more_than) {
         const unsigned wave = wave_of_block(), lane = threadIdx.x % kLanes, all = per_pe * npes;
-        unsigned own[2], sum = 0;
+        constexpr unsigned kEach = kMostExperts / (WAVES * kLanes);
+        unsigned own[kEach], sum = 0;
 #pragma unroll
-        for (unsigned i = 0; i < 2; ++i) {
-            const unsigned e = threadIdx.x * 2 + i;
+        for (unsigned i = 0; i < kEach; ++i) {
+            const unsigned e = threadIdx.x * kEach + i;
             uint64_t at = 0, rows = 0;
             if (e < all) expert_range(copy_of(expert_row, e / per_pe, stride), e % per_pe, cap, at, rows);
             own[i] = rows > more_than ? (unsigned)((rows + tile_rows - 1) / tile_rows) * columns : 0;
@@ -129,9 +132,12 @@ struct TileList {
         __syncthreads();
         for (unsigned w = 0; w < wave; ++w) before += wave_sum[w];
         before -= sum;
-        first[threadIdx.x * 2] = before;
-        first[threadIdx.x * 2 + 1] = before + own[0];
-        if (threadIdx.x == kTileThreads - 1) first[kMostExperts] = before + sum;
+#pragma unroll
+        for (unsigned i = 0; i < kEach; ++i) {
+            first[threadIdx.x * kEach + i] = before;
+            before += own[i];
+        }
+        if (threadIdx.x == WAVES * kLanes - 1) first[kMostExperts] = before;
         __syncthreads();
     }
     __device__ __forceinline__ unsigned total() const { return __builtin_amdgcn_readfirstlane(first[kMostExperts]); }
@@ -302,16 +308,15 @@ constexpr bool a_by_k() { return OP == kDwIn || OP == kDwOut; }
 template <int OP>
 constexpr bool b_by_k() { return OP != kIn && OP != kOut; }
 
-// The multiplication of a tile, once its first two steps are on their way (start()).  A wavefront goes through a step in groups of one
+// The multiplication of a tile, once its first STAGES steps are on their way (start()).  A wavefront goes through a step in groups of one
 // piece of A with all of its pieces of B, kAhead groups after it read the piece, so that reads of LDS and products overlap.  All of a
-// step's pieces are in registers kAhead groups before its end: there the block meets, the step after the next takes the step's place in
+// step's pieces are in registers kAhead groups before its end: there the block meets, the step STAGES further takes the step's place in
 // LDS, and what is read from there on is of the next step.  us for 131072 rows of 64 experts (7168 x 2048 bf16, kIn / kOut) with the reads left to
 // the compiler, which waits for each pair of them: 6473 / 3637.
-template <typename T, typename A, typename B, unsigned kMi, unsigned kNi>
+template <typename T, typename A, typename B, unsigned kMi, unsigned kNi, unsigned STAGES>
 struct TileProduct {
-    static constexpr unsigned kGroups = 2 * kMi, kAhead = kMi < 4 ? 1 : 2;
-    static constexpr int kMoves = A::kMoves + B::kMoves;
-    NVSHMEM_AMD_LDS char *lds_a, *lds_b;  // two steps of each
+    static constexpr unsigned kGroups = 2 * kMi, kAhead = kMi < 4 ? 1 : 2, kMoves = A::kMoves + B::kMoves;
+    NVSHMEM_AMD_LDS char *lds_a, *lds_b;  // STAGES steps of each
     unsigned wave, lane;
 
     // fetch(buffer, step): starts the step's way; land(buffer): ends it where it leads through registers.
@@ -320,13 +325,21 @@ struct TileProduct {
         if (steps == 0) return;
         fetch(0, 0);
         land(0);
-        if (steps > 1) fetch(1, 1);
+#pragma unroll
+        for (unsigned i = 1; i < STAGES; ++i)
+            if (i < steps) fetch(i, i);
+    }
+    // Until no more than `later` steps' loads are on their way (a barrier alone does not wait for what goes to LDS); all of them where
+    // the last steps' were not asked for.
+    __device__ __forceinline__ void wait(bool all_there, unsigned later) const {
+        if (STAGES > 2 && all_there && later == STAGES - 1) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((STAGES - 1) * kMoves) : "memory");
+        else if (STAGES > 2 && all_there) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((STAGES - 2) * kMoves) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
     }
     template <bool DMA, typename FETCH, typename LAND>
     __device__ __forceinline__ void run(unsigned steps, FETCH fetch, LAND land, v4f (&acc)[kMi][kNi]) const {
         if (steps == 0) return;
-        if (DMA && steps > 1) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kMoves) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+        wait(steps >= STAGES, STAGES - 1);
         __syncthreads();
         const unsigned wm = wave / 4, wn = wave % 4;
         v4u fa[2 * kAhead], fb[2][kNi];
@@ -338,19 +351,19 @@ struct TileProduct {
         for (unsigned ni = 0; ni < kNi; ++ni) read_b(0, 0, ni);
 #pragma unroll
         for (unsigned g = 0; g < kAhead; ++g) read_a(0, g);
-        for (unsigned step = 0; step < steps; ++step) {
-            const unsigned buffer = step & 1;
+        unsigned buffer = 0, other = 1;
+        for (unsigned step = 0; step < steps; ++step, buffer = other, other = other + 1 == STAGES ? 0 : other + 1) {
 #pragma unroll
             for (unsigned g = 0; g < kGroups; ++g) {
                 if (g == kGroups - kAhead) {
-                    land(buffer ^ 1);
-                    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // (a barrier alone does not wait for what is on its way to LDS)
+                    land(other);
+                    wait(step + STAGES <= steps, STAGES - 2);
                     __syncthreads();
-                    if (step + 2 < steps) fetch(buffer, step + 2);
+                    if (step + STAGES < steps) fetch(buffer, step + STAGES);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 // (behind the last step: what LDS happens to hold, unused)
-                const unsigned from = g < kGroups - kAhead ? buffer : buffer ^ 1;
+                const unsigned from = g < kGroups - kAhead ? buffer : other;
                 read_a(from, (g + kAhead) % kGroups);
                 // the other half step's pieces of B, spread over the groups in front of it
                 if (g < kMi) {
@@ -360,7 +373,7 @@ struct TileProduct {
                 } else if (g >= kGroups - kAhead) {
 #pragma unroll
                     for (unsigned ni = 0; ni < kNi; ++ni)
-                        if (ni * kAhead / kNi == g - (kGroups - kAhead)) read_b(buffer ^ 1, 0, ni);
+                        if (ni * kAhead / kNi == g - (kGroups - kAhead)) read_b(other, 0, ni);
                 }
 #pragma unroll
                 for (unsigned ni = 0; ni < kNi; ++ni) acc[g % kMi][ni] = Mma<T>::step(fb[g / kMi][ni], fa[g % (2 * kAhead)], acc[g % kMi][ni]);
@@ -370,14 +383,28 @@ struct TileProduct {
     }
 };
 
+// Wavefronts of a block lie in one or two rows of four.
+template <unsigned BM>
+constexpr unsigned tile_wave_rows() {
+    return BM == 32 ? 1 : 2;
+}
+
+// Steps of a tile in LDS.
+template <unsigned BM>
+constexpr unsigned tile_stages() {
+    return BM <= 64 ? 3 : 2;
+}
+
 template <typename T, int OP, unsigned BM, unsigned BN, bool DMA>
-__global__ __launch_bounds__(kTileThreads, 2) void expert_tile_kernel(const ExpertArgs<T> args) {
-    typedef TileSide<T, BM, a_by_k<OP>(), DMA> A;
-    typedef TileSide<T, BN, b_by_k<OP>(), DMA> B;
-    constexpr unsigned kMi = BM / 32, kNi = BN / 64, kStepK = A::kStepK;
+__global__ __launch_bounds__(tile_wave_rows<BM>() * 256, tile_wave_rows<BM>()) void expert_tile_kernel(const ExpertArgs<T> args) {
+    constexpr unsigned kWaveRows = tile_wave_rows<BM>();
+    typedef TileSide<T, BM, a_by_k<OP>(), DMA, kWaveRows * 4> A;
+    typedef TileSide<T, BN, b_by_k<OP>(), DMA, kWaveRows * 4> B;
+    constexpr unsigned kMi = BM / 16 / kWaveRows, kNi = BN / 64, kStepK = A::kStepK;
     constexpr bool kWeights = OP == kDwIn || OP == kDwOut;  // D is a weight's gradient: k runs over rows
-    __shared__ __attribute__((aligned(1024))) char lds_a[2 * A::kBytes];
-    __shared__ __attribute__((aligned(1024))) char lds_b[2 * B::kBytes];
+    constexpr unsigned kStages = DMA ? tile_stages<BM>() : 2;
+    __shared__ __attribute__((aligned(1024))) char lds_a[kStages * A::kBytes];
+    __shared__ __attribute__((aligned(1024))) char lds_b[kStages * B::kBytes];
     __shared__ TileList list;
     const unsigned wave = wave_of_block(), lane = threadIdx.x % kLanes;
     const unsigned dim = args.dim, hidden = args.hidden;
@@ -387,9 +414,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_kernel(const Expe
     const unsigned lda = OP == kIn || OP == kDh || OP == kDwOut ? dim : OP == kOut ? hidden : 2 * hidden;
     const unsigned ldb = OP == kIn || OP == kDx || OP == kDwIn ? dim : hidden;
     const unsigned high_w = (m_all + BM - 1) / BM;
-    if (!kWeights) list.make(args.expert_row, args.stride, args.cap, args.experts, args.npes, BM, wide, args.more_than);
+    if (!kWeights) list.template make<kWaveRows * 4>(args.expert_row, args.stride, args.cap, args.experts, args.npes, BM, wide, args.more_than);
     const unsigned total = kWeights ? args.experts * args.npes * high_w * wide : list.total();
-    const TileProduct<T, A, B, kMi, kNi> product = {(NVSHMEM_AMD_LDS char *)lds_a, (NVSHMEM_AMD_LDS char *)lds_b, wave, lane};
+    const TileProduct<T, A, B, kMi, kNi, kStages> product = {(NVSHMEM_AMD_LDS char *)lds_a, (NVSHMEM_AMD_LDS char *)lds_b, wave, lane};
     A side_a;
     B side_b;
     for (unsigned i = 0;; ++i) {
@@ -510,7 +537,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_kernel(const Expe
     }
 }
 
-// One block a compute unit takes tiles as long as there are any; of the smaller ones, two have room.
+// As many blocks as have room on a compute unit take tiles as long as there are any.
 inline unsigned tile_blocks(uint64_t tiles, unsigned blocks_per_cu) {
     const uint64_t most = 256 * blocks_per_cu;
     return (unsigned)((tiles < most ? tiles : most) + 7) / 8 * 8;
@@ -531,21 +558,27 @@ inline void launch_tiles_as(const ExpertArgs<T> &args, hipStream_t stream) {
     const uint64_t high = OP == kDwIn || OP == kDwOut ? args.experts * (uint64_t)div_up(OP == kDwIn ? 2 * (uint64_t)args.hidden : args.dim, BM)
                                                       : args.cap / BM + (args.experts < args.cap ? args.experts : args.cap);
     const uint64_t tiles = high * wide * args.npes;
-    if (tiles) launch_kernel((expert_tile_kernel<T, OP, BM, BN, DMA>), dim3(tile_blocks(tiles, BN == 128 ? BM == 64 ? 3 : 2 : 1)), dim3(kTileThreads), 0, stream, args);
+    if (tiles) launch_kernel((expert_tile_kernel<T, OP, BM, BN, DMA>), dim3(tile_blocks(tiles, BN == 256 ? 1 : DMA || BM == 128 ? 2 : 3)), dim3(tile_wave_rows<BM>() * 256), 0, stream, args);
 }
-// Large tiles read the least and overlap the best within a tile, small ones waste less on experts of few rows and let one block of a compute
-// unit multiply while another stores.  What an expert may have on average, `rows`, is all that the host knows of the rows.
-// us of the forward pass, 256 x 256 / 128 x 128 / 64 x 128: bf16, 64 experts of 2048 x 1408 with 48 rows each 329 / 284 / 294, 100: 343 / 330 / 352, 300: 504 /
-// 519 / 612, 600: 754 / 821 / 1045; 32 of 7168 x 2048 with 48: 741 / 661 / 606, 300: 1148 / 1159 / 1479, 600: 1776 / 1971 / 2592.  fp32, 16 experts of 2048 x
-// 1408 with 48 rows 901 / 435 / 283, 180: 831 / 672 / 572, 600: 1648 / 1494 / 1401.  Tiles of 128 x 256 and 64 x 256 were not ahead of these anywhere.
+// Large tiles read the least, small ones waste less on experts of few rows, have more steps on their way to LDS at a time, and two blocks of
+// a compute unit, of which one multiplies while the other stores.  What an expert may have on average, `rows`, is all that the host knows
+// of the rows.  us of the forward pass, 256 x 256 / 128 x 128 / 64 x 128 / 32 x 128:
+//   bf16, 64 experts of 4096 x 1536 with 12 rows each - / 436 / 414 / 454, 40: - / 461 / 468 / 548; 57 rows for 64 experts of 7168 x 2048 - / 652 / 630 / 612;
+//   8 rows for 8 experts of 2048 x 1408, too few for the larger tiles to fill the GPU: - / 41.8 / 28.2 / 26.9;
+//   64 experts of 2048 x 1408 with 300 rows each 504 / 519, 600: 754 / 821; 32 of 7168 x 2048 with 180: 880 / 862, 600: 1776 / 1971.
+//   fp32, 16 rows for 64 experts of 4096 x 1536 - / 671 / 370 / 218; 16 of 2048 x 1408 with 180 rows each 831 / 672 / 572, 600: 1648 / 1494 / 1401.
+// A kernel without LDS for few rows, whose wavefronts split k, took 39 in the smallest of these and 501 in the first.
 template <typename T, int OP, bool DMA>
 inline void launch_expert_tiles(const ExpertArgs<T> &args, hipStream_t stream) {
     constexpr bool kWeights = OP == kDwIn || OP == kDwOut;
     const uint64_t rows = (args.cap + args.experts - 1) / args.experts;
     if constexpr (DMA && sizeof(T) == 2)
         if (rows > 448 && tiles_of<T, OP>(args, 256, 256) >= 256) return launch_tiles_as<T, OP, 256, 256, DMA>(args, stream);
-    if constexpr (!kWeights)
-        if (sizeof(T) == 4 || rows <= 80 || tiles_of<T, OP>(args, 128, 128) < 256) return launch_tiles_as<T, OP, 64, 128, DMA>(args, stream);
+    if constexpr (!kWeights) {
+        const bool many = tiles_of<T, OP>(args, 128, 128) >= 256;
+        if (rows <= 12 || ((sizeof(T) == 4 || !many) && rows <= 40)) return launch_tiles_as<T, OP, 32, 128, DMA>(args, stream);
+        if (sizeof(T) == 4 || !many || rows <= 32) return launch_tiles_as<T, OP, 64, 128, DMA>(args, stream);
+    }
     launch_tiles_as<T, OP, 128, 128, DMA>(args, stream);
 }
 

@@ -4,20 +4,11 @@
 //
 // for the rows [expert_row[i], expert_row[i + 1]) of expert i.  Both input projections, the activation and the product are one
 // kernel; h goes through memory in the rows' type, rounded once, and is what the second kernel reads.
-#include "expert_few.hpp"
+#include "expert_tiles.hpp"
 
 namespace nvshmem_amd {
 namespace tokens {
 namespace {
-
-// Which experts have few rows is known on the GPU only, so both kernels start: a block that finds its expert to be the other's ends.
-template <typename T, int OP>
-void launch_experts(const ExpertArgs<T> &args, bool whole, int npes, hipStream_t stream) {
-    launch_kernel((expert_few_kernel<T, OP>), few_rows_grid<OP>(args, npes), dim3(kFewThreads), 0, stream, args);
-    if (args.cap <= kFewRows) return;
-    if (whole) launch_expert_tiles<T, OP, true>(args, stream);
-    else launch_expert_tiles<T, OP, false>(args, stream);
-}
 
 template <typename API>
 int experts_on_stream(API *out, API *pre, void *workspace, const API *rows, const API *w_in, const API *w_out,
@@ -45,9 +36,13 @@ int experts_on_stream(API *out, API *pre, void *workspace, const API *rows, cons
     // (the slices' stride is a multiple of 2 MiB, so that every PE's copies are aligned like PE 0's)
     const bool whole = dim * sizeof(T) % 16 == 0 && hidden * sizeof(T) % 16 == 0 && aligned16(args.rows) && aligned16(args.w_in) &&
                        aligned16(args.w_out);
-    args.more_than = kFewRows;
-    launch_experts<T, kIn>(args, whole, rt.npes, stream);
-    launch_experts<T, kOut>(args, whole, rt.npes, stream);
+    if (whole) {
+        launch_expert_tiles<T, kIn, true>(args, stream);
+        launch_expert_tiles<T, kOut, true>(args, stream);
+    } else {
+        launch_expert_tiles<T, kIn, false>(args, stream);
+        launch_expert_tiles<T, kOut, false>(args, stream);
+    }
     return launched("moe_experts");
 }
 

@@ -3,7 +3,7 @@
 //   pre = [gate | up] = x W_in^T      h = gate * sigmoid(gate) * up      out = h W_out^T
 //
 // The matrix cores get x and the whole numbers q exactly; what a group adds up to is multiplied with its scale in fp32.
-#include "expert_few.hpp"
+#include "expert_tiles.hpp"
 
 namespace nvshmem_amd {
 namespace tokens {
