@@ -90,7 +90,7 @@ int dropout_on_stream(API *out, const API *rows, const API *residual, const uint
     T *y = (T *)ops.out("out", out, elems);
     if (!ops.ok()) return NVSHMEMX_ERROR_INVALID_VALUE;
     if (elems == 0) return 0;
-    const uint64_t blocks = (elems + 8 * 256 - 1) / (8 * 256), most = 1u << 20;
+    const uint64_t blocks = (elems + 8 * 256 - 1) / (8 * 256), most = (1u << 23) / (unsigned)rt.npes;  // (a launch holds fewer than 2^32 threads)
     launch_kernel(dropout_kernel<T>, dim3((unsigned)(blocks < most ? blocks : most), 1, rt.npes), dim3(256), 0, stream, y, x, r, s,
                   rt.heap_size, elems, limit, (float)(65536.0 / (65536.0 - limit)));
     return launched("dropout");

@@ -179,3 +179,17 @@ def test_equal_inputs_give_equal_bits():
         first = check_forward(rt, new, c, False)
         for _ in range(3):
             assert np.array_equal(check_forward(rt, new, c, False), first, equal_nan=True)
+
+
+# Experts of so many rows that every product takes the largest tiles (test_expert_calls.py holds them to that).
+LARGE = dict(npes=2, mine=16, cap=16 * 460, dim=776, hidden=776)
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "half"])
+def test_largest_tiles(kind):
+    rng = np.random.default_rng(12)
+    with runtime(LARGE["npes"], 512 << 20) as rt, Arrays(rt) as new:
+        sizes = [1000, 700, 3, 0, 257, 500, 512, 700, 460, 461, 600, 300, 256, 900, 127, 553]
+        c = Case(new, rng, kind, expert_row=starts(LARGE["npes"], LARGE["mine"], LARGE["cap"], sizes, rng, 5), **LARGE)
+        check_forward(rt, new, c, True)
+        check_backward(rt, new, c)

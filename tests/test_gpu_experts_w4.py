@@ -79,6 +79,15 @@ def test_operands_on_any_element(kind, shift):
         check(rt, new, rng, kind, mine, cap, dim, hidden, 128, starts(npes, mine, cap, [70, 5, 40], rng, 2), shift)
 
 
+@pytest.mark.parametrize("kind", ["bfloat16", "half"])
+@pytest.mark.parametrize("group", [32, 64])
+def test_tiles_of_256_rows(kind, group):
+    npes, mine, dim, hidden = 2, 3, 776, 328
+    rng = np.random.default_rng(group)
+    with runtime(npes, 128 << 20) as rt, Arrays(rt) as new:
+        check(rt, new, rng, kind, mine, 960, dim, hidden, group, starts(npes, mine, 960, [500, 257, 190], rng, 4))
+
+
 @pytest.mark.parametrize("npes,mine", [(1, 1), (1, 130), (16, 2), (64, 1)])
 def test_numbers_of_pes_and_experts(npes, mine):
     cap, dim, hidden = 200, 48, 40
