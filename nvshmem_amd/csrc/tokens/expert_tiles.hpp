@@ -576,7 +576,8 @@ inline void launch_expert_tiles(const ExpertArgs<T> &args, hipStream_t stream) {
         if (rows > 448 && tiles_of<T, OP>(args, 256, 256) >= 256) return launch_tiles_as<T, OP, 256, 256, DMA>(args, stream);
     if constexpr (!kWeights) {
         const bool many = tiles_of<T, OP>(args, 128, 128) >= 256;
-        if (rows <= 12 || ((sizeof(T) == 4 || !many) && rows <= 40)) return launch_tiles_as<T, OP, 32, 128, DMA>(args, stream);
+        if (rows <= 12 || ((sizeof(T) == 4 || !many) && (rows <= 40 || tiles_of<T, OP>(args, 64, 128) < 256)))
+            return launch_tiles_as<T, OP, 32, 128, DMA>(args, stream);
         if (sizeof(T) == 4 || !many || rows <= 32) return launch_tiles_as<T, OP, 64, 128, DMA>(args, stream);
     }
     launch_tiles_as<T, OP, 128, 128, DMA>(args, stream);
