@@ -290,15 +290,13 @@ __device__ __forceinline__ void store_32(T *row, unsigned c, v4f lo, v4f hi, uns
     }
 }
 template <typename T>
-__device__ __forceinline__ v4f load_four(const T *p, unsigned n) {
-    typedef T four __attribute__((ext_vector_type(4)));
-    typedef four four_unaligned __attribute__((aligned(sizeof(T))));
-    if (n >= 4) return __builtin_convertvector(*(const four_unaligned *)p, v4f);
-    v4f v = {};
-#pragma unroll
-    for (unsigned i = 0; i < 3; ++i)
-        if (i < n) v[i] = (float)p[i];
-    return v;
+struct Four {
+    typedef T vec __attribute__((ext_vector_type(4)));
+    typedef vec vec_unaligned __attribute__((aligned(sizeof(T))));
+};
+template <typename T>
+__device__ __forceinline__ v4f as_float(typename Four<T>::vec v) {
+    return __builtin_convertvector(v, v4f);
 }
 // 1 / (1 + exp(-x)); exp overflows to an infinity, whose reciprocal is 0.
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
@@ -474,9 +472,24 @@ __global__ __launch_bounds__(tile_wave_rows<BM>() * 256, tile_wave_rows<BM>()) v
         product.template run<DMA>(steps, fetch, land, acc);
         // A lane has four consecutive columns of row lane % 16 of each 16 x 16 piece.
         const unsigned r = lane % 16, g = lane / 16;
+        // kDh: gate and up of the next 16 rows are on their way while these are worked on
+        typename Four<T>::vec pre[2][2][kNi];
+        const auto load_pre = [&](unsigned mi) {
+            const unsigned m = (wm * kMi + mi) * 16 + r;
+            const T *from = copy_of(args.pre_in, pe, args.stride) + (first + m0 + (m < m_here ? m : m_here - 1)) * 2 * hidden + n0;
+#pragma unroll
+            for (unsigned ni = 0; ni < kNi; ++ni) {
+                // (behind the last column: what lies there, unused)
+                const unsigned at = wn * (BN / 4) + ni * 16 + g * 4, there = at < n_here ? at : n_here - 1;
+                pre[mi % 2][0][ni] = *(const typename Four<T>::vec_unaligned *)(from + there);
+                pre[mi % 2][1][ni] = *(const typename Four<T>::vec_unaligned *)(from + hidden + there);
+            }
+        };
+        if (OP == kDh) load_pre(0);
 #pragma unroll
         for (unsigned mi = 0; mi < kMi; ++mi) {
             const unsigned m = (wm * kMi + mi) * 16 + r;
+            if (OP == kDh && mi + 1 < kMi) load_pre(mi + 1);
             if (m >= m_here) continue;
             const uint64_t row = kWeights ? m0 + m : first + m0 + m;
             if (OP == kIn) {
@@ -508,12 +521,10 @@ __global__ __launch_bounds__(tile_wave_rows<BM>() * 256, tile_wave_rows<BM>()) v
             for (unsigned ni = 0; ni < kNi; ni += 2) {
                 const unsigned c = wn * (BN / 4) + ni * 16;
                 if (OP == kDh) {
-                    const T *pre = copy_of(args.pre_in, pe, args.stride) + row * 2 * hidden + n0;
                     v4f dgate[2], dup[2], h[2];
 #pragma unroll
                     for (unsigned half = 0; half < 2; ++half) {
-                        const unsigned at = c + half * 16 + g * 4, there = at < n_here ? n_here - at : 0;
-                        const v4f gate = load_four(pre + at, there), up = load_four(pre + hidden + at, there), dh = acc[mi][ni + half];
+                        const v4f gate = as_float<T>(pre[mi % 2][0][ni + half]), up = as_float<T>(pre[mi % 2][1][ni + half]), dh = acc[mi][ni + half];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float s = sigmoid(gate[i]), silu = gate[i] * s;
