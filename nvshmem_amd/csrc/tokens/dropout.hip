@@ -26,7 +26,9 @@ __device__ __forceinline__ v4u philox(uint64_t block, uint64_t second, uint64_t 
     return v4u{c0, c1, c2, c3};
 }
 
-// The two or one chunks of 16 bytes that eight elements are.
+// A lane has eight elements, one block of the generator, in one or two chunks of 16 bytes.  16 bits an element, as 32 would have the generator run
+// twice as often (ten rounds of two products, 28 operations an element): the vector unit, not memory, would bound it.  Bound by memory: 8 x 4096 rows
+// of 7168 bf16 and a residual (1.41 GB) take 217 us, 6.5 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void dropout_kernel(T *out, const T *rows, const T *residual, const uint64_t *seed, uint64_t stride,
                                                       uint64_t elems, unsigned limit, float scale) {

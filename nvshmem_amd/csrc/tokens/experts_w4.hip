@@ -106,13 +106,15 @@ struct words<4> {
     typedef v4u type;
 };
 
-// A block has 32 rows of one expert's weights for each of its wavefronts, and up to 32 rows of x.  It goes over k in chunks of 256: weights go to LDS as
-// they are, whole lines of memory (128 bytes of a row) at a time; x goes there in the order that the matrix cores take (fp32: as three
-// parts), and the rows' scales.  While a chunk is multiplied the next is on its way.
+// A block has 32 rows of one expert's weights for each of its wavefronts, and up to 32 rows of x (fp32: 16).  It goes over k in chunks of 256:
+// weights go to LDS as they are, whole lines of memory (128 bytes of a row) at a time; x goes there in the order that the matrix cores take
+// (fp32: as three parts), and the rows' scales.  While a chunk is multiplied the next is on its way.
 // Within a chunk a step is 32 * WORDS k, all of one group: lane (r, g) has of each of two groups of 16 rows 4 * WORDS bytes, 8 * WORDS
 // consecutive k of row r.  WORDS is 4 where the group is a multiple of 128, else 2 or 1.
-
-
+// Bound by reading the weights, at 5 TB/s, and by what the vector unit does for them.  us for one token on each of 8 PEs, 256 experts of 7168 x 2048,
+// bf16, groups of 128 (1.3 GB), and for 64 tokens a PE (5.9 GB): 225 and 1440; with weights read into registers, 16 to 64 bytes of a row at a time, 564
+// and 3900 (the lines came from memory up to four times); with two blocks a compute unit and x of two chunks in LDS 238 and 1530, with blocks of
+// eight wavefronts 307 and 1730; with three operations for two weights instead of one 253 and 1690.
 // Wavefronts of a block.  A few small blocks to a compute unit wait for memory apart from each other; only of fp32 elements, whose three
 // parts fill LDS, eight wavefronts share one x.
 template <typename T>
@@ -277,7 +279,7 @@ __device__ __forceinline__ void few_w4_store(const ExpertArgs<T> &args, const v4
     }
 }
 
-// An expert of up to `more_than` rows has a block for each 32 of them, which reads the weights again.
+// An expert of up to `more_than` rows has a block for each 32 (16) of them, which reads the weights again.
 template <typename T, int OP, unsigned WORDS, bool DMA>
 __global__ __launch_bounds__(few_w4_waves<T>() * kLanes, sizeof(T) == 4 ? 2 : 3) void expert_few_w4_kernel(const W4Args<T> args4) {
     typedef FewFourBits<T, WORDS, DMA> W;
@@ -362,7 +364,10 @@ struct FourBitSide {
     }
 };
 
-// HALVES: the halves of a step may be of two groups.
+// HALVES: the halves of a step may be of two groups.  Bound by the vector unit: it makes q - 8 of a block's weights once for BM rows, and for each
+// product of the matrix cores multiplies four sums with their scales (HALVES; two otherwise), which takes as long as the product.  us for 32768 rows of 64
+// experts of 7168 x 2048, groups of 32: 3970 with BM of 256 (0.73 PFLOP/s); with weights fetched behind the products' start 5040, with BM of 128
+// before that 7780.
 template <typename T, int OP, unsigned BM, bool HALVES, bool DMA>
 __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_w4_kernel(const W4Args<T> args4) {
     constexpr unsigned kMi = BM / 32, kNi = 4;
@@ -391,9 +396,10 @@ __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_w4_kernel(const W
         expert_range(copy_of(args.expert_row, pe, args.stride), e, args.cap, first, rows);
         first = scalar64(first), rows = scalar64(rows);
         unsigned tm, tn;
-        tile_place(t, (unsigned)((rows + BM - 1) / BM), wide, tm, tn);
+        const uint64_t high = (rows + BM - 1) / BM;
+        if (t >= high * wide) continue;  // (a table whose ranges overlap many times over may count past 2^32)
+        tile_place(t, (unsigned)high, wide, tm, tn);
         const uint64_t m0 = (uint64_t)tm * BM;
-        if (m0 >= rows) continue;  // (a table whose ranges overlap many times over may count past 2^32)
         const unsigned n0 = tn * n_tile, m_here = rows - m0 < BM ? (unsigned)(rows - m0) : BM;
         const unsigned n_here = n_all - n0 < n_tile ? n_all - n0 : n_tile;
         const T *a = copy_of(OP == kIn ? args.rows : (const T *)args.h, pe, args.stride) + (first + m0) * k_all;
@@ -489,9 +495,11 @@ __global__ __launch_bounds__(kTileThreads, 2) void expert_tile_w4_kernel(const W
     }
 }
 
-// Experts of more rows are the tiles'.
+// Experts of more rows are the tiles'.  us with 64 / 128 here: 64 tokens on each of 8 PEs, 256 experts of 7168 x 2048, 1560 / 1660; 128 rows each for 64
+// experts of 4096 x 1536 820 / 780; a step of four tokens that no expert can have more than 74 rows of 16.4 / 11.3 (no launch of tiles).
 constexpr unsigned kW4FewRows = 64;
-// ... and those of 256 rows where experts have more than this on average at most: weights are made ready half as often.
+// ... and those of 256 rows where experts have more than this on average at most: weights are made ready half as often.  us with 128 / 256 rows, 64
+// experts of 4096 x 1536 with 100 rows each 531 / -, 200: 883 / 869, 400: 1512 / 1276, 800: 2665 / 2303.
 constexpr unsigned kW4LargeRows = 256;
 
 template <typename T, int OP, bool DMA>

@@ -85,7 +85,8 @@ def four_bits(packed, scale, k, group):
 
 def forward_four_bits(x, w_in, s_in, w_out, s_out, kind):
     """forward() where a sum goes over 16 + q and takes 24 back: its magnitudes are those of 55 times the scales `s`, expanded like the
-    weights.  That are 2 n additions; those of an fp32 element's second and third part are of 2^-8 of the first's magnitude."""
+    weights.  That are 2 n additions; those of an fp32 element's second and third part are of 2^-8 of the first's magnitude.  (Sums over
+    another power of two plus q are of larger magnitudes; they are held to this all the same.)"""
     hidden = w_out.shape[1]
 
     def product4(a, da, w, s):
