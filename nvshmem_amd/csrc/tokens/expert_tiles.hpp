@@ -321,6 +321,7 @@ constexpr bool b_by_k() { return OP != kIn && OP != kOut; }
 template <typename T, typename A, typename B, unsigned kMi, unsigned kNi, unsigned STAGES>
 struct TileProduct {
     static constexpr unsigned kGroups = 2 * kMi, kAhead = kMi < 4 ? 1 : 2, kMoves = A::kMoves + B::kMoves;
+    static constexpr unsigned kAlone = 256 / A::kStepK;  // steps
     NVSHMEM_AMD_LDS char *lds_a, *lds_b;  // STAGES steps of each
     unsigned wave, lane;
 
@@ -357,7 +358,16 @@ struct TileProduct {
 #pragma unroll
         for (unsigned g = 0; g < kAhead; ++g) read_a(0, g);
         unsigned buffer = 0, other = 1;
+        // Of fp32 elements, whose results are rounded no further, products of 256 k are added up by themselves: a sum of thousands in a row
+        // would lose a bit or two more (relative to 64 bits, of 3918: 1.3e-6 in a row, 5e-7 so; and 7.5e-7 in PyTorch).
+        v4f all[sizeof(T) == 4 ? kMi : 1][kNi] = {};
         for (unsigned step = 0; step < steps; ++step, buffer = other, other = other + 1 == STAGES ? 0 : other + 1) {
+            if (sizeof(T) == 4 && step && step % kAlone == 0) {
+#pragma unroll
+                for (unsigned mi = 0; mi < kMi; ++mi)
+#pragma unroll
+                    for (unsigned ni = 0; ni < kNi; ++ni) all[mi % (sizeof(T) == 4 ? kMi : 1)][ni] += acc[mi][ni], acc[mi][ni] = v4f{};
+            }
 #pragma unroll
             for (unsigned g = 0; g < kGroups; ++g) {
                 if (g == kGroups - kAhead) {
@@ -385,6 +395,12 @@ struct TileProduct {
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
+        if (sizeof(T) == 4) {
+#pragma unroll
+            for (unsigned mi = 0; mi < kMi; ++mi)
+#pragma unroll
+                for (unsigned ni = 0; ni < kNi; ++ni) acc[mi][ni] += all[mi % (sizeof(T) == 4 ? kMi : 1)][ni];
+        }
     }
 };
 
@@ -401,7 +417,7 @@ constexpr unsigned tile_stages() {
 }
 
 template <typename T, int OP, unsigned BM, unsigned BN, bool DMA>
-__global__ __launch_bounds__(tile_wave_rows<BM>() * 256, tile_wave_rows<BM>()) void expert_tile_kernel(const ExpertArgs<T> args) {
+__global__ __launch_bounds__(tile_wave_rows<BM>() * 256, tile_wave_rows<BM>() * (sizeof(T) == 4 && BM == 128 && DMA ? 2 : 1)) void expert_tile_kernel(const ExpertArgs<T> args) {
     constexpr unsigned kWaveRows = tile_wave_rows<BM>();
     typedef TileSide<T, BM, a_by_k<OP>(), DMA, kWaveRows * 4> A;
     typedef TileSide<T, BN, b_by_k<OP>(), DMA, kWaveRows * 4> B;
