@@ -615,7 +615,7 @@ inline void launch_expert_tiles(const ExpertArgs<T> &args, hipStream_t stream) {
             return launch_tiles_as<T, OP, 32, 128, DMA>(args, stream);
         if (sizeof(T) == 4 || !many || rows <= 32) return launch_tiles_as<T, OP, 64, 128, DMA>(args, stream);
     }
-    launch_tiles_as<T, OP, 128, 128, DMA>(args, stream);
+    if constexpr (kWeights || sizeof(T) == 2) launch_tiles_as<T, OP, 128, 128, DMA>(args, stream);
 }
 
 // Products of one PE's experts may be at most so wide and high; their offsets inside a tile stay under 2^31 bytes.

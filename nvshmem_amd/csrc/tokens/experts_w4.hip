@@ -521,9 +521,10 @@ void launch_tiles_w4_as(const W4Args<T> &args, int npes, hipStream_t stream) {
 template <typename T, int OP, bool HALVES>
 void launch_tiles_w4(const W4Args<T> &args, bool whole, int npes, hipStream_t stream) {
     const uint64_t rows = (args.e.cap + args.e.experts - 1) / args.e.experts;
-    if (!whole) launch_tiles_w4_as<T, OP, 128, HALVES, false>(args, npes, stream);
-    else if (sizeof(T) == 2 && rows > kW4LargeRows) launch_tiles_w4_as<T, OP, 256, HALVES, true>(args, npes, stream);
-    else launch_tiles_w4_as<T, OP, 128, HALVES, true>(args, npes, stream);
+    if (!whole) return launch_tiles_w4_as<T, OP, 128, HALVES, false>(args, npes, stream);
+    if constexpr (sizeof(T) == 2)
+        if (rows > kW4LargeRows) return launch_tiles_w4_as<T, OP, 256, HALVES, true>(args, npes, stream);
+    launch_tiles_w4_as<T, OP, 128, HALVES, true>(args, npes, stream);
 }
 template <typename T, int OP>
 void launch_w4(const W4Args<T> &args, bool whole, int npes, hipStream_t stream) {
@@ -531,8 +532,9 @@ void launch_w4(const W4Args<T> &args, bool whole, int npes, hipStream_t stream) 
     if (row_bytes % 16 == 0 && aligned16(OP == kIn ? args.w_in : args.w_out)) launch_few_w4<T, OP, true>(args, npes, stream);
     else launch_few_w4<T, OP, false>(args, npes, stream);
     if (args.e.cap <= kW4FewRows) return;
-    if (sizeof(T) == 2 && args.group % 64) launch_tiles_w4<T, OP, true>(args, whole, npes, stream);
-    else launch_tiles_w4<T, OP, false>(args, whole, npes, stream);
+    if constexpr (sizeof(T) == 2)
+        if (args.group % 64) return launch_tiles_w4<T, OP, true>(args, whole, npes, stream);
+    launch_tiles_w4<T, OP, false>(args, whole, npes, stream);
 }
 
 template <typename API>
