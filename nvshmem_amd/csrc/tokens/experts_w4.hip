@@ -19,23 +19,23 @@ struct W4Args {
 
 // ---- experts of few rows ----
 
-// What x and a weight become for the matrix cores.  Of 16-bit elements a weight is a power of two plus q, whose bits are those of the power
-// with q in the mantissa: one operation for two weights.  What that is too much, times the sum of x, goes into the sums first as a product
-// with too_much().  The sums are in fp32, so that what they lose by it is far below what the result is rounded to.  An fp32 element is the
-// sum of three bf16 ones, of 8 bits of its mantissa each, and weights are q - 8: nothing of it is lost in front of the sum.
+// What x and a weight become for the matrix cores.  Of bfloat16 elements a weight is 128 + q, whose bits are those of 128 with q in the
+// mantissa: one operation for two weights.  The 136 that this is too much, times the sum of x, goes into the sums first, as a product with
+// too_much(); what the sums, in fp32, lose by it is some 2^-16 of the result where a row's elements are of one sign, and less where they are
+// not, far below the 2^-8 that the result is rounded to.  For a half, whose results have eight times the steps and whose bits would need 1024 in
+// 128's place, that does not hold: 1024 + q (64 + q of the next four bits) loses the 1032 (72) by one more operation for two weights, exactly.
+// An fp32 element is the sum of three bf16 ones, of 8 bits of its mantissa each, and weights are q - 8: nothing of it is lost in front of
+// the sum.  us of 64 tokens on each of 8 PEs, halves, 256 experts of 7168 x 2048, groups of 64, by products with the 1032 and 72 and now: 1618 / 1641.
 template <typename T>
 struct Nibble;
 template <>
 struct Nibble<__bf16> {
     typedef __bf16 type;
-    // 128 + q, and 136 to take back
     static __device__ __forceinline__ v4u too_much() { return v4u{0xC308C308u, 0xC308C308u, 0xC308C308u, 0xC308C308u}; }
 };
 template <>
 struct Nibble<_Float16> {
     typedef _Float16 type;
-    // 1024 + q where q is the lowest four bits of a half, 64 + q where it is the next four: 1032 and 72 to take back
-    static __device__ __forceinline__ v4u too_much() { return v4u{0xE408E408u, 0xD480D480u, 0xE408E408u, 0xD480D480u}; }
 };
 template <>
 struct Nibble<float> : Nibble<__bf16> {};
@@ -55,11 +55,13 @@ __device__ __forceinline__ v4u eight_weights(unsigned q) {
         return v;
     }
     // (constants that the compiler does not see through stay in registers, where an "and" and an "or" are one instruction)
-    unsigned low = 0x000F000Fu, next = 0x00F000F0u, base = sizeof(T) == 4 ? 0 : __is_same(T, _Float16) ? 0x64006400u : 0x43004300u, base_next = 0x54005400u;
+    unsigned low = 0x000F000Fu, next = 0x00F000F0u, base = __is_same(T, _Float16) ? 0x64006400u : 0x43004300u, base_next = 0x54005400u;
     asm("" : "+v"(base), "+v"(base_next));
     if (__is_same(T, _Float16)) {
+        typedef _Float16 two __attribute__((ext_vector_type(2)));
         const unsigned upper = q >> 8;
-        return v4u{(q & low) | base, (q & next) | base_next, (upper & low) | base, (upper & next) | base_next};
+        const auto less = [](unsigned w, float by) { return __builtin_bit_cast(unsigned, __builtin_bit_cast(two, w) - two{(_Float16)by, (_Float16)by}); };
+        return v4u{less((q & low) | base, 1032), less((q & next) | base_next, 72), less((upper & low) | base, 1032), less((upper & next) | base_next, 72)};
     }
 #pragma unroll
     for (unsigned j = 0; j < 4; ++j) v[j] = (q >> j * 4 & low) | base;
@@ -200,7 +202,7 @@ struct FewFourBits {
                 for (unsigned q = 0; q < kParts; ++q) {
                     const unsigned chunk = (j * 4 + g) * WORDS + i;
                     a[mi][i][q] = *(NVSHMEM_AMD_LDS const v4u *)(lds_x + ((q * MT + mi) * 16 + r) * kRowBytes + (chunk ^ (r & 7)) * 16);
-                    if (sizeof(T) == 2) sum[mi] = Mma<M>::step(Nibble<T>::too_much(), a[mi][i][q], sum[mi]);
+                    if constexpr (__is_same(T, __bf16)) sum[mi] = Mma<M>::step(Nibble<T>::too_much(), a[mi][i][q], sum[mi]);
                 }
 #pragma unroll
         for (unsigned ni = 0; ni < 2; ++ni) {
