@@ -390,7 +390,8 @@ NVSHMEMI_REPT_FOR_ALL_REDUCE_TYPES_AND_OPS(NVSHMEMI_DECL_TYPED_REDUCE_HOST)
  * <T>_moe_experts_w4: moe_experts with weights of 4 bits.  Element k of a row of w_in (of 2 hidden rows of dim) and w_out (dim rows of hidden)
  *   is (q - 8) * scale[row][k / group], q in the low half of byte k / 2 of the row for even k, in the high half for odd ones; rows are
  *   ceil(elements / 2) bytes and ceil(elements / group) scales of T long.  group is a multiple of 32.  The weights' values are taken as they
- *   are, without rounding to T.  A row of `rows` with an infinity, or with bfloat16 elements from 2^119 on, gives NaN.  The workspace is
+ *   are, without rounding to T.  Up to 128 products are added up in front of their scale, sixteenths of them in fp32: a row whose elements (or
+ *   its h's) reach 2^121 may give infinities and NaN where the formula does not.  An infinity gives what the formula gives.  The workspace is
  *   moe_experts'.
  * <T>_dropout: out[e] = residual[e] + (keep(e) ? rows[e] / (1 - P) : 0) over the tokens * dim elements of a PE (residual NULL: zeros), with P
  *   the probability p, 0 <= p < 1, in steps of 2^-16.  keep follows from seed[0], seed[1] (the PE's own copy, e.g. a run's seed and a step's

@@ -24,7 +24,7 @@ struct W4Args {
 // too_much(); what the sums, in fp32, lose by it is some 2^-16 of the result where a row's elements are of one sign, and less where they are
 // not, far below the 2^-8 that the result is rounded to.  For a half, whose results have eight times the steps and whose bits would need 1024 in
 // 128's place, that does not hold: 1024 + q (64 + q of the next four bits) loses the 1032 (72) by one more operation for two weights, exactly.
-// An fp32 element is the sum of three bf16 ones, of 8 bits of its mantissa each, and weights are q - 8: nothing of it is lost in front of
+// An fp32 element is the sum of three bf16 ones, of 8 bits of its mantissa each, and weights are (q - 8) / 16: nothing of it is lost in front of
 // the sum.  us of 64 tokens on each of 8 PEs, halves, 256 experts of 7168 x 2048, groups of 64, by products with the 1032 and 72 and now: 1618 / 1641.
 template <typename T>
 struct Nibble;
@@ -40,17 +40,17 @@ struct Nibble<_Float16> {
 template <>
 struct Nibble<float> : Nibble<__bf16> {};
 
-// Eight weights, k in the order 0 4 1 5 2 6 3 7.
-template <typename T>
+// Eight weights, k in the order 0 4 1 5 2 6 3 7.  SIXTEENTHS: (q - 8) / 16, as the tiles take them, so that sums of 128 elements under 2^121 stay in fp32.
+template <typename T, bool SIXTEENTHS>
 __device__ __forceinline__ v4u eight_weights(unsigned q) {
     v4u v;
-    if (sizeof(T) == 4) {
-        const unsigned even = q & 0x0F0F0F0Fu, odd = q >> 4 & 0x0F0F0F0Fu;
+    if (SIXTEENTHS) {
+        const unsigned even = q ^ 0x88888888u, odd = even >> 4;
 #pragma unroll
         for (unsigned j = 0; j < 4; ++j) {
             const unsigned from = j % 2 ? odd : even;
-            const float a = (float)(from >> j / 2 * 8 & 255) - 8.0f, b = (float)(from >> (j / 2 * 8 + 16) & 255) - 8.0f;
-            v[j] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);  // (small whole numbers: bf16 is their upper half)
+            const float a = __builtin_amdgcn_cvt_off_f32_i4((int)(from >> j / 2 * 8)), b = __builtin_amdgcn_cvt_off_f32_i4((int)(from >> (j / 2 * 8 + 16)));
+            v[j] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);  // (few bits: bf16 is their upper half)
         }
         return v;
     }
@@ -188,7 +188,7 @@ struct FewFourBits {
             lds_s[(threadIdx.x / kColumns * (kSteps / 2) + j) * kColumns + threadIdx.x % kColumns] = (float)h.scale[j];
     }
     // D = w x^T: element i of a lane is row lane / 16 * 4 + i of the weights' 16, column lane % 16: a row of x.
-    template <int MT>
+    template <bool SIXTEENTHS, int MT>
     __device__ __forceinline__ void multiply(unsigned j, NVSHMEM_AMD_LDS const char *lds_w, NVSHMEM_AMD_LDS const char *lds_x,
                                              NVSHMEM_AMD_LDS const float *lds_s, unsigned wave, unsigned lane, v4f (&acc)[MT][2]) const {
         const unsigned r = lane % 16, g = lane / 16;
@@ -202,7 +202,7 @@ struct FewFourBits {
                 for (unsigned q = 0; q < kParts; ++q) {
                     const unsigned chunk = (j * 4 + g) * WORDS + i;
                     a[mi][i][q] = *(NVSHMEM_AMD_LDS const v4u *)(lds_x + ((q * MT + mi) * 16 + r) * kRowBytes + (chunk ^ (r & 7)) * 16);
-                    if constexpr (__is_same(T, __bf16)) sum[mi] = Mma<M>::step(Nibble<T>::too_much(), a[mi][i][q], sum[mi]);
+                    if constexpr (__is_same(T, __bf16) && !SIXTEENTHS) sum[mi] = Mma<M>::step(Nibble<T>::too_much(), a[mi][i][q], sum[mi]);
                 }
 #pragma unroll
         for (unsigned ni = 0; ni < 2; ++ni) {
@@ -216,7 +216,7 @@ struct FewFourBits {
                 unsigned word;
                 if constexpr (WORDS == 1) word = held;
                 else word = held[i];
-                const v4u b = eight_weights<T>(word);
+                const v4u b = eight_weights<T, SIXTEENTHS>(word);
 #pragma unroll
                 for (int mi = 0; mi < MT; ++mi)
 #pragma unroll
@@ -229,8 +229,8 @@ struct FewFourBits {
                 for (int i = 0; i < 4; ++i) acc[mi][ni][i] = __builtin_fmaf(s[i], d[mi][i], acc[mi][ni][i]);
         }
     }
-    template <int MT>
-    __device__ __forceinline__ void sum(char *lds_w, char *lds_x, float *lds_s, bool in, v4f (&acc)[MT][2]) {
+    template <bool SIXTEENTHS, int MT>
+    __device__ __forceinline__ void sum_as(char *lds_w, char *lds_x, float *lds_s, bool in, v4f (&acc)[MT][2]) {
         constexpr unsigned kXBytes = kParts * MT * 16 * kRowBytes, kScales = kSteps * kColumns;
         const unsigned wave = wave_of_block(), lane = threadIdx.x % kLanes;
         Held<MT> next;
@@ -248,9 +248,50 @@ struct FewFourBits {
             if (k + kChunk < k_all) fetch(next, (NVSHMEM_AMD_LDS char *)lds_w + (buffer ^ 1) * Side::kBytes, k + kChunk, in);
 #pragma unroll
             for (unsigned j = 0; j < kSteps; ++j) {
-                multiply<MT>(j, lw, lx, ls, wave, lane, acc);
+                multiply<SIXTEENTHS, MT>(j, lw, lx, ls, wave, lane, acc);
                 __builtin_amdgcn_sched_barrier(0);  // (the compiler would gather all steps' reads, in registers for all)
             }
+        }
+    }
+    // Sums over 128 + q leave fp32 before those over q - 8 do (128 elements of one sign from 2^114 on), and an infinity meets its negative in
+    // them.  Once one has, it stays an infinity or a NaN.  So a block that has such a sum makes all of its sums again, of sixteenths, and takes
+    // those in place of what was not finite: an element's result is the same whatever rows it came with.
+    // us of one token on each of 8 PEs, 256 experts of 7168 x 2048, without / with: 225 / 227.
+    template <int MT>
+    __device__ __forceinline__ void sum(char *lds_w, char *lds_x, float *lds_s, bool in, v4f (&acc)[MT][2]) {
+        constexpr bool kSixteenths = sizeof(T) == 4;
+        sum_as<kSixteenths, MT>(lds_w, lds_x, lds_s, in, acc);
+        if constexpr (__is_same(T, __bf16)) {
+            float zero = 0.0f;  // (or a NaN)
+#pragma unroll
+            for (int mi = 0; mi < MT; ++mi)
+#pragma unroll
+                for (unsigned ni = 0; ni < 2; ++ni)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) zero = __builtin_fmaf(acc[mi][ni][i], 0.0f, zero);
+            const bool any = __any(zero != 0.0f);
+            __syncthreads();  // (all have multiplied the last chunk)
+            if (threadIdx.x % kLanes == 0) lds_s[wave_of_block()] = any ? 1.0f : 0.0f;
+            __syncthreads();
+            float blocks = 0.0f;
+#pragma unroll
+            for (unsigned w = 0; w < kWaves; ++w) blocks += lds_s[w];
+            if (__builtin_amdgcn_readfirstlane(__float_as_uint(blocks)) == 0) return;
+            __syncthreads();  // (all have read it)
+            v4f again[MT][2] = {};
+            sum_as<true, MT>(lds_w, lds_x, lds_s, in, again);
+#pragma unroll
+            for (int mi = 0; mi < MT; ++mi)
+#pragma unroll
+                for (unsigned ni = 0; ni < 2; ++ni)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[mi][ni][i] = acc[mi][ni][i] * 0.0f == 0.0f ? acc[mi][ni][i] : again[mi][ni][i] * 16.0f;
+        }
+        if constexpr (kSixteenths) {
+#pragma unroll
+            for (int mi = 0; mi < MT; ++mi)
+#pragma unroll
+                for (unsigned ni = 0; ni < 2; ++ni) acc[mi][ni] *= 16.0f;
         }
     }
 };
