@@ -224,11 +224,15 @@ struct TileSide {
                 const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, 0x7fffffff, 0x00020000);
                 const unsigned o = along[j] < left ? off[j] : kNowhere;
                 // Not the builtin: behind that, the compiler waits for all loads on their way to LDS in front of every read of it.
-                // The step's barrier waits for them instead.  (Four wait states: the buffer's words may come from v_readfirstlane.)
+                // The step's barrier waits for them instead.  (Five wait states: the buffer's words may come from v_readfirstlane.  m0 is
+                // named as changed: the compiler gives it to no variable, and says so, but may keep an address there for LDS.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
                 asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                              :
                              : "s"((unsigned)(uintptr_t)(lds + (wave * kMoves + j) * 1024)), "v"(o), "s"(rsrc)
-                             : "memory");
+                             : "memory", "m0");
+#pragma clang diagnostic pop
             } else {
                 const unsigned n = off[j] == kNowhere || along[j] >= left ? 0 : KM ? width[j] : (left - along[j] < N ? left - along[j] : N);
                 held[j] = chunk_load_front((const T *)(p + (n ? off[j] : 0)), n);
