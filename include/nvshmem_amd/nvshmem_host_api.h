@@ -383,20 +383,21 @@ NVSHMEMI_REPT_FOR_ALL_REDUCE_TYPES_AND_OPS(NVSHMEMI_DECL_TYPED_REDUCE_HOST)
  *   [gate | up] = x w_in[i]^T, h = gate * sigmoid(gate) * up, out = h w_out[i]^T, with w_in[i] of 2 hidden x dim (the rows of gate, then
  *   those of up) and w_out[i] of dim x hidden elements.  `rows`, `out` (and `pre`) have recv_cap_rows rows; those that no expert has are
  *   neither read nor written.  What expert_row holds beyond [0, recv_cap_rows] is cut off.  `pre`, 2 hidden elements a row, gets
- *   [gate | up] for moe_experts_grad, or is NULL.  h is rounded to T on its way from one product to the next.  dim and hidden are at most
- *   65536, experts at most 1024 and the same number on every PE.
+ *   [gate | up] for moe_experts_grad, or is NULL.  h is rounded to T on its way from one product to the next (of halves, to an infinity where it
+ *   is beyond 65504).  dim and hidden are at most 65536, experts at most 1024 and the same number on every PE.
  * <T>_moe_experts_grad: drows, dw_in and dw_out from dout, rows, weights and moe_experts' pre.  [dgate | dup] and h are rounded to T in
- *   between.  An expert without rows gets weights' gradients of zeros; rows of drows that no expert has are left as they were.
+ *   between, as h is in moe_experts.  An expert without rows gets weights' gradients of zeros; rows of drows that no expert has are left as they were.
  * <T>_moe_experts_w4: moe_experts with weights of 4 bits.  Element k of a row of w_in (of 2 hidden rows of dim) and w_out (dim rows of hidden)
  *   is (q - 8) * scale[row][k / group], q in the low half of byte k / 2 of the row for even k, in the high half for odd ones; rows are
  *   ceil(elements / 2) bytes and ceil(elements / group) scales of T long.  group is a multiple of 32.  The weights' values are taken as they
  *   are, without rounding to T.  Up to 128 products are added up in front of their scale, sixteenths of them in fp32: a row whose elements (or
- *   its h's) reach 2^121 may give infinities and NaN where the formula does not.  An infinity gives what the formula gives.  The workspace is
- *   moe_experts'.
+ *   its h's) reach 2^121 may give infinities and NaN where the formula does not, and what a float holds below 2^-133 may be lost.  An infinity
+ *   gives what the formula gives.  The workspace is moe_experts'.  There are no gradients through it.
  * <T>_dropout: out[e] = residual[e] + (keep(e) ? rows[e] / (1 - P) : 0) over the tokens * dim elements of a PE (residual NULL: zeros), with P
  *   the probability p, 0 <= p < 1, in steps of 2^-16.  keep follows from seed[0], seed[1] (the PE's own copy, e.g. a run's seed and a step's
  *   number, read when the kernel runs), the PE and e, by Philox4x32-10, and from nothing else: the gradient is the same call on dout without
- *   a residual.  What is dropped may be an infinity or a NaN.  out may be residual, or rows where there is no residual.
+ *   a residual, and calls with equal seeds drop the same elements, so that every layer needs one of its own.  What is dropped may be an
+ *   infinity or a NaN.  out may be residual, or rows where there is no residual.
  */
 #define NVSHMEMI_AMD_DECL_TOKENS(NAME, TYPE)                                                                              \
     NVSHMEMI_HOST_ONLY int nvshmemx_amd_##NAME##_embedding_on_stream(                                                     \
