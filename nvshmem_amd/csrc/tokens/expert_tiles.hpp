@@ -600,8 +600,9 @@ inline void launch_tiles_as(const ExpertArgs<T> &args, hipStream_t stream) {
     if (tiles) launch_kernel((expert_tile_kernel<T, OP, BM, BN, DMA>), dim3(tile_blocks(tiles, BN == 256 ? 1 : DMA || BM == 128 ? 2 : 3)), dim3(tile_wave_rows<BM>() * 256), 0, stream, args);
 }
 // Large tiles read the least, small ones waste less on experts of few rows, have more steps on their way to LDS at a time, and two blocks of
-// a compute unit, of which one multiplies while the other stores.  What an expert may have on average, `rows`, is all that the host knows
-// of the rows.  us of the forward pass, 256 x 256 / 128 x 128 / 64 x 128 / 32 x 128:
+// a compute unit, of which one multiplies while the other stores.  What an expert may have on average by the buffers' capacity, `rows`, is all
+// that the host knows of the rows, and what the limits are in.  In the following the rows are those that came; there is room for a quarter more
+// and for 64 a PE (of 12: 23, of 57 in all: 10 each, of 300: 383).  us of the forward pass, 256 x 256 / 128 x 128 / 64 x 128 / 32 x 128:
 //   bf16, 64 experts of 4096 x 1536 with 12 rows each - / 436 / 414 / 454, 40: - / 461 / 468 / 548; 57 rows for 64 experts of 7168 x 2048 - / 652 / 630 / 612;
 //   8 rows for 8 experts of 2048 x 1408, too few for the larger tiles to fill the GPU: - / 41.8 / 28.2 / 26.9;
 //   64 experts of 2048 x 1408 with 300 rows each 504 / 519, 600: 754 / 821; 32 of 7168 x 2048 with 180: 880 / 862, 600: 1776 / 1971.

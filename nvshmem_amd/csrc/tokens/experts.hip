@@ -4,7 +4,8 @@
 //
 // for the rows [expert_row[i], expert_row[i + 1]) of expert i.  Both input projections, the activation and the product are one
 // kernel; h goes through memory in the rows' type, rounded once, and is what the second kernel reads: the matrix cores take it in no
-// other.  us for bf16, 64 experts of 7168 x 2048: 131072 rows 9400 (1.23 PFLOP/s), 64 rows (3.7 GB of weights) 590 (6.3 TB/s).
+// other (a half beyond 65504 becomes an infinity there).  us for bf16, 64 experts of 7168 x 2048: 131072 rows 9250 to 9800
+// by board (1.18 to 1.25 PFLOP/s), 64 rows (3.7 GB of weights) 580 to 600 (6.1 to 6.4 TB/s).
 #include "expert_tiles.hpp"
 
 namespace nvshmem_amd {

@@ -5,8 +5,8 @@
 //   drows = [dgate | dup] W_in      dW_in = [dgate | dup]^T x      dW_out = dout^T h
 //
 // The first kernel makes dh in its accumulators and stores [dgate | dup] and h, in the rows' type, rounded once each: the matrix cores
-// take them in no other.  An expert without rows gets weights' gradients of zeros.  us for bf16, 65536 rows of 32 experts of 7168 x 2048: 10200 to 10800
-// (1.07 to 1.13 PFLOP/s; dh 2120, drows 3240, dw_in 3670, dw_out 1840).
+// take them in no other.  An expert without rows gets weights' gradients of zeros.  us for bf16, 65536 rows of 32 experts of 7168 x 2048: 10050 to 10800
+// by board (1.07 to 1.15 PFLOP/s; dh 1980, drows 3280 to 3350, dw_in 3640, dw_out 1840).
 #include "expert_tiles.hpp"
 
 namespace nvshmem_amd {
