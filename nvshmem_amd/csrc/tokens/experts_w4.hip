@@ -21,11 +21,12 @@ struct W4Args {
 
 // What x and a weight become for the matrix cores.  Of bfloat16 elements a weight is 128 + q, whose bits are those of 128 with q in the
 // mantissa: one operation for two weights.  The 136 that this is too much, times the sum of x, goes into the sums first, as a product with
-// too_much(); what the sums, in fp32, lose by it is some 2^-16 of the result where a row's elements are of one sign, and less where they are
-// not, far below the 2^-8 that the result is rounded to.  For a half, whose results have eight times the steps and whose bits would need 1024 in
-// 128's place, that does not hold: 1024 + q (64 + q of the next four bits) loses the 1032 (72) by one more operation for two weights, exactly.
-// An fp32 element is the sum of three bf16 ones, of 8 bits of its mantissa each, and weights are (q - 8) / 16: nothing of it above 2^-133, bf16's
-// least number, is lost in front of the sum.  us of 64 tokens on each of 8 PEs, halves, 256 experts of 7168 x 2048, groups of 64, by products with the 1032 and 72 and now: 1618 / 1641.
+// too_much().  What the sums, in fp32, lose by it is some 2^-17 of the sum of |x|, which x's own rounding to 2^-8 has long lost; 2^-16 of the result
+// where a row's elements are of one sign.  For a half, which is rounded to 2^-11 and whose bits would need 1024 in 128's place, that does not
+// hold: 1024 + q (64 + q of the next four bits) loses the 1032 (72) by one more operation for two weights, exactly.  An fp32 element is the sum of
+// three bf16 ones, of 8 bits of its mantissa each, and weights are (q - 8) / 16: nothing of it above 2^-133, bf16's least number, is lost in front
+// of the sum.
+// us of 64 tokens on each of 8 PEs, halves, 256 experts of 7168 x 2048, groups of 64, by products with the 1032 and 72 and now: 1618 / 1641.
 template <typename T>
 struct Nibble;
 template <>
